@@ -63,7 +63,8 @@ extern "C" {
  * 4: fused warp -> correlation, 5: fused flow upsample -> warp, corr into a slice,
  * 6: pwc_set_debug, 7: grouped warp / warp -> correlation launches, 8: one-launch warp
  * backward with a workspace, 9: pwc_corr_forward_plan, 10: pwc_corr_backward_plan,
- * 11: pwc_warp_corr_backward). */
+ * 11: pwc_warp_corr_backward, 12: the feature operators pwc_layer_norm_*, pwc_rotary,
+ * pwc_linear_*, pwc_gated_linear_*). */
 PWC_API int pwc_abi_version(void);
 
 /* Which kernel family pwc_corr_forward would launch for these arguments (the same dispatch
@@ -296,6 +297,93 @@ typedef struct {
 PWC_API int pwc_corr_forward_group(const pwc_corr_problem* problems, int count, int pad_size,
                                    int kernel_size, int max_displacement, int stride1,
                                    int stride2, int corr_multiply, int dtype, void* stream);
+
+/* ---- Feature operators: what a model puts between the feature pyramid and the correlation.
+ * They replace nothing in the reference.  A matrix of tokens and channels lies as
+ *   PWC_LAYOUT_MAP     x[B][C][P], the framework's feature maps (P = H * W); image n starts at
+ *                      x + n * x_stride elements (>= C * P)
+ *   PWC_LAYOUT_TOKENS  x[P][C] (B = 1); token m starts at x + m * x_stride elements (>= C)
+ * Only the first input may be strided that way; every other tensor is dense in the same layout.
+ * Weights, biases and activations share one `dtype`; sums, statistics and activations are fp32,
+ * every output is rounded once.  Any alignment of a pointer to its element type is accepted.
+ * Empty batches return 1 (weight gradients over no tokens are written as zeros). */
+#define PWC_LAYOUT_MAP 0
+#define PWC_LAYOUT_TOKENS 1
+
+/* `activation` arguments; negative_slope is LEAKY_RELU's */
+#define PWC_ACT_NONE 0
+#define PWC_ACT_RELU 1
+#define PWC_ACT_LEAKY_RELU 2
+#define PWC_ACT_SIGMOID 3
+#define PWC_ACT_TANH 4
+#define PWC_ACT_SILU 5
+#define PWC_ACT_GELU 6      /* z * Phi(z) */
+#define PWC_ACT_GELU_TANH 7 /* the tanh form */
+
+/* y = (x - mean) * rstd * weight + bias over the C channels of each token, rstd = 1 / sqrt(var +
+ * eps).  weight / bias may be NULL (ones / zeros).  mean, rstd: [B * P] fp32 for the backward
+ * pass, or both NULL.  y must not overlap x. */
+PWC_API int pwc_layer_norm_forward(const void* x, const void* weight, const void* bias, void* y,
+                                   void* mean, void* rstd, int layout, long long B, long long P,
+                                   int C, long long x_stride, float eps, int dtype, void* stream);
+/* grad_x, grad_weight, grad_bias (each may be NULL: not computed) from grad_out and the forward's
+ * mean / rstd.  Deterministic.  `workspace` is needed for the weight and bias gradients. */
+PWC_API size_t pwc_layer_norm_backward_workspace_size(int layout, long long B, long long P, int C,
+                                                      int dtype);
+PWC_API int pwc_layer_norm_backward(const void* x, const void* weight, const void* grad_out,
+                                    const void* mean, const void* rstd, void* grad_x,
+                                    void* grad_weight, void* grad_bias, int layout, long long B,
+                                    long long P, int C, long long x_stride, int dtype,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions: x[B][N][heads][D] at any strides.  Pair j < pairs of a head's channels --
+ * (j, pairs + j), or (2j, 2j + 1) with `interleaved` -- turns by the angle positions[b][n][axis[j]]
+ * * inv_freq[j] (computed in fp64); channels from 2 * pairs on are copied.  `inverse` turns back
+ * (the backward pass).  inv_freq: `pairs` doubles, axis: `pairs` int32 in [0, axes), device memory.
+ * positions NULL: token n stands at its raster place in grid[axes] (product = N) plus origin.
+ * y must not overlap x, except that y == x with equal strides turns in place. */
+typedef struct {
+  long long B, N;
+  int heads, D, pairs, axes;
+  int position_type; /* 0 fp32, 1 int32, 2 int64 */
+  int interleaved;
+  long long x_stride[4], y_stride[4]; /* of b, n, head, channel, in elements */
+  long long position_stride[3];       /* of b (0: shared), n, axis */
+  long long grid[4], origin[4];
+} pwc_rotary_shape;
+PWC_API int pwc_rotary(const void* x, void* y, const void* positions, const void* inv_freq,
+                       const void* axis, const pwc_rotary_shape* shape, int inverse, int dtype,
+                       void* stream);
+
+/* y = act(x weight^T + bias) + residual; weight [O][K], bias [O] or NULL, residual like y or
+ * NULL. */
+PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bias,
+                               const void* residual, void* y, int layout, long long B, long long P,
+                               int K, int O, long long x_stride, int activation,
+                               float negative_slope, int dtype, void* stream);
+/* grad_x, grad_weight, grad_bias (each may be NULL; grad_bias only with grad_weight).  The
+ * residual's gradient is grad_out itself.  Deterministic. */
+PWC_API size_t pwc_linear_backward_workspace_size(int layout, long long B, long long P, int K,
+                                                  int O, int activation, int dtype);
+PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* bias,
+                                const void* grad_out, void* grad_x, void* grad_weight,
+                                void* grad_bias, int layout, long long B, long long P, int K,
+                                int O, long long x_stride, int activation, float negative_slope,
+                                int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = act(x Wg^T + bg) * (x Wu^T + bu); weight [2 * O][K] = [Wg; Wu], bias [2 * O] or NULL. */
+PWC_API int pwc_gated_linear_forward(const void* x, const void* weight, const void* bias, void* y,
+                                     int layout, long long B, long long P, int K, int O,
+                                     long long x_stride, int activation, float negative_slope,
+                                     int dtype, void* stream);
+PWC_API size_t pwc_gated_linear_backward_workspace_size(int layout, long long B, long long P,
+                                                        int K, int O, int dtype);
+PWC_API int pwc_gated_linear_backward(const void* x, const void* weight, const void* bias,
+                                      const void* grad_out, void* grad_x, void* grad_weight,
+                                      void* grad_bias, int layout, long long B, long long P, int K,
+                                      int O, long long x_stride, int activation,
+                                      float negative_slope, int dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream);
 #ifdef __cplusplus
 }
 #endif

@@ -178,7 +178,7 @@ hipError_t add_inplace_f32(void* y, const void* x, size_t n, hipStream_t stream)
 
 extern "C" {
 
-int pwc_abi_version(void) { return 11; }
+int pwc_abi_version(void) { return 12; }
 
 int pwc_corr_forward_plan(const void* in1, const void* in2, const void* out, int B, int C, int H,
                           int W, int pad_size, int kernel_size, int max_displacement, int stride1,
@@ -853,6 +853,11 @@ int pwc_warp_corr_backward(const void* in1, const void* x2, const void* flow,
 }
 
 }  // extern "C"
+
+namespace pwc {
+int api_fail(const char* fn, const char* msg) { return fail(fn, msg); }
+int api_launch(const char* fn, hipError_t e) { return check_launch(fn, e); }
+}  // namespace pwc
 
 // ---- grouped correlation (independent problems; the bench's l2 + l3) ----
 // A problem the row-band kernel takes in a single call: model.py:24's configuration in fp32,

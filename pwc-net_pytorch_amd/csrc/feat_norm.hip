@@ -1,0 +1,580 @@
+// feat_norm.hip — layer norm over the channels of feature maps and tokens.
+//
+//   forward   mu = mean_c x,  r = 1 / sqrt(mean_c (x - mu)^2 + eps),  y = (x - mu) r w + b
+//   backward  with xh = (x - mu) r and h = w dy:
+//             dx = r (h - mean_c h - xh mean_c (h xh)),  dw = sum_m dy xh,  db = sum_m dy
+//
+// Both are bound by memory: one read of x (and dy), one write of y (dx).  A row's values stay in
+// registers between the statistics and the result, the variance is summed from x - mu (so a large
+// mean costs no digits), every sum is in 32 bits.  The weight's gradient is summed by each thread
+// for its own channels over the rows of a block that stays on its CU, then over the blocks in
+// their order: no atomics, the same sums each time.
+#include "feat_common.cuh"
+#include "feat_norm.cuh"
+
+namespace pwc {
+namespace feat {
+
+// V values from p at any alignment as floats, `n` of them there
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+  Pack<T, V> o;
+  __builtin_memcpy(&o, p, sizeof(o));
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = to_f32(o.v[e]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
+  Pack<T, V> o;
+#pragma unroll
+  for (int e = 0; e < V; ++e) o.v[e] = from_f32<T>(v[e]);
+  __builtin_memcpy(p, &o, sizeof(o));
+}
+
+// ------------------------------------------------------------------------------ tokens [M][C]
+// TPR threads share a row; each has NV vectors of V channels, TPR * V apart.
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+  v = lanes_sum<(TPR < 64 ? TPR : 64)>(v);
+  if constexpr (TPR > 64) {  // the whole block: waves joined through LDS
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TPR / 64; ++w) v += red[w];
+  }
+  return v;
+}
+
+template <typename T, int TPR, int NV, int V>
+__global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
+  __shared__ float red[4];
+  constexpr int RPB = 256 / TPR;
+  const int t = threadIdx.x % TPR;
+  const long long m = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const bool row = m < a.M;
+  const T* x = (const T*)a.x + (row ? m : 0) * a.x_stride;
+  float v[NV][V];
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * TPR + t) * V;
+    if (c < a.C) {
+      load_v<T, V>(x + c, v[k]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += v[k][e];
+    }
+  }
+  const float mu = row_sum<TPR>(s, red) / a.C;
+  s = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if ((k * TPR + t) * V < a.C)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k][e] -= mu;
+        s += v[k][e] * v[k][e];
+      }
+  const float r = 1.f / sqrtf(row_sum<TPR>(s, red) / a.C + a.eps);
+  if (!row) return;
+  if (a.mean && t == 0) {
+    a.mean[m] = mu;
+    a.rstd[m] = r;
+  }
+  T* y = (T*)a.y + m * a.C;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * TPR + t) * V;
+    if (c < a.C) {
+      float w[V], b[V];
+      if (a.w) load_v<T, V>((const T*)a.w + c, w);
+      if (a.b) load_v<T, V>((const T*)a.b + c, b);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * r * (a.w ? w[e] : 1.f) + (a.b ? b[e] : 0.f);
+      store_v<T, V>(y + c, v[k]);
+    }
+  }
+}
+
+template <typename T, int TPR, int NV, int V>
+__global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
+  extern __shared__ float lds[];
+  constexpr int RPB = 256 / TPR;
+  float* red = lds;
+  const int t = threadIdx.x % TPR;
+  float w[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * TPR + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      w[k][e] = 1.f;
+      dw[k][e] = db[k][e] = 0.f;
+    }
+    if (a.w && c < a.C) load_v<T, V>((const T*)a.w + c, w[k]);
+  }
+  for (long long m0 = (long long)blockIdx.x * RPB; m0 < a.M; m0 += (long long)gridDim.x * RPB) {
+    const long long m = m0 + threadIdx.x / TPR;
+    const bool row = m < a.M;
+    const T* x = (const T*)a.x + (row ? m : 0) * a.x_stride;
+    const T* dy = (const T*)a.dy + (row ? m : 0) * a.C;
+    const float mu = row ? a.mean[m] : 0.f, r = row ? a.rstd[m] : 0.f;
+    float xh[NV][V], h[NV][V];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + t) * V;
+      if (row && c < a.C) {
+        load_v<T, V>(x + c, xh[k]);
+        load_v<T, V>(dy + c, h[k]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          xh[k][e] = (xh[k][e] - mu) * r;
+          dw[k][e] += h[k][e] * xh[k][e];
+          db[k][e] += h[k][e];
+          h[k][e] *= w[k][e];
+          s1 += h[k][e];
+          s2 += h[k][e] * xh[k][e];
+        }
+      }
+    }
+    s1 = row_sum<TPR>(s1, red) / a.C;
+    s2 = row_sum<TPR>(s2, red) / a.C;
+    if (row && a.dx) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * TPR + t) * V;
+        if (c < a.C) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) h[k][e] = r * (h[k][e] - s1 - xh[k][e] * s2);
+          store_v<T, V>((T*)a.dx + m * a.C + c, h[k]);
+        }
+      }
+    }
+  }
+  if (!a.part) return;
+  // rows of the wave, then waves of the block, then [2][blocks][C]
+  float* acc = lds + 4;  // RPB > 1: [4][2][C]
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * TPR + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if constexpr (TPR < 64) {
+#pragma unroll
+        for (int o = TPR; o < 64; o <<= 1) {
+          dw[k][e] += __shfl_xor(dw[k][e], o, 64);
+          db[k][e] += __shfl_xor(db[k][e], o, 64);
+        }
+      }
+      if (c + e < a.C) {
+        if constexpr (RPB == 1) {
+          a.part[(long long)blockIdx.x * a.C + c + e] = dw[k][e];
+          a.part[((long long)gridDim.x + blockIdx.x) * a.C + c + e] = db[k][e];
+        } else if ((threadIdx.x & 63) < TPR) {
+          acc[(threadIdx.x >> 6) * 2 * a.C + c + e] = dw[k][e];
+          acc[((threadIdx.x >> 6) * 2 + 1) * a.C + c + e] = db[k][e];
+        }
+      }
+    }
+  }
+  if constexpr (RPB > 1) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * a.C; i += 256) {
+      const float v = acc[i] + acc[2 * a.C + i] + acc[4 * a.C + i] + acc[6 * a.C + i];
+      const int c = i < a.C ? i : i - a.C;
+      a.part[((long long)(i < a.C ? 0 : gridDim.x) + blockIdx.x) * a.C + c] = v;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ maps [B][C][P]
+// A block takes 64 pixels; wave g of G holds channels g, g + G, ... of them in registers.
+constexpr int kMapChannels = 16;  // of a thread; more channels (> 256) go by the loops below
+
+template <int G> __device__ __forceinline__ float pixel_sum(float v, float (*red)[64]) {
+  if constexpr (G > 1) {
+    const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
+    __syncthreads();
+    red[g][l] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) v += red[k][l];
+  }
+  return v;
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
+  __shared__ float red[G][64];
+  const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const long long tiles = (a.P + 63) / 64;
+  const long long img = blockIdx.x / tiles, p = blockIdx.x % tiles * 64 + l;
+  const bool ok = p < a.P;
+  const T* x = (const T*)a.x + img * a.x_stride + p;
+  float v[kMapChannels];
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMapChannels; ++k) {
+    const int c = k * G + g;
+    v[k] = ok && c < a.C ? to_f32(x[c * a.P]) : 0.f;
+    s += v[k];
+  }
+  const float mu = pixel_sum<G>(s, red) / a.C;
+  s = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMapChannels; ++k)
+    if (k * G + g < a.C) {
+      v[k] -= mu;
+      s += v[k] * v[k];
+    }
+  const float r = 1.f / sqrtf(pixel_sum<G>(s, red) / a.C + a.eps);
+  if (!ok) return;
+  if (a.mean && g == 0) {
+    a.mean[img * a.P + p] = mu;
+    a.rstd[img * a.P + p] = r;
+  }
+  T* y = (T*)a.y + img * a.C * a.P + p;
+#pragma unroll
+  for (int k = 0; k < kMapChannels; ++k) {
+    const int c = k * G + g;
+    if (c < a.C) {
+      const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
+      const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
+      y[c * a.P] = from_f32<T>(v[k] * r * w + b);
+    }
+  }
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
+  __shared__ float red[G][64];
+  const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const long long tiles = (a.P + 63) / 64;
+  float w[kMapChannels], dw[kMapChannels], db[kMapChannels];
+#pragma unroll
+  for (int k = 0; k < kMapChannels; ++k) {
+    const int c = k * G + g;
+    w[k] = a.w && c < a.C ? to_f32(((const T*)a.w)[c]) : 1.f;
+    dw[k] = db[k] = 0.f;
+  }
+  for (long long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
+    const long long img = t / tiles, p = t % tiles * 64 + l;
+    const bool ok = p < a.P;
+    const T* x = (const T*)a.x + img * a.x_stride + p;
+    const T* dy = (const T*)a.dy + img * a.C * a.P + p;
+    const float mu = ok ? a.mean[img * a.P + p] : 0.f, r = ok ? a.rstd[img * a.P + p] : 0.f;
+    float xh[kMapChannels], h[kMapChannels];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMapChannels; ++k) {
+      const int c = k * G + g;
+      const bool have = ok && c < a.C;
+      xh[k] = have ? (to_f32(x[c * a.P]) - mu) * r : 0.f;
+      h[k] = have ? to_f32(dy[c * a.P]) : 0.f;
+      dw[k] += h[k] * xh[k];
+      db[k] += h[k];
+      h[k] *= w[k];
+      s1 += h[k];
+      s2 += h[k] * xh[k];
+    }
+    s1 = pixel_sum<G>(s1, red) / a.C;
+    s2 = pixel_sum<G>(s2, red) / a.C;
+    if (ok && a.dx) {
+      T* dx = (T*)a.dx + img * a.C * a.P + p;
+#pragma unroll
+      for (int k = 0; k < kMapChannels; ++k) {
+        const int c = k * G + g;
+        if (c < a.C) dx[c * a.P] = from_f32<T>(r * (h[k] - s1 - xh[k] * s2));
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < kMapChannels; ++k) {
+    const int c = k * G + g;
+    if (c < a.C) {
+      const float sw = lanes_sum<64>(dw[k]), sb = lanes_sum<64>(db[k]);
+      if (l == 0) {
+        a.part[(long long)blockIdx.x * a.C + c] = sw;
+        a.part[((long long)gridDim.x + blockIdx.x) * a.C + c] = sb;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ any C
+// Rows longer than the registers are read again for each pass.  S threads share a row: a whole
+// block (tokens, S = 256), or one of 64 pixels' four threads (maps, S = 4).
+struct RowAt {
+  long long base, y, stride;  // first value in x, in y / dy / dx; between channels
+  long long m;
+  bool ok;
+};
+template <bool MAP> __device__ __forceinline__ RowAt row_at(const NormArgs& a) {
+  RowAt r;
+  if (MAP) {
+    const long long tiles = (a.P + 63) / 64, img = blockIdx.x / tiles;
+    const long long p = blockIdx.x % tiles * 64 + (threadIdx.x & 63);
+    r.ok = p < a.P;
+    r.base = img * a.x_stride + (r.ok ? p : 0);
+    r.y = img * a.C * a.P + (r.ok ? p : 0);
+    r.stride = a.P;
+    r.m = img * a.P + p;
+  } else {
+    r.m = blockIdx.x;
+    r.ok = true;
+    r.base = r.m * a.x_stride;
+    r.y = r.m * a.C;
+    r.stride = 1;
+  }
+  return r;
+}
+template <bool MAP> __device__ __forceinline__ float any_sum(float v, float (*red)[64]) {
+  if (MAP) return pixel_sum<4>(v, red);
+  return row_sum<256>(v, red[0]);
+}
+
+template <typename T, bool MAP> __global__ __launch_bounds__(256) void norm_any(const NormArgs a) {
+  __shared__ float red[4][64];
+  const RowAt r = row_at<MAP>(a);
+  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x, S = MAP ? 4 : 256;
+  const T* x = (const T*)a.x + r.base;
+  float s = 0.f;
+  for (int c = first; c < a.C; c += S) s += to_f32(x[c * r.stride]);
+  const float mu = any_sum<MAP>(s, red) / a.C;
+  s = 0.f;
+  for (int c = first; c < a.C; c += S) {
+    const float d = to_f32(x[c * r.stride]) - mu;
+    s += d * d;
+  }
+  const float rs = 1.f / sqrtf(any_sum<MAP>(s, red) / a.C + a.eps);
+  if (!r.ok) return;
+  if (a.mean && first == 0) {
+    a.mean[r.m] = mu;
+    a.rstd[r.m] = rs;
+  }
+  T* y = (T*)a.y + r.y;
+  for (int c = first; c < a.C; c += S) {
+    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
+    const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
+    y[c * r.stride] = from_f32<T>((to_f32(x[c * r.stride]) - mu) * rs * w + b);
+  }
+}
+
+template <typename T, bool MAP>
+__global__ __launch_bounds__(256) void norm_any_dx(const NormArgs a) {
+  __shared__ float red[4][64];
+  const RowAt r = row_at<MAP>(a);
+  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x, S = MAP ? 4 : 256;
+  const T* x = (const T*)a.x + r.base;
+  const T* dy = (const T*)a.dy + r.y;
+  const float mu = r.ok ? a.mean[r.m] : 0.f, rs = r.ok ? a.rstd[r.m] : 0.f;
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = first; c < a.C; c += S) {
+    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
+    const float h = to_f32(dy[c * r.stride]) * w;
+    s1 += h;
+    s2 += h * (to_f32(x[c * r.stride]) - mu) * rs;
+  }
+  s1 = any_sum<MAP>(s1, red) / a.C;
+  s2 = any_sum<MAP>(s2, red) / a.C;
+  if (!r.ok) return;
+  T* dx = (T*)a.dx + r.y;
+  for (int c = first; c < a.C; c += S) {
+    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
+    const float xh = (to_f32(x[c * r.stride]) - mu) * rs;
+    dx[c * r.stride] = from_f32<T>(rs * (to_f32(dy[c * r.stride]) * w - s1 - xh * s2));
+  }
+}
+
+// dw, db of one channel over a share of the rows: tokens, a thread a channel; maps, a block
+template <typename T, bool MAP>
+__global__ __launch_bounds__(256) void norm_any_dw(const NormArgs a, int parts) {
+  __shared__ float red[4];
+  const long long part = blockIdx.y;
+  float sw = 0.f, sb = 0.f;
+  const long long c = MAP ? blockIdx.x : blockIdx.x * 256LL + threadIdx.x;
+  if (MAP) {
+    const long long lo = a.M * part / parts, hi = a.M * (part + 1) / parts;
+    for (long long m = lo + threadIdx.x; m < hi; m += 256) {
+      const long long img = m / a.P, p = m - img * a.P;
+      const float d = to_f32(((const T*)a.dy)[(img * a.C + c) * a.P + p]);
+      sw += d * (to_f32(((const T*)a.x)[img * a.x_stride + c * a.P + p]) - a.mean[m]) * a.rstd[m];
+      sb += d;
+    }
+    sw = row_sum<256>(sw, red);
+    sb = row_sum<256>(sb, red);
+    if (threadIdx.x != 0) return;
+  } else {
+    if (c >= a.C) return;
+    const long long lo = a.M * part / parts, hi = a.M * (part + 1) / parts;
+    for (long long m = lo; m < hi; ++m) {
+      const float d = to_f32(((const T*)a.dy)[m * a.C + c]);
+      sw += d * (to_f32(((const T*)a.x)[m * a.x_stride + c]) - a.mean[m]) * a.rstd[m];
+      sb += d;
+    }
+  }
+  a.part[part * a.C + c] = sw;
+  a.part[(parts + part) * a.C + c] = sb;
+}
+
+// dw, db: the blocks' sums [2][blocks][C] in their order; 32 channels by 32 shares of the blocks
+template <typename T>
+__global__ __launch_bounds__(1024) void norm_add_parts(const float* __restrict__ part,
+                                                       T* __restrict__ dw, T* __restrict__ db,
+                                                       int C, int blocks) {
+  __shared__ float red[32][33];
+  const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + l;
+  const float* p = part + (long long)blockIdx.y * blocks * C;
+  float s = 0.f;
+  if (c < C)
+    for (int b = g; b < blocks; b += 32) s += p[(long long)b * C + c];
+  red[g][l] = s;
+  __syncthreads();
+  if (g == 0 && c < C) {
+    for (int k = 1; k < 32; ++k) s += red[k][l];
+    T* out = blockIdx.y == 0 ? dw : db;
+    if (out) out[c] = from_f32<T>(s);
+  }
+}
+
+// ------------------------------------------------------------------------------ launches
+// Threads of a row and vectors of a thread for C channels in vectors of V: the fewest threads that
+// hold a row in 16 values each (32 where the whole block shares it), so that short rows share a
+// wave.  128, 1024 and 8192 channels end the three; 0 = too long.
+constexpr int most_values(int tpr) { return tpr == 256 ? 32 : 16; }
+struct RowPlan {
+  int tpr, nv;
+};
+static RowPlan row_plan(int C, int V) {
+  const int n = (C + V - 1) / V;
+  for (int tpr : {8, 64, 256})
+    for (int nv = 1; nv * V <= most_values(tpr); nv *= 2)
+      if (n <= tpr * nv) return {tpr, nv};
+  return {0, 0};
+}
+
+template <typename T> static bool vector_rows(const NormArgs& a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  return a.C % V == 0;
+}
+
+constexpr int kBlocksBackward = 1024;  // blocks that stay: four of 256 threads on each of 256 CUs
+
+int norm_parts(int layout, long long B, long long P, int C, int dtype) {
+  const long long M = layout == kMap ? B * P : P;
+  long long rows = 1;  // rows of a block's turn
+  if (layout == kMap) {
+    rows = 64;
+  } else {
+    const int V = dtype == 0 ? 4 : 8;
+    const RowPlan p = row_plan(C, C % V == 0 ? V : 1);
+    if (p.tpr) rows = 256 / p.tpr;
+  }
+  const long long n = (M + rows - 1) / rows;
+  return (int)(n < kBlocksBackward ? n : kBlocksBackward);
+}
+
+template <typename T, int TPR, int V, int NV = 1>
+static void tokens_nv(const NormArgs& a, int nv, bool back, int parts, hipStream_t s) {
+  if constexpr (NV * V <= most_values(TPR)) {
+    if (nv != NV) return tokens_nv<T, TPR, V, 2 * NV>(a, nv, back, parts, s);
+    const unsigned grid = (unsigned)((a.M + 256 / TPR - 1) / (256 / TPR));
+    const size_t lds = 16 + (TPR < 256 ? 8 * sizeof(float) * a.C : 0);
+    if (back)
+      norm_tokens_backward<T, TPR, NV, V><<<parts, 256, lds, s>>>(a);
+    else
+      norm_tokens<T, TPR, NV, V><<<grid, 256, 0, s>>>(a);
+  }
+}
+
+template <typename T> static bool tokens(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool vec = vector_rows<T>(a);
+  const RowPlan p = row_plan(a.C, vec ? V : 1);
+  if (p.tpr == 0) return false;
+  if (vec) {
+    p.tpr == 8    ? tokens_nv<T, 8, V>(a, p.nv, back, parts, s)
+    : p.tpr == 64 ? tokens_nv<T, 64, V>(a, p.nv, back, parts, s)
+                  : tokens_nv<T, 256, V>(a, p.nv, back, parts, s);
+  } else {
+    p.tpr == 8    ? tokens_nv<T, 8, 1>(a, p.nv, back, parts, s)
+    : p.tpr == 64 ? tokens_nv<T, 64, 1>(a, p.nv, back, parts, s)
+                  : tokens_nv<T, 256, 1>(a, p.nv, back, parts, s);
+  }
+  return true;
+}
+
+template <typename T> static bool map(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  if (a.C > 16 * kMapChannels) return false;
+  const unsigned grid = (unsigned)(a.B * ((a.P + 63) / 64));
+#define NORM_MAP(G)                                                        \
+  (back ? norm_map_backward<T, G><<<parts, 64 * G, 0, s>>>(a)              \
+        : norm_map<T, G><<<grid, 64 * G, 0, s>>>(a))
+  a.C <= kMapChannels       ? NORM_MAP(1)
+  : a.C <= 4 * kMapChannels ? NORM_MAP(4)
+  : a.C <= 8 * kMapChannels ? NORM_MAP(8)
+                            : NORM_MAP(16);
+#undef NORM_MAP
+  return true;
+}
+
+template <typename T> static hipError_t forward_t(const NormArgs& a, hipStream_t s) {
+  const bool is_map = a.layout == kMap;
+  if (is_map ? map<T>(a, false, 0, s) : tokens<T>(a, false, 0, s)) return hipGetLastError();
+  if (is_map)
+    norm_any<T, true><<<(unsigned)(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
+  else
+    norm_any<T, false><<<(unsigned)a.M, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T> static hipError_t backward_t(const NormArgs& a, int parts, hipStream_t s) {
+  const bool is_map = a.layout == kMap;
+  if (!(is_map ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s))) {
+    if (a.dx) {
+      if (is_map)
+        norm_any_dx<T, true><<<(unsigned)(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
+      else
+        norm_any_dx<T, false><<<(unsigned)a.M, 256, 0, s>>>(a);
+    }
+    if (a.part) {
+      if (is_map)
+        norm_any_dw<T, true><<<dim3(a.C, parts), 256, 0, s>>>(a, parts);
+      else
+        norm_any_dw<T, false><<<dim3((a.C + 255) / 256, parts), 256, 0, s>>>(a, parts);
+    }
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !a.part) return e;
+  norm_add_parts<T><<<dim3((a.C + 31) / 32, 2), 1024, 0, s>>>(a.part, (T*)a.dw, (T*)a.db, a.C,
+                                                             parts);
+  return hipGetLastError();
+}
+
+template <typename T> static hipError_t no_rows_t(const NormArgs& a, hipStream_t s) {
+  norm_add_parts<T><<<dim3((a.C + 31) / 32, 2), 1024, 0, s>>>(nullptr, (T*)a.dw, (T*)a.db, a.C, 0);
+  return hipGetLastError();
+}
+
+hipError_t norm_no_rows(const NormArgs& a, int dtype, hipStream_t s) {
+  return dtype == 0   ? no_rows_t<float>(a, s)
+         : dtype == 1 ? no_rows_t<__half>(a, s)
+                      : no_rows_t<__hip_bfloat16>(a, s);
+}
+hipError_t norm_forward(const NormArgs& a, int dtype, hipStream_t s) {
+  return dtype == 0   ? forward_t<float>(a, s)
+         : dtype == 1 ? forward_t<__half>(a, s)
+                      : forward_t<__hip_bfloat16>(a, s);
+}
+hipError_t norm_backward(const NormArgs& a, int parts, int dtype, hipStream_t s) {
+  return dtype == 0   ? backward_t<float>(a, parts, s)
+         : dtype == 1 ? backward_t<__half>(a, parts, s)
+                      : backward_t<__hip_bfloat16>(a, parts, s);
+}
+
+}  // namespace feat
+}  // namespace pwc

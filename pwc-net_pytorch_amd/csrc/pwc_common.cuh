@@ -162,6 +162,11 @@ int debug_knob(const char* name, int def);
 // (kernel, device): a process that launches on several devices sets it on each (capi.hip).
 hipError_t lds_limit(const void* kernel, int bytes);
 
+// The C entries' error convention (capi.hip): the thread's message is set, 0 is returned; a launch
+// that succeeded returns 1.
+int api_fail(const char* fn, const char* msg);
+int api_launch(const char* fn, hipError_t e);
+
 // XCD-aware bijective remap of a 1-D block id (cdna_hip_programming.md §5 "XCD swizzle must
 // be bijective"): consecutive logical tiles land on the same XCD (and L2), so neighbouring
 // tiles that re-read each other's halo rows hit the same L2.  Pure speed choice.

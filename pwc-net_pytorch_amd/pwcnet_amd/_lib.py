@@ -28,6 +28,8 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _Z = ctypes.c_size_t
 _IP = ctypes.POINTER(ctypes.c_int)
+_L = ctypes.c_longlong
+_F = ctypes.c_float
 
 
 class WarpCorrProblem(ctypes.Structure):
@@ -46,6 +48,15 @@ class CorrProblem(ctypes.Structure):
     """pwc_corr_problem (include/pwc_hotpath.h)."""
     _fields_ = [("in1", _P), ("in2", _P), ("out", _P), ("B", _I), ("C", _I), ("H", _I),
                 ("W", _I)]
+
+
+class RotaryShape(ctypes.Structure):
+    """pwc_rotary_shape (include/pwc_hotpath.h)."""
+    _fields_ = [("B", ctypes.c_longlong), ("N", ctypes.c_longlong), ("heads", _I), ("D", _I),
+                ("pairs", _I), ("axes", _I), ("position_type", _I), ("interleaved", _I),
+                ("x_stride", ctypes.c_longlong * 4), ("y_stride", ctypes.c_longlong * 4),
+                ("position_stride", ctypes.c_longlong * 3), ("grid", ctypes.c_longlong * 4),
+                ("origin", ctypes.c_longlong * 4)]
 
 
 SYMBOLS = {
@@ -80,8 +91,19 @@ SYMBOLS = {
     "pwc_corr_forward_into_workspace_size": (_Z, [_I] * 10),
     "pwc_corr_forward_into": (_I, [_P, _P, _P, ctypes.c_longlong, ctypes.c_float] + [_I] * 11
                               + [_P, _Z, _P]),
+    "pwc_layer_norm_forward": (_I, [_P] * 6 + [_I, _L, _L, _I, _L, _F, _I, _P]),
+    "pwc_layer_norm_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I]),
+    "pwc_layer_norm_backward": (_I, [_P] * 8 + [_I, _L, _L, _I, _L, _I, _P, _Z, _P]),
+    "pwc_rotary": (_I, [_P] * 5 + [ctypes.POINTER(RotaryShape), _I, _I, _P]),
+    "pwc_linear_forward": (_I, [_P] * 5 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P]),
+    "pwc_linear_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I, _I, _I]),
+    "pwc_linear_backward": (_I, [_P] * 7 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z, _P]),
+    "pwc_gated_linear_forward": (_I, [_P] * 4 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P]),
+    "pwc_gated_linear_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I, _I]),
+    "pwc_gated_linear_backward": (_I, [_P] * 7 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z,
+                                                  _P]),
 }
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _lock = threading.Lock()
 _lib = None

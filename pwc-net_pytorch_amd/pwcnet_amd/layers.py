@@ -4,14 +4,20 @@
 * ``WarpingLayer``    — modules.py:25-42 (ctor takes the reference's ``args`` namespace)
 * ``CostVolumeLayer`` — modules.py:45-74 (ctor reads ``args.search_range``)
 * ``WarpCorrelation`` — model.py:80-83 (warp, then correlation) as one module / one launch
+* ``layer_norm``, ``rotary``, ``linear``, ``gated_linear`` and their modules ``LayerNorm``,
+  ``RotaryPosition``, ``ChannelLinear``, ``GatedLinear``, ``FeatureBlock`` — the feature operators
+  (features.py; no counterpart in the reference)
 * ``get_grid``        — utils.py:3-8 (host-built normalised base grid, for API completeness;
   the HIP warp recomputes it in registers and never calls this)
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import nn
 
+from . import features as _features
 from . import library as _library  # registers torch.ops.pwcnet.* (traceable single nodes)
 from .ops import (CorrelationCatFunction, UpsampleWarpFunction, WarpCorrelationFunction)
 
@@ -142,6 +148,191 @@ class CostVolumeLayer(nn.Module):
 
     def forward(self, src, tgt):
         return _library.cost_volume(src, tgt, self.search_range)
+
+
+# ---------------------------------------------------------------------------------------
+# feature operators (features.py): functions and modules
+# ---------------------------------------------------------------------------------------
+def _traced(x):
+    """Tracers see one opaque torch.ops.pwcnet node; eager calls go straight to the kernels."""
+    return torch.compiler.is_compiling() or type(x) not in (torch.Tensor, nn.Parameter)
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=1):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the channels of each pixel of a map
+    [B, C, *spatial] (``channel_dim=1``) or of each token [..., C] (``channel_dim=-1``)."""
+    if _traced(x):
+        return _library.layer_norm(x, weight, bias, eps, channel_dim)[0]
+    if _wants_grad(x, weight, bias):
+        return _features.LayerNormFunction.apply(x, weight, bias, eps, channel_dim)
+    with _features._on(x):
+        return _features.layer_norm_forward(x, weight, bias, eps, channel_dim)[0]
+
+
+def rotary(x, inv_freq, axis, positions=None, grid=None, origin=None, interleaved=False):
+    """x [B, N, heads, D] with its channel pairs turned by position[axis[j]] * inv_freq[j]; see
+    ``features.rotary_forward``.  ``inv_freq`` and ``axis`` come from ``rotary_frequencies``."""
+    if positions is not None and positions.requires_grad:
+        raise ValueError("rotary: positions have no gradient")
+    if _traced(x):
+        grid = None if grid is None else list(grid)
+        origin = None if origin is None else list(origin)
+        return _library.rotary(x, inv_freq, axis, positions, grid, origin, interleaved, False)
+    if _wants_grad(x):
+        return _features.RotaryFunction.apply(x, inv_freq, axis, positions, grid, origin,
+                                              interleaved)
+    with _features._on(x):
+        return _features.rotary_forward(x, inv_freq, axis, positions, grid, origin, interleaved)
+
+
+def linear(x, weight, bias=None, residual=None, activation="none", negative_slope=0.1,
+           channel_dim=1):
+    """act(x W^T + bias) + residual over x's channels: on maps a 1x1 convolution with its
+    activation and skip in one kernel.  ``activation``: one of ``features.ACTIVATIONS``."""
+    activation = activation or "none"
+    if _traced(x):
+        return _library.linear(x, weight, bias, residual, activation, negative_slope, channel_dim)
+    if _wants_grad(x, weight, bias, residual):
+        return _features.LinearFunction.apply(x, weight, bias, residual, activation,
+                                              negative_slope, channel_dim)
+    with _features._on(x):
+        return _features.linear_forward(x, weight, bias, residual, activation, negative_slope,
+                                        channel_dim)
+
+
+def gated_linear(x, weight, bias=None, activation="silu", negative_slope=0.1, channel_dim=1):
+    """act(x Wg^T + bg) * (x Wu^T + bu) over x's channels, weight = [Wg; Wu]: both projections,
+    the activation and the product in one kernel."""
+    activation = activation or "none"
+    if _traced(x):
+        return _library.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
+    if _wants_grad(x, weight, bias):
+        return _features.GatedLinearFunction.apply(x, weight, bias, activation, negative_slope,
+                                                   channel_dim)
+    with _features._on(x):
+        return _features.gated_linear_forward(x, weight, bias, activation, negative_slope,
+                                              channel_dim)
+
+
+class LayerNorm(nn.Module):
+    """``layer_norm`` with a weight (ones) and, unless ``bias=False``, a bias (zeros)."""
+
+    def __init__(self, channels, eps=1e-5, bias=True, channel_dim=1):
+        super().__init__()
+        self.eps, self.channel_dim = eps, channel_dim
+        self.weight = nn.Parameter(torch.ones(channels))
+        self.bias = nn.Parameter(torch.zeros(channels)) if bias else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps, self.channel_dim)
+
+    def extra_repr(self):
+        return f"{self.weight.numel()}, eps={self.eps}, channel_dim={self.channel_dim}"
+
+
+class RotaryPosition(nn.Module):
+    """Rotary positions for maps [B, heads * D, *spatial] (``channel_dim=1``) or tokens
+    [B, N, heads, D] (``channel_dim=-1``).
+
+    ``sections``: channel pairs of each axis, the last spatial axis last; axes before the map's
+    own (a frame's time) are constants of the call's ``origin``.  Tokens need ``positions``."""
+
+    def __init__(self, sections, heads=1, base=10000.0, shared=False, interleaved=False,
+                 channel_dim=1):
+        super().__init__()
+        if channel_dim not in (1, -1):
+            raise ValueError(f"RotaryPosition: channel_dim {channel_dim} is neither 1 nor -1")
+        inv_freq, axis = _features.rotary_frequencies(sections, base, shared)
+        self.register_buffer("inv_freq", inv_freq, persistent=False)
+        self.register_buffer("axis", axis, persistent=False)
+        self.sections, self.heads = tuple(sections), heads
+        self.interleaved, self.channel_dim = interleaved, channel_dim
+
+    def _apply(self, fn, recurse=True):
+        # angles stay in 64 bits when the module is cast: only the device follows
+        kept = self.inv_freq
+        super()._apply(fn, recurse)
+        if self.inv_freq.dtype != torch.float64:
+            self.inv_freq = kept.to(self.inv_freq.device)
+        return self
+
+    def forward(self, x, positions=None, origin=None):
+        if self.channel_dim == -1:
+            return rotary(x, self.inv_freq, self.axis, positions, interleaved=self.interleaved)
+        spatial, axes = tuple(x.shape[2:]), len(self.sections)
+        if x.dim() < 3 or len(spatial) > axes or x.shape[1] % self.heads:
+            raise ValueError(f"RotaryPosition: map {tuple(x.shape)} for {axes} axes and "
+                             f"{self.heads} heads")
+        B, C = x.shape[:2]
+        n = math.prod(spatial)
+        v = x.reshape(B, self.heads, C // self.heads, n).permute(0, 3, 1, 2)
+        grid = None if positions is not None else (1,) * (axes - len(spatial)) + spatial
+        y = rotary(v, self.inv_freq, self.axis, positions, grid, origin, self.interleaved)
+        return y.permute(0, 2, 3, 1).reshape(x.shape)
+
+    def extra_repr(self):
+        return f"{self.sections}, heads={self.heads}, channel_dim={self.channel_dim}"
+
+
+class ChannelLinear(nn.Module):
+    """``linear`` with its weight [out, in] and bias; on maps a 1x1 convolution."""
+
+    def __init__(self, in_channels, out_channels, bias=True, activation="none",
+                 negative_slope=0.1, channel_dim=1):
+        super().__init__()
+        self.activation, self.negative_slope = activation, negative_slope
+        self.channel_dim = channel_dim
+        self.weight = nn.Parameter(torch.empty(out_channels, in_channels))
+        nn.init.xavier_uniform_(self.weight)
+        self.bias = nn.Parameter(torch.zeros(out_channels)) if bias else None
+
+    def forward(self, x, residual=None):
+        return linear(x, self.weight, self.bias, residual, self.activation, self.negative_slope,
+                      self.channel_dim)
+
+    def extra_repr(self):
+        return f"{self.weight.shape[1]}, {self.weight.shape[0]}, activation={self.activation!r}"
+
+
+class GatedLinear(nn.Module):
+    """``gated_linear`` with its weight [gate; up] of 2 * hidden rows and bias."""
+
+    def __init__(self, in_channels, hidden_channels, bias=True, activation="silu",
+                 negative_slope=0.1, channel_dim=1):
+        super().__init__()
+        self.activation, self.negative_slope = activation, negative_slope
+        self.channel_dim = channel_dim
+        self.weight = nn.Parameter(torch.empty(2 * hidden_channels, in_channels))
+        for half in self.weight.chunk(2):
+            nn.init.xavier_uniform_(half)
+        self.bias = nn.Parameter(torch.zeros(2 * hidden_channels)) if bias else None
+
+    def forward(self, x):
+        return gated_linear(x, self.weight, self.bias, self.activation, self.negative_slope,
+                            self.channel_dim)
+
+    def extra_repr(self):
+        return (f"{self.weight.shape[1]}, {self.weight.shape[0] // 2}, "
+                f"activation={self.activation!r}")
+
+
+class FeatureBlock(nn.Module):
+    """x + project(gated(norm(x))) over the channels of a map: three kernels forward, the skip in
+    the last one's epilogue."""
+
+    def __init__(self, channels, hidden_channels=None, activation="silu", channel_dim=1):
+        super().__init__()
+        hidden = hidden_channels or 2 * channels
+        self.norm = LayerNorm(channels, channel_dim=channel_dim)
+        self.gated = GatedLinear(channels, hidden, activation=activation, channel_dim=channel_dim)
+        self.project = ChannelLinear(hidden, channels, channel_dim=channel_dim)
+
+    def forward(self, x):
+        return self.project(self.gated(self.norm(x)), residual=x)
 
 
 def get_grid(x: torch.Tensor) -> torch.Tensor:

@@ -11,17 +11,19 @@ trace ``Correlation``, ``WarpingLayer`` and ``CostVolumeLayer`` as single nodes:
     torch.ops.pwcnet.correlation_backward(in1, in2, gO, pad, ...)      cu:108-290
     torch.ops.pwcnet.cost_volume(src, tgt, sr) / _backward             modules.py:53-74
     torch.ops.pwcnet.warp(x, flow) / warp_backward                     modules.py:31-42
+    torch.ops.pwcnet.layer_norm / rotary / linear / gated_linear       (features.py)
 
 The real implementations are the HIP kernels behind the C ABI (ops.py); there is no CPU
 kernel, so calling these ops on CPU tensors raises, as the reference's CPU stubs did.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 
+from . import features as _features
 from . import ops as _ops
 
 _NS = "pwcnet"
@@ -174,3 +176,173 @@ def _warp_bwd(ctx, grad):
 
 
 warp.register_autograd(_warp_bwd, setup_context=_warp_setup)
+
+
+# ---------------------------------------------------------------------------------------
+# feature operators (features.py)
+# ---------------------------------------------------------------------------------------
+def _tokens(x, channel_dim):
+    n = 1
+    for d, size in enumerate(x.shape):
+        if d != channel_dim % x.dim():
+            n = n * size
+    return n
+
+
+@torch.library.custom_op(f"{_NS}::layer_norm", mutates_args=())
+def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+               channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y, mean, rstd)"""
+    with _on(x):
+        return _features.layer_norm_forward(x, weight, bias, eps, channel_dim, stats=True)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps, channel_dim):
+    n = _tokens(x, channel_dim)
+    return (x.new_empty(x.shape), x.new_empty((n,), dtype=torch.float32),
+            x.new_empty((n,), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::layer_norm_backward", mutates_args=())
+def layer_norm_backward(x: Tensor, weight: Optional[Tensor], grad: Tensor, mean: Tensor,
+                        rstd: Tensor, channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
+    with _on(x):
+        return _features.layer_norm_backward(x, weight, grad, mean, rstd, channel_dim)
+
+
+@layer_norm_backward.register_fake
+def _(x, weight, grad, mean, rstd, channel_dim):
+    C = x.shape[channel_dim]
+    return x.new_empty(x.shape), x.new_empty((C,)), x.new_empty((C,))
+
+
+def _norm_setup(ctx, inputs, output):
+    x, weight, bias, eps, ctx.channel_dim = inputs
+    ctx.has = (weight is not None, bias is not None)
+    ctx.save_for_backward(x, weight, output[1], output[2])
+
+
+def _norm_bwd(ctx, grad, grad_mean, grad_rstd):
+    x, weight, mean, rstd = ctx.saved_tensors
+    gx, gw, gb = layer_norm_backward(x, weight, grad.contiguous(), mean, rstd, ctx.channel_dim)
+    return gx, gw if ctx.has[0] else None, gb if ctx.has[1] else None, None, None
+
+
+layer_norm.register_autograd(_norm_bwd, setup_context=_norm_setup)
+
+
+@torch.library.custom_op(f"{_NS}::rotary", mutates_args=())
+def rotary(x: Tensor, inv_freq: Tensor, axis: Tensor, positions: Optional[Tensor],
+           grid: Optional[List[int]], origin: Optional[List[int]], interleaved: bool,
+           inverse: bool) -> Tensor:
+    with _on(x):
+        return _features.rotary_forward(x, inv_freq, axis, positions, grid, origin, interleaved,
+                                        inverse)
+
+
+@rotary.register_fake
+def _(x, inv_freq, axis, positions, grid, origin, interleaved, inverse):
+    return torch.empty_like(x)
+
+
+def _rotary_setup(ctx, inputs, output):
+    x, inv_freq, axis, positions, *ctx.args = inputs
+    ctx.save_for_backward(inv_freq, axis, positions)
+
+
+def _rotary_bwd(ctx, grad):
+    inv_freq, axis, positions = ctx.saved_tensors
+    grid, origin, interleaved, inverse = ctx.args
+    g = rotary(grad, inv_freq, axis, positions, grid, origin, interleaved, not inverse)
+    return (g,) + (None,) * 7
+
+
+rotary.register_autograd(_rotary_bwd, setup_context=_rotary_setup)
+
+
+def _product_fake(x, weight, channel_dim, halves):
+    shape = list(x.shape)
+    shape[channel_dim] = weight.shape[0] // halves
+    return x.new_empty(shape)
+
+
+@torch.library.custom_op(f"{_NS}::linear", mutates_args=())
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
+           activation: str, negative_slope: float, channel_dim: int) -> Tensor:
+    with _on(x):
+        return _features.linear_forward(x, weight, bias, residual, activation, negative_slope,
+                                        channel_dim)
+
+
+@linear.register_fake
+def _(x, weight, bias, residual, activation, negative_slope, channel_dim):
+    return _product_fake(x, weight, channel_dim, 1)
+
+
+@torch.library.custom_op(f"{_NS}::linear_backward", mutates_args=())
+def linear_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], grad: Tensor,
+                    activation: str, negative_slope: float,
+                    channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
+    with _on(x):
+        return _features.linear_backward(x, weight, bias, grad, activation, negative_slope,
+                                         channel_dim)
+
+
+@torch.library.custom_op(f"{_NS}::gated_linear", mutates_args=())
+def gated_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: str,
+                 negative_slope: float, channel_dim: int) -> Tensor:
+    with _on(x):
+        return _features.gated_linear_forward(x, weight, bias, activation, negative_slope,
+                                              channel_dim)
+
+
+@gated_linear.register_fake
+def _(x, weight, bias, activation, negative_slope, channel_dim):
+    return _product_fake(x, weight, channel_dim, 2)
+
+
+@torch.library.custom_op(f"{_NS}::gated_linear_backward", mutates_args=())
+def gated_linear_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], grad: Tensor,
+                          activation: str, negative_slope: float,
+                          channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
+    with _on(x):
+        return _features.gated_linear_backward(x, weight, bias, grad, activation, negative_slope,
+                                               channel_dim)
+
+
+def _product_backward_fake(x, weight, *args):
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+            weight.new_empty((weight.shape[0],)))
+
+
+linear_backward.register_fake(_product_backward_fake)
+gated_linear_backward.register_fake(_product_backward_fake)
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, *ctx.args = inputs
+    ctx.has = (bias is not None, residual is not None)
+    ctx.save_for_backward(x, weight, bias)
+
+
+def _linear_bwd(ctx, grad):
+    x, weight, bias = ctx.saved_tensors
+    gx, gw, gb = linear_backward(x, weight, bias, grad.contiguous(), *ctx.args)
+    return (gx, gw, gb if ctx.has[0] else None, grad if ctx.has[1] else None, None, None, None)
+
+
+def _gated_setup(ctx, inputs, output):
+    x, weight, bias, *ctx.args = inputs
+    ctx.has_bias = bias is not None
+    ctx.save_for_backward(x, weight, bias)
+
+
+def _gated_bwd(ctx, grad):
+    x, weight, bias = ctx.saved_tensors
+    gx, gw, gb = gated_linear_backward(x, weight, bias, grad.contiguous(), *ctx.args)
+    return gx, gw, gb if ctx.has_bias else None, None, None, None
+
+
+linear.register_autograd(_linear_bwd, setup_context=_linear_setup)
+gated_linear.register_autograd(_gated_bwd, setup_context=_gated_setup)
