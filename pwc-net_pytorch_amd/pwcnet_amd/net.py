@@ -19,6 +19,10 @@ fused forms: ``UpsampleWarp`` (model.py:78 + :80 in one launch) and, for the GPU
 Correlation, ``CorrelationCat`` (model.py:83-91: the correlation written into the cat
 buffer, leaky_relu fused).  Returns ``(flows, summaries)`` as model.py does.
 
+``feature_blocks`` and ``feature_rotary`` (off by default; no counterpart in the reference) refine
+both frames' pyramid features before the warp: ``FeatureBlock``s mix the channels of each pixel, and
+rotary positions in (frame, y, x) make the correlation's dot product tell displacements apart.
+
 Reference: model.py:11-115, modules.py:11-22 (conv), :77-99 (FeaturePyramidExtractor),
 :102-128 (OpticalFlowEstimator), :131-160 (ContextNetwork); defaults main.py:42-81.
 """
@@ -30,8 +34,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .layers import (Correlation, CorrelationCat, CostVolumeLayer, UpsampleWarp,
-                     WarpingLayer)
+from .layers import (Correlation, CorrelationCat, CostVolumeLayer, FeatureBlock, RotaryPosition,
+                     UpsampleWarp, WarpingLayer)
 
 
 @dataclass
@@ -49,6 +53,8 @@ class NetArgs:
     corr: str = "cost_volume"        # anything but 'CostVolumeLayer' -> Correlation (model.py:21)
     corr_activation: bool = False
     device: str = "cuda"
+    feature_blocks: int = 0          # FeatureBlocks on each level's features of both frames
+    feature_rotary: bool = False     # rotary positions (frame, y, x) on them
 
 
 def conv(batch_norm, in_planes, out_planes, kernel_size=3, stride=1):
@@ -152,6 +158,30 @@ class Net(nn.Module):
                     nn.init.uniform_(m.bias)
                 nn.init.xavier_uniform_(m.weight)
 
+        self.feature_refiners, self.feature_rotaries = [], []  # by level, coarsest first
+        for l, ch in enumerate(args.lv_chs[::-1][:args.output_level + 1]):
+            if args.feature_blocks:
+                layer = nn.Sequential(*(FeatureBlock(ch) for _ in range(args.feature_blocks)))
+                self.add_module(f"FeatureBlocks(Lv{l})", layer)
+                self.feature_refiners.append(layer)
+            if args.feature_rotary:
+                pairs = ch // 2  # a quarter for the frame, the rest for y and x
+                t = pairs // 4
+                y = (pairs - t) // 2
+                layer = RotaryPosition((t, y, pairs - t - y))
+                self.add_module(f"FeatureRotary(Lv{l})", layer)
+                self.feature_rotaries.append(layer)
+
+    def refine(self, pyramid, frame: int):
+        """The pyramid's features (coarsest first) of frame 0 or 1 through the level's blocks and
+        rotary positions; the pyramid itself where neither is built."""
+        for layers, extra in ((self.feature_refiners, {}),
+                              (self.feature_rotaries, {"origin": (frame, 0, 0)})):
+            if layers:
+                pyramid = ([m(x, **extra) for m, x in zip(layers, pyramid)]
+                           + list(pyramid[len(layers):]))
+        return pyramid
+
     def forward(self, x, fused: bool = True):
         args = self.args
         if args.input_norm:
@@ -159,8 +189,8 @@ class Net(nn.Module):
             x = (x - mean.view(x.size()[:2] + (1, 1, 1))) / args.rgb_max
         x1_raw = x[:, :, 0].contiguous()
         x2_raw = x[:, :, 1].contiguous()
-        x1_pyr = self.feature_pyramid_extractor(x1_raw) + [x1_raw]
-        x2_pyr = self.feature_pyramid_extractor(x2_raw) + [x2_raw]
+        x1_pyr = self.refine(self.feature_pyramid_extractor(x1_raw), 0) + [x1_raw]
+        x2_pyr = self.refine(self.feature_pyramid_extractor(x2_raw), 1) + [x2_raw]
         cat_fused = fused and isinstance(self.corr, Correlation)
 
         flows, summaries = [], {"x2_warps": []}

@@ -213,3 +213,17 @@ def test_traced_as_single_nodes():
         assert P.linear(x.reshape(-1, 8), w, channel_dim=-1).shape == (60, 12)
         assert P.RotaryPosition((2, 2))(x).shape == x.shape
         assert P.FeatureBlock(8)(x).shape == x.shape
+
+
+def test_net_is_unchanged_without_refined_features():
+    from pwcnet_amd.net import Net, NetArgs
+    torch.manual_seed(5)
+    a = Net(NetArgs())
+    torch.manual_seed(5)
+    b = Net(NetArgs(feature_blocks=1, feature_rotary=True))
+    extra = set(b.state_dict()) - set(a.state_dict())
+    assert len(extra) == 5 * 6 and all(k.startswith("FeatureBlocks(Lv") for k in extra)
+    assert all(torch.equal(v, b.state_dict()[k]) for k, v in a.state_dict().items())
+    assert a.refine([1, 2], 0) == [1, 2]
+    assert [m.sections for m in b.feature_rotaries] == [
+        (24, 36, 36), (16, 24, 24), (12, 18, 18), (8, 12, 12), (4, 6, 6)]

@@ -776,3 +776,42 @@ def test_compiled_node_matches_eager():
         assert torch.equal(a, c)
         assert torch.equal(torch.autograd.grad(a, leaf, grad)[0],
                            torch.autograd.grad(c, leaf, grad)[0])
+
+
+def test_net_with_refined_features():
+    """Net's refined pyramid against the formula in 64 bits (2e-6 by norms, as the block above), and
+    a forward and backward pass through all of it."""
+    from pwcnet_amd.net import Net, NetArgs
+    torch.manual_seed(3)
+    args = NetArgs(feature_blocks=2, feature_rotary=True)
+    net = Net(args).to(DEV)
+    gen = _gen("net")
+    pyr = [_rand(gen, 2, c, 2 << i, 3 << i) for i, c in enumerate(args.lv_chs[::-1])]
+    with torch.no_grad():
+        got = net.refine(pyr, 1)
+    assert len(got) == 6 and got[5] is pyr[5]  # beyond the output level
+    for l, (x, y) in enumerate(zip(pyr[:5], got)):
+        t = _tok(x.double(), True)
+        for blk in net.feature_refiners[l]:
+            q = {n: p.detach().double() for n, p in blk.named_parameters()}
+            d = t - t.mean(1, keepdim=True)
+            h = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-5) * q["norm.weight"]
+            z = (h + q["norm.bias"]) @ q["gated.weight"].t() + q["gated.bias"]
+            n = z.shape[1] // 2
+            h = z[:, :n] * torch.sigmoid(z[:, :n]) * z[:, n:]
+            t = t + h @ q["project.weight"].t() + q["project.bias"]
+        rot = net.feature_rotaries[l]
+        H, W = x.shape[2:]
+        n = torch.arange(H * W, device=DEV)
+        at = torch.stack((torch.ones_like(n), n // W, n % W), -1)[None]
+        ref, _ = _rotary64(t.view(2, H * W, 1, -1), rot.inv_freq, rot.axis, at, False)
+        ref = ref[:, :, 0].movedim(1, 2).reshape(x.shape)
+        assert ((y.double() - ref).norm() / ref.norm()).item() < 2e-6
+    # 128 x 128 is the least: at 64 x 64 the coarsest level is one pixel, where the warp's
+    # flow / ((W - 1) / 2) is 0 / 0 whatever the features are
+    x = torch.rand(1, 3, 2, 128, 128, generator=gen).to(DEV)
+    flows, _ = net(x)
+    sum(f.square().mean() for f in flows).backward()
+    for name, p in net.named_parameters():
+        if name.startswith("FeatureBlocks"):
+            assert torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, name
