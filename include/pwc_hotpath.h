@@ -361,8 +361,8 @@ PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bi
                                const void* residual, void* y, int layout, long long B, long long P,
                                int K, int O, long long x_stride, int activation,
                                float negative_slope, int dtype, void* stream);
-/* grad_x, grad_weight, grad_bias (each may be NULL; grad_bias only with grad_weight).  The
- * residual's gradient is grad_out itself.  Deterministic. */
+/* grad_x, grad_weight, grad_bias (each may be NULL: not computed).  The residual's
+ * gradient is grad_out itself.  Deterministic. */
 PWC_API size_t pwc_linear_backward_workspace_size(int layout, long long B, long long P, int K,
                                                   int O, int activation, int dtype);
 PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* bias,

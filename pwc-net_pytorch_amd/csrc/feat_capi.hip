@@ -80,15 +80,13 @@ ProductArgs forward_args(const Problem& p, const void* x, const void* w, const v
     g.b = x, g.ldb = p.x_stride, g.b_k = 1, g.J = (int)p.M;
     g.ldo = out_rows;
     g.ldother = p.O;
-    g.bias_i = 1;
-    g.pair_side = p.gated ? 1 : 0;
+    g.channel_i = 1;
   } else {
     g.a = x, g.lda = p.P, g.a_batch = p.x_stride, g.a_k = 0, g.I = (int)p.P;
     g.b = w, g.ldb = p.K, g.b_k = 1, g.J = p.rows;
     g.batches = (int)p.B;
     g.ldo = p.P, g.out_batch = (long long)out_rows * p.P;
     g.ldother = p.P, g.other_batch = (long long)p.O * p.P;
-    g.pair_side = p.gated ? 2 : 0;
   }
   return g;
 }
@@ -97,25 +95,37 @@ bool needs_z(const Problem& p) { return p.gated || p.act != kActNone; }
 size_t elem(int dtype) { return dtype == 0 ? 4 : 2; }
 
 struct BackwardSpace {
-  size_t dz, part, sums, total;  // bytes from the start
-  int splits;
+  size_t part, sums, total;  // bytes from the start; dz lies at 0
+  int splits, rows;          // rows of partial bias gradients
 };
-BackwardSpace backward_space(const Problem& p) {
+ProductArgs dz_args(const Problem& p, const void* x, const void* w, const void* bias,
+                    const void* dy, void* dz) {
+  return forward_args(p, x, w, bias, dy, dz, p.gated ? kGatedDz : kLinearDz, p.rows);
+}
+// The pointers matter for their alignment alone: without them the larger space.
+BackwardSpace backward_space(const Problem& p, const void* x, const void* w) {
   BackwardSpace s = {};
   s.splits = p.layout == PWC_LAYOUT_MAP
                  ? product_splits(p.K, p.rows, (int)p.B, p.P, p.dtype)
                  : product_splits(p.K, p.rows, 1, p.M, p.dtype);
+  s.rows = needs_z(p) ? product_sum_rows(dz_args(p, x, w, nullptr, nullptr, nullptr), p.dtype)
+                      : product_column_parts(p.layout, p.B, p.P, p.rows);
   s.part = needs_z(p) ? align256((size_t)p.M * p.rows * elem(p.dtype)) : 0;
-  s.sums = s.part + align256((size_t)s.splits * p.rows * p.K * 4);
-  s.total = s.sums + align256((size_t)s.splits * p.rows * 4);
+  s.sums = s.part + (s.splits > 1 ? align256((size_t)s.splits * p.rows * p.K * 4) : 0);
+  s.total = s.sums + align256((size_t)s.rows * p.rows * 4);
   return s;
+}
+size_t most_backward_space(const Problem& p) {
+  if (bad_problem(p) || p.M == 0) return 0;
+  const size_t a = backward_space(p, nullptr, nullptr).total;
+  const size_t b = backward_space(p, (const void*)1, (const void*)1).total;
+  return a > b ? a : b;
 }
 
 int product_backward(const char* fn, const Problem& p, const void* x, const void* w,
                      const void* bias, const void* dy, void* dx, void* dw, void* db,
                      void* workspace, size_t bytes, hipStream_t stream) {
   if (const char* e = bad_problem(p)) return api_fail(fn, e);
-  if (db && !dw) return api_fail(fn, "the bias gradient comes with the weight gradient");
   if (p.M == 0) {  // sums over no tokens
     hipError_t e = hipSuccess;
     if (dw) e = product_add_splits(nullptr, dw, (long long)p.rows * p.K, 0, p.dtype, stream);
@@ -123,14 +133,14 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     return api_launch(fn, e);
   }
   if (!x || !w || !dy) return api_fail(fn, "null buffer");
-  if (!dx && !dw) return api_launch(fn, hipSuccess);
-  const BackwardSpace s = backward_space(p);
+  if (!dx && !dw && !db) return api_launch(fn, hipSuccess);
+  const BackwardSpace s = backward_space(p, x, w);
   if (!workspace || bytes < s.total) return api_fail(fn, "workspace too small");
   char* ws = (char*)workspace;
   const void* dz = dy;
   if (needs_z(p)) {
-    const ProductArgs g = forward_args(p, x, w, bias, dy, ws, p.gated ? kGatedDz : kLinearDz,
-                                       p.rows);
+    ProductArgs g = dz_args(p, x, w, bias, dy, ws);
+    g.sums = db ? (float*)(ws + s.sums) : nullptr;
     const hipError_t e = product_launch(g, p.dtype, stream);
     if (e != hipSuccess) return api_launch(fn, e);
     dz = ws;
@@ -140,7 +150,7 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     ProductArgs g = blank();
     g.K = p.rows;
     g.out = dx;
-    g.mode = kLinear;
+    g.mode = kPlain;
     if (p.layout == PWC_LAYOUT_TOKENS) {
       g.a = w, g.lda = p.K, g.a_k = 0, g.I = p.K;
       g.b = dz, g.ldb = p.rows, g.b_k = 1, g.J = (int)p.M;
@@ -158,10 +168,10 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     ProductArgs g = blank();
     g.mode = kPartial;
     g.splits = s.splits;
-    g.out = ws + s.part;
-    g.sums = db ? (float*)(ws + s.sums) : nullptr;
+    g.out = s.splits > 1 ? (void*)(ws + s.part) : dw;
     g.I = p.K;
     g.J = p.rows;
+    g.ldo = p.K;
     if (p.layout == PWC_LAYOUT_TOKENS) {
       g.K = (int)p.M;
       g.a = x, g.lda = p.x_stride, g.a_k = 0;
@@ -173,11 +183,17 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
       g.b = dz, g.ldb = p.P, g.b_segment = dz_image, g.b_k = 1;
     }
     hipError_t e = product_launch(g, p.dtype, stream);
-    if (e == hipSuccess)
+    if (e == hipSuccess && s.splits > 1)
       e = product_add_splits((const float*)(ws + s.part), dw, (long long)p.rows * p.K, s.splits,
                              p.dtype, stream);
-    if (e == hipSuccess && db)
-      e = product_add_splits(g.sums, db, p.rows, s.splits, p.dtype, stream);
+    if (e != hipSuccess) return api_launch(fn, e);
+  }
+  if (db) {
+    float* sums = (float*)(ws + s.sums);
+    hipError_t e = hipSuccess;
+    if (!needs_z(p))
+      e = product_column_sums(dy, sums, p.layout, p.B, p.P, p.rows, s.rows, p.dtype, stream);
+    if (e == hipSuccess) e = sum_rows(sums, db, p.rows, s.rows, p.dtype, stream);
     if (e != hipSuccess) return api_launch(fn, e);
   }
   return api_launch(fn, hipSuccess);
@@ -336,7 +352,7 @@ PWC_API size_t pwc_linear_backward_workspace_size(int layout, long long B, long 
                                                   int O, int activation, int dtype) {
   const Problem p = problem(layout, B, P, K, O, layout == PWC_LAYOUT_MAP ? P * K : K, activation,
                             0.f, dtype, 0);
-  return bad_problem(p) || p.M == 0 ? 0 : backward_space(p).total;
+  return most_backward_space(p);
 }
 
 PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* bias,
@@ -364,7 +380,7 @@ PWC_API size_t pwc_gated_linear_backward_workspace_size(int layout, long long B,
                                                         int K, int O, int dtype) {
   const Problem p = problem(layout, B, P, K, O, layout == PWC_LAYOUT_MAP ? P * K : K, 0, 0.f,
                             dtype, 1);
-  return bad_problem(p) || p.M == 0 ? 0 : backward_space(p).total;
+  return most_backward_space(p);
 }
 
 PWC_API int pwc_gated_linear_backward(const void* x, const void* weight, const void* bias,

@@ -13,14 +13,63 @@ namespace feat {
 
 enum Layout : int { kMap = 0, kTokens = 1 };
 
-// ---- 16-byte vectors of the storage type ----
-template <typename T> struct alignas(16) Vec16 {
-  static constexpr int N = 16 / (int)sizeof(T);
-  T v[N];
-};
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
+
+// The rounding to storage, with the conversion instructions that this target has for bfloat16.
+template <typename T> __device__ __forceinline__ T narrow(float v) { return from_f32<T>(v); }
+template <> __device__ __forceinline__ __hip_bfloat16 narrow<__hip_bfloat16>(float v) {
+  return __builtin_bit_cast(__hip_bfloat16, (__bf16)v);
+}
+
+// 16 bytes at any alignment of their values
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct Any16 { typedef u32x4_at2 type; };
+template <> struct Any16<float> { typedef u32x4_at4 type; };
+template <typename T> __device__ __forceinline__ u32x4 load16(const T* p) {
+  return *(const typename Any16<T>::type*)p;
+}
+// the first `have` values of 16 bytes, zeros behind them
+template <typename T> __device__ __forceinline__ u32x4 load_some(const T* p, int have) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < have) v[e] = ((const uint32_t*)p)[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < have) v[e / 2] |= (uint32_t)((const uint16_t*)p)[e] << (e % 2 * 16);
+  }
+  return v;
+}
+// V values (16 bytes, or one) as floats
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else {
+    static_assert(V * sizeof(T) == 16, "");
+    const Pack<T, V> o = __builtin_bit_cast(Pack<T, V>, load16(p));
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = to_f32(o.v[e]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = narrow<T>(v[0]);
+  } else {
+    static_assert(V * sizeof(T) == 16, "");
+    Pack<T, V> o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o.v[e] = narrow<T>(v[e]);
+    *(typename Any16<T>::type*)p = __builtin_bit_cast(u32x4, o);
+  }
+}
 
 // Sum over the `W` neighbouring lanes (a power of two) that share a row.
 template <int W> __device__ __forceinline__ float lanes_sum(float v) {
@@ -41,49 +90,87 @@ enum Act : int {
   kActGeluTanh = 7,  // x * sigmoid(2 a), a = sqrt(2 / pi) (x + 0.044715 x^3)
 };
 
-// 1 / (1 + exp(-z)): exp overflows to infinity for z < -88, where the quotient is the right 0.
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + expf(-z)); }
+// The functions for 32-bit results are the device library's.  For 16-bit results (FAST) they are
+// the hardware's exponential and reciprocal, 2^-22 of the value, against a rounding of 2^-11.
+template <bool FAST> __device__ __forceinline__ float exp_neg(float x) {  // exp(-x)
+  return FAST ? __builtin_amdgcn_exp2f(-1.4426950408889634f * x) : expf(-x);
+}
+template <bool FAST> __device__ __forceinline__ float recip(float x) {
+  return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x;
+}
+// exp overflows to infinity for z < -88, where the reciprocal is the right 0
+template <bool FAST> __device__ __forceinline__ float sigmoid_f(float z) {
+  return recip<FAST>(1.f + exp_neg<FAST>(z));
+}
+// Phi(z), the normal distribution function.  FAST: erfc by the rational form of Abramowitz and
+// Stegun 7.1.26 (error 1.5e-7 absolute), whose factor exp(-z^2 / 2) the derivative needs as well.
+template <bool FAST> __device__ __forceinline__ float phi_f(float z, float gauss) {
+  if (!FAST) return 0.5f * erfcf(-0.7071067811865476f * z);
+  const float a = fabsf(z) * 0.7071067811865476f;
+  const float t = recip<true>(1.f + 0.3275911f * a);
+  const float p =
+      t * (0.254829592f +
+           t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * gauss;  // Phi(-|z|)
+  return z > 0.f ? 1.f - tail : tail;
+}
 
 constexpr float kSqrt2OverPi = 0.7978845608028654f;
 
-__device__ __forceinline__ float act_value(int act, float z, float slope) {
-  switch (act) {
-    case kActRelu: return z > 0.f ? z : (z != z ? z : 0.f);
-    case kActLeaky: return z > 0.f ? z : z * slope;
-    case kActSigmoid: return sigmoid_f(z);
-    case kActTanh: return tanhf(z);
-    case kActSilu: return z * sigmoid_f(z);
-    case kActGelu: return 0.5f * z * erfcf(-0.7071067811865476f * z);
-    case kActGeluTanh:
-      return z * sigmoid_f(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
-    default: return z;
-  }
-}
-
-__device__ __forceinline__ float act_slope(int act, float z, float slope) {
-  switch (act) {
-    case kActRelu: return z > 0.f ? 1.f : 0.f;
-    case kActLeaky: return z > 0.f ? 1.f : slope;
-    case kActSigmoid: {
-      const float p = sigmoid_f(z);
-      return p * (1.f - p);
+// f = act(z) and, where SLOPE, d = act'(z), for N values: one branch for all of them.  `slope` is
+// leaky relu's.
+template <bool FAST, bool SLOPE, int N>
+__device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f)[N],
+                                         float (&d)[N], float slope) {
+  if (act == kActSilu) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float p = sigmoid_f<FAST>(z[e]);
+      f[e] = z[e] * p;
+      if (SLOPE) d[e] = p * (1.f + z[e] * (1.f - p));
     }
-    case kActTanh: {
-      const float t = tanhf(z);
-      return 1.f - t * t;
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float g = FAST || SLOPE ? exp_neg<FAST>(0.5f * z[e] * z[e]) : 0.f;
+      const float p = phi_f<FAST>(z[e], g);
+      f[e] = z[e] * p;
+      if (SLOPE) d[e] = p + z[e] * 0.3989422804014327f * g;
     }
-    case kActSilu: {
-      const float p = sigmoid_f(z);
-      return p * (1.f + z * (1.f - p));
+  } else if (act == kActGeluTanh) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float q = z[e] * z[e];
+      const float p = sigmoid_f<FAST>(2.f * kSqrt2OverPi * (z[e] + 0.044715f * z[e] * q));
+      f[e] = z[e] * p;
+      if (SLOPE) d[e] = p + f[e] * (1.f - p) * 2.f * kSqrt2OverPi * (1.f + 0.134145f * q);
     }
-    case kActGelu:
-      return 0.5f * erfcf(-0.7071067811865476f * z) +
-             z * 0.3989422804014327f * expf(-0.5f * z * z);
-    case kActGeluTanh: {
-      const float p = sigmoid_f(2.f * kSqrt2OverPi * (z + 0.044715f * z * z * z));
-      return p + z * p * (1.f - p) * 2.f * kSqrt2OverPi * (1.f + 0.134145f * z * z);
+  } else if (act == kActRelu || act == kActLeaky) {
+    const float s = act == kActRelu ? 0.f : slope;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      f[e] = z[e] > 0.f ? z[e] : act == kActRelu ? (z[e] != z[e] ? z[e] : 0.f) : z[e] * s;
+      if (SLOPE) d[e] = z[e] > 0.f ? 1.f : s;
     }
-    default: return 1.f;
+  } else if (act == kActSigmoid) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      f[e] = sigmoid_f<FAST>(z[e]);
+      if (SLOPE) d[e] = f[e] * (1.f - f[e]);
+    }
+  } else if (act == kActTanh) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      // small z in 16 bits: 2 sigmoid(2 z) - 1 loses the digits that 1 has more than z
+      f[e] = tanhf(z[e]);
+      if (SLOPE) d[e] = 1.f - f[e] * f[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      f[e] = z[e];
+      if (SLOPE) d[e] = 1.f;
+    }
   }
 }
 

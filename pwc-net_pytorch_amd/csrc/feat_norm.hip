@@ -15,22 +15,6 @@
 namespace pwc {
 namespace feat {
 
-// V values from p at any alignment as floats, `n` of them there
-template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-  Pack<T, V> o;
-  __builtin_memcpy(&o, p, sizeof(o));
-#pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = to_f32(o.v[e]);
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
-  Pack<T, V> o;
-#pragma unroll
-  for (int e = 0; e < V; ++e) o.v[e] = from_f32<T>(v[e]);
-  __builtin_memcpy(p, &o, sizeof(o));
-}
-
 // ------------------------------------------------------------------------------ tokens [M][C]
 // TPR threads share a row; each has NV vectors of V channels, TPR * V apart.
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
@@ -60,7 +44,7 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
   for (int k = 0; k < NV; ++k) {
     const int c = (k * TPR + t) * V;
     if (c < a.C) {
-      load_v<T, V>(x + c, v[k]);
+      load_values<T, V>(x + c, v[k]);
 #pragma unroll
       for (int e = 0; e < V; ++e) s += v[k][e];
     }
@@ -87,11 +71,11 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
     const int c = (k * TPR + t) * V;
     if (c < a.C) {
       float w[V], b[V];
-      if (a.w) load_v<T, V>((const T*)a.w + c, w);
-      if (a.b) load_v<T, V>((const T*)a.b + c, b);
+      if (a.w) load_values<T, V>((const T*)a.w + c, w);
+      if (a.b) load_values<T, V>((const T*)a.b + c, b);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * r * (a.w ? w[e] : 1.f) + (a.b ? b[e] : 0.f);
-      store_v<T, V>(y + c, v[k]);
+      store_values<T, V>(y + c, v[k]);
     }
   }
 }
@@ -111,7 +95,7 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
       w[k][e] = 1.f;
       dw[k][e] = db[k][e] = 0.f;
     }
-    if (a.w && c < a.C) load_v<T, V>((const T*)a.w + c, w[k]);
+    if (a.w && c < a.C) load_values<T, V>((const T*)a.w + c, w[k]);
   }
   for (long long m0 = (long long)blockIdx.x * RPB; m0 < a.M; m0 += (long long)gridDim.x * RPB) {
     const long long m = m0 + threadIdx.x / TPR;
@@ -125,8 +109,8 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + t) * V;
       if (row && c < a.C) {
-        load_v<T, V>(x + c, xh[k]);
-        load_v<T, V>(dy + c, h[k]);
+        load_values<T, V>(x + c, xh[k]);
+        load_values<T, V>(dy + c, h[k]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           xh[k][e] = (xh[k][e] - mu) * r;
@@ -147,7 +131,7 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
         if (c < a.C) {
 #pragma unroll
           for (int e = 0; e < V; ++e) h[k][e] = r * (h[k][e] - s1 - xh[k][e] * s2);
-          store_v<T, V>((T*)a.dx + m * a.C + c, h[k]);
+          store_values<T, V>((T*)a.dx + m * a.C + c, h[k]);
         }
       }
     }
@@ -242,7 +226,7 @@ __global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
     if (c < a.C) {
       const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
       const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
-      y[c * a.P] = from_f32<T>(v[k] * r * w + b);
+      y[c * a.P] = narrow<T>(v[k] * r * w + b);
     }
   }
 }
@@ -286,7 +270,7 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
 #pragma unroll
       for (int k = 0; k < kMapChannels; ++k) {
         const int c = k * G + g;
-        if (c < a.C) dx[c * a.P] = from_f32<T>(r * (h[k] - s1 - xh[k] * s2));
+        if (c < a.C) dx[c * a.P] = narrow<T>(r * (h[k] - s1 - xh[k] * s2));
       }
     }
   }
@@ -359,7 +343,7 @@ template <typename T, bool MAP> __global__ __launch_bounds__(256) void norm_any(
   for (int c = first; c < a.C; c += S) {
     const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
     const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
-    y[c * r.stride] = from_f32<T>((to_f32(x[c * r.stride]) - mu) * rs * w + b);
+    y[c * r.stride] = narrow<T>((to_f32(x[c * r.stride]) - mu) * rs * w + b);
   }
 }
 
@@ -385,7 +369,7 @@ __global__ __launch_bounds__(256) void norm_any_dx(const NormArgs a) {
   for (int c = first; c < a.C; c += S) {
     const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
     const float xh = (to_f32(x[c * r.stride]) - mu) * rs;
-    dx[c * r.stride] = from_f32<T>(rs * (to_f32(dy[c * r.stride]) * w - s1 - xh * s2));
+    dx[c * r.stride] = narrow<T>(rs * (to_f32(dy[c * r.stride]) * w - s1 - xh * s2));
   }
 }
 
@@ -437,7 +421,7 @@ __global__ __launch_bounds__(1024) void norm_add_parts(const float* __restrict__
   if (g == 0 && c < C) {
     for (int k = 1; k < 32; ++k) s += red[k][l];
     T* out = blockIdx.y == 0 ? dw : db;
-    if (out) out[c] = from_f32<T>(s);
+    if (out) out[c] = narrow<T>(s);
   }
 }
 
@@ -560,6 +544,17 @@ template <typename T> static hipError_t no_rows_t(const NormArgs& a, hipStream_t
   return hipGetLastError();
 }
 
+hipError_t sum_rows(const float* part, void* out, int C, int rows, int dtype, hipStream_t s) {
+  const dim3 grid((C + 31) / 32, 1);
+  if (dtype == 0)
+    norm_add_parts<float><<<grid, 1024, 0, s>>>(part, (float*)out, nullptr, C, rows);
+  else if (dtype == 1)
+    norm_add_parts<__half><<<grid, 1024, 0, s>>>(part, (__half*)out, nullptr, C, rows);
+  else
+    norm_add_parts<__hip_bfloat16><<<grid, 1024, 0, s>>>(part, (__hip_bfloat16*)out, nullptr, C,
+                                                        rows);
+  return hipGetLastError();
+}
 hipError_t norm_no_rows(const NormArgs& a, int dtype, hipStream_t s) {
   return dtype == 0   ? no_rows_t<float>(a, s)
          : dtype == 1 ? no_rows_t<__half>(a, s)

@@ -11,7 +11,8 @@ enum ProductMode : int {
   kLinearDz = 1,  // other * act'(sum + bias)
   kGated = 2,     // act(gate) * up
   kGatedDz = 3,   // [other * up * act'(gate), other * act(gate)]
-  kPartial = 4,   // 32-bit sums of one split of k, and the sums of B's rows
+  kPlain = 5,     // the sum
+  kPartial = 4,   // 32-bit sums of one split of k; one split alone: the result
 };
 
 // Out(i, j) = sum_k A(i, k) B(j, k), at out[j * ldo + i]; strides in elements.
@@ -19,22 +20,32 @@ struct ProductArgs {
   const void* a;
   const void* b;
   void* out;
-  const void* bias;   // along i (bias_i) or j, or NULL
+  const void* bias;   // along the channels, or NULL
   const void* other;  // residual or output gradient, or NULL; at ldother
-  float* sums;        // kPartial: [splits][J] sums over k of B(j, k), or NULL
+  float* sums;        // k*Dz: partial sums of dz over the tokens, product_sum_rows rows, or NULL
   long long lda, ldb, ldo, ldother;
   long long a_batch, b_batch, out_batch, other_batch;
   long long a_segment, b_segment;  // k runs over `segments` segments of K
   int I, J, K, segments, batches, splits;
   int a_k, b_k;        // the operand lies along k
-  int pair_side;       // 0, or 1 (A) / 2 (B): that operand is [gate; up], `pair` rows each
-  int pair;
-  int bias_i, mode, act;
+  int pair;            // kGated*: W is [gate; up], `pair` rows each
+  int channel_i;       // forward / dz: the channels lie along i (tokens) or j (maps)
+  int mode, act;
   float slope;
   int tiles_i, tiles_j;  // set by the launcher
 };
 
+struct TileShape {
+  int bi, bj, passes;
+};
+template <typename T>
+hipError_t product_t(const ProductArgs& g, TileShape t, bool direct, hipStream_t stream);
+
 hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream);
+int product_sum_rows(const ProductArgs& g, int dtype);
+int product_column_parts(int layout, long long B, long long P, int C);
+hipError_t product_column_sums(const void* dy, float* part, int layout, long long B, long long P,
+                               int C, int parts, int dtype, hipStream_t stream);
 int product_splits(long long I, long long J, int segments, long long K, int dtype);
 hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
                               hipStream_t stream);

@@ -1,0 +1,648 @@
+// feat_product_kernel.cuh — the matrix product kernel of feat_product.hip, instantiated per type.
+#pragma once
+
+#include <type_traits>
+
+#include "feat_product.cuh"
+
+namespace pwc {
+namespace feat {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Frag;
+template <> struct Frag<float> { typedef f32x4 type; };
+template <> struct Frag<__half> { typedef s16x8 type; };
+template <> struct Frag<__hip_bfloat16> { typedef s16x8 type; };
+
+__device__ __forceinline__ f32x4 mma(const f32x4& a, const f32x4& b, f32x4 c, float) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, f32x4 c, __half) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a),
+                                                __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, f32x4 c, __hip_bfloat16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a),
+                                                 __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+// The same with the sums pinned to the accumulation registers: left to itself the compiler moves
+// a 256 x 256 tile's sums between the two register files, 350 moves a step.  Nothing but these
+// instructions touches the sums until the waits behind the loop have let the last of them finish.
+__device__ __forceinline__ void mma_pinned(const s16x8& a, const s16x8& b, f32x4& c, __half) {
+  asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mma_pinned(const s16x8& a, const s16x8& b, f32x4& c,
+                                           __hip_bfloat16) {
+  asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mma_pinned(const f32x4& a, const f32x4& b, f32x4& c, float) {
+  c = mma(a, b, c, 0.f);
+}
+constexpr int kStepBytes = 128;           // bytes of k in a step
+constexpr uint32_t kOOB = 0x80000000u;    // beyond every buffer range: the load returns zeros
+
+// The chunk (16 bytes) of row `r` where logical chunk c lies.
+// K tile: 8 chunks a row; a wave's 16-byte reads take 16 rows at one logical chunk.
+__device__ __forceinline__ int swz_k(int r, int c) { return c ^ ((r >> 1) & 7); }
+// N tile, 16 bits: a transposing read takes, per 16 lanes, 4 rows of 32 bytes; lanes 0-31 take
+// rows 0-3 and 8-11.  32 bits: rows q*4+s of the four lane groups q, 64 bytes each.
+template <typename T, int CHUNKS> __device__ __forceinline__ int swz_n(int k, int c) {
+  const int g = sizeof(T) == 2 ? ((k & 3) | ((k >> 1) & 4)) * 2 : ((k >> 2) & 3) * 4;
+  return c ^ (g & (CHUNKS - 1));
+}
+
+// Chunk c of four sums of row j in the turned tile: 16 neighbouring rows write one chunk each.
+template <int WI> __device__ __forceinline__ int swz_turn(int j, int c) {
+  return c ^ (j & (WI / 4 < 16 ? WI / 4 - 1 : 15));
+}
+
+// V neighbouring sums of row j of the turned tile, from column i on
+template <int WI, int V>
+__device__ __forceinline__ void turned(const float* tile, int j, int i, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = tile[j * WI + swz_turn<WI>(j, i / 4) * 4 + i % 4];
+  } else {
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c) {
+      const f32x4 q = *(const f32x4*)(tile + j * WI + swz_turn<WI>(j, i / 4 + c) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[c * 4 + e] = q[e];
+    }
+  }
+}
+
+// One operand's tile: R rows (its i or j) times a k step, loaded by NW waves.
+template <typename T, int R, bool KC, int NW> struct Tile {
+  static constexpr int E = 16 / (int)sizeof(T);             // values in a chunk
+  static constexpr int KS = kStepBytes / (int)sizeof(T);    // k in a step
+  static constexpr int BYTES = R * kStepBytes;
+  static constexpr int ROWB = KC ? kStepBytes : R * (int)sizeof(T);
+  static constexpr int CHUNKS = ROWB / 16;
+  static constexpr int LOADS = BYTES / 16 / (NW * 64);      // chunks of a thread
+  static_assert(LOADS * NW * 64 * 16 == BYTES, "tile splits over the threads");
+
+  // Chunk n of this thread: its place in LDS is linear (what a wave's direct load wants).
+  static __device__ __forceinline__ int place(int n) {
+    return ((n * NW * 64) + (int)threadIdx.x) * 16;
+  }
+  // row of memory and value within it (relative to the tile) that belong there
+  static __device__ __forceinline__ void source(int n, int& row, int& at) {
+    const int p = place(n);
+    row = p / ROWB;
+    const int c = (p % ROWB) / 16;
+    at = (KC ? swz_k(row, c) : swz_n<T, CHUNKS>(row, c)) * E;
+  }
+  // fragment of 16 rows from r0 (K: rows, N: columns), k part kk (of 2)
+  static __device__ __forceinline__ typename Frag<T>::type frag(const char* lds, int r0, int kk) {
+    const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+    if constexpr (KC) {
+      const int r = r0 + l;
+      return *(const typename Frag<T>::type*)(lds + r * ROWB + swz_k(r, kk * 4 + q) * 16);
+    } else if constexpr (sizeof(T) == 2) {
+      s16x8 f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = kk * 32 + q * 8 + h * 4 + (l >> 2);
+        const int col = r0 + (l & 3) * 4;
+        const char* p = lds + k * ROWB + swz_n<T, CHUNKS>(k, col / 8) * 16 + (col % 8) * 2;
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[h * 4 + e] = v[e];
+      }
+      return f;
+    } else {
+      f32x4 f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = kk * 16 + q * 4 + s, col = r0 + l;
+        f[s] = *(const float*)(lds + k * ROWB + swz_n<T, CHUNKS>(k, col / 4) * 16 + (col % 4) * 4);
+      }
+      return f;
+    }
+  }
+};
+
+// The loads of one operand.  DIRECT: memory -> LDS by the buffer unit, whose range check gives the
+// zeros outside; it wants 16-byte aligned rows.  Otherwise through registers from any address;
+// a chunk that crosses the end of its row is read value by value.
+template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
+  typedef Tile<T, R, KC, NW> Tl;
+  const T* base;      // of the tile's first row and this batch
+  long long ld;
+  int K, limit;       // k in a segment; N: rows left of the tile's own dimension
+  uint32_t off[Tl::LOADS];  // DIRECT: bytes from base, or kOOB
+  int at[Tl::LOADS];        // first k (K) or row k (N) of the chunk within the step
+  long long row[DIRECT ? 1 : Tl::LOADS];
+  int left[DIRECT ? 1 : Tl::LOADS];  // N: valid values from the chunk's start; K: 0 or 1 (row valid)
+  u32x4 reg[DIRECT ? 1 : Tl::LOADS];
+
+  // `pair` > 0: rows alternate in groups of 16 between the halves of a matrix of 2 * pair rows
+  __device__ __forceinline__ void init(const T* b, long long ld_, int K_, int r0, int rows,
+                                       int pair) {
+    ld = ld_;
+    K = K_;
+    base = KC ? b + (pair ? (long long)(r0 / 2) : (long long)r0) * ld : b + r0;
+    limit = rows - r0;
+#pragma unroll
+    for (int n = 0; n < Tl::LOADS; ++n) {
+      int r, c;
+      Tl::source(n, r, c);
+      if constexpr (KC) {
+        long long rr = r;
+        bool ok = r < limit;
+        if (pair) {
+          const int o = (r >> 5) * 16 + (r & 15);
+          ok = r0 / 2 + o < pair;
+          rr = o + ((r >> 4) & 1) * (long long)pair;
+        }
+        at[n] = c;
+        if constexpr (DIRECT) {
+          off[n] = ok ? (uint32_t)(rr * ld + c) * (uint32_t)sizeof(T) : kOOB;
+        } else {
+          row[n] = rr * ld + c;
+          left[n] = ok;
+        }
+      } else {
+        at[n] = r;
+        if constexpr (DIRECT) {
+          off[n] = c < limit ? (uint32_t)(r * ld + c) * (uint32_t)sizeof(T) : kOOB;
+        } else {
+          row[n] = r * ld + c;
+          left[n] = limit - c;
+        }
+      }
+    }
+  }
+
+  // start loading the step at k0 of the segment at `seg` values from base
+  __device__ __forceinline__ void load(char* lds, long long seg, int k0) {
+    const T* b = base + seg + (KC ? (long long)k0 : (long long)k0 * ld);
+    if constexpr (DIRECT) {
+      const uint64_t a = (uint64_t)(uintptr_t)b;
+      const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+      const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(uintptr_t)(((uint64_t)hi << 32) | lo), (short)0, 0x7fffffff, 0x00020000);
+      const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+      for (int n = 0; n < Tl::LOADS; ++n) {
+        const uint32_t o = at[n] < K - k0 ? off[n] : kOOB;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(lds + (n * NW + wave) * 1024), 16, o, 0, 0,
+            0);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < Tl::LOADS; ++n) {
+        // K: k0 + at .. < K;  N: row k0 + at < K, `left` values of it
+        const int have = KC ? (left[n] ? K - k0 - at[n] : 0) : (at[n] < K - k0 ? left[n] : 0);
+        const T* p = b + row[n];
+        if (have >= Tl::E) {
+          reg[n] = load16(p);
+        } else {
+          reg[n] = u32x4{0u, 0u, 0u, 0u};
+          if (have > 0) reg[n] = load_some(p, have);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void finish(char* lds) {
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int n = 0; n < Tl::LOADS; ++n) *(u32x4*)(lds + Tl::place(n)) = reg[n];
+    }
+  }
+};
+
+// What the epilogue needs of one wave's sums: they lie in LDS as rows of i (`tile`, WI long).
+struct Finish {
+  const float* tile;
+  float* row_sums;   // LDS, this wave's: sums of dz over the tokens of a row (maps)
+  int i0, j0;        // first output column and row; gated: counted in outputs
+  int i_end, j_end;  // the output's bounds
+};
+
+// A lane keeps V neighbouring i, so that whole rows leave in 16-byte pieces, and goes over the rows
+// j in batches whose loads are all under way before the first is used: there may be one wave a
+// SIMD, and nothing else would hide them.  V = 1 takes the columns behind the last whole piece.
+template <typename T, int MODE, bool CI, int WI, int WJ, int V>
+__device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finish& f, T* out,
+                                               const T* other, int sum_row) {
+  constexpr bool kFast = sizeof(T) == 2, kPair = MODE == kGated || MODE == kGatedDz;
+  constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
+  constexpr int E = 16 / (int)sizeof(T);                    // columns of a whole piece
+  constexpr int COLS = kPair && CI ? WI / 2 : WI, ROWS = kPair && !CI ? WJ / 2 : WJ;
+  constexpr int U = V == 1 ? E : COLS / V, RS = 64 / U, N = ROWS / RS;
+  constexpr int NB = V == 1 ? 1 : (kPair ? 2 : 4) < N ? (kPair ? 2 : 4) : N;
+  const int lane = threadIdx.x & 63, ul = lane % U, uj = lane / U;
+  const int have = min(COLS, f.i_end - f.i0);               // columns that exist
+  const int ui = V == 1 ? have / E * E + ul : ul * V, i = f.i0 + ui;
+  const bool column = ui + V <= have;
+  const int ti = kPair && CI ? (ui >> 4) * 32 + (ui & 15) : ui;
+  const T* bias = (const T*)g.bias;
+  const long long ldo = g.ldo, ldother = g.ldother;
+  const int act = g.act;
+  const float slope = g.slope;
+
+  // Bias: of a lane's own channels (along i), or of the row
+  float b[V], c[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) b[e] = c[e] = 0.f;
+  if (CI && bias && column) {
+    load_values<T, V>(bias + i, b);
+    if (kPair) load_values<T, V>(bias + g.pair + i, c);
+  }
+  // Bias gradient: sums of dz before it is rounded
+  float sv[V], sw[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sv[e] = sw[e] = 0.f;
+
+#pragma unroll 1
+  for (int r0 = 0; r0 < N; r0 += NB) {
+    float v[NB][V], w[NB][V], o[NB][V], bj[NB], cj[NB];
+    bool ok[NB];
+#pragma unroll
+    for (int r = 0; r < NB; ++r) {
+      const int j = f.j0 + uj + (r0 + r) * RS;
+      ok[r] = column && j < f.j_end;
+      bj[r] = cj[r] = 0.f;
+      if (!CI && bias && ok[r]) {
+        bj[r] = to_f32(bias[j]);
+        if (kPair) cj[r] = to_f32(bias[g.pair + j]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[r][e] = 0.f;
+      if (MODE != kGated && other && ok[r])
+        load_values<T, V>(other + (long long)j * ldother + i, o[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < NB; ++r) {
+      const int rj = uj + (r0 + r) * RS;
+      const int tj = kPair && !CI ? (rj >> 4) * 32 + (rj & 15) : rj;
+      turned<WI, V>(f.tile, tj, ti, v[r]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[r][e] += b[e] + bj[r];
+      if constexpr (kPair) {
+        turned<WI, V>(f.tile, CI ? tj : tj + 16, CI ? ti + 16 : ti, w[r]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[r][e] += c[e] + cj[r];
+      }
+      if constexpr (MODE == kLinear) {
+        if (act != kActNone) activate<kFast, false>(act, v[r], v[r], sv, slope);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[r][e] += o[r][e];
+      } else if constexpr (MODE == kLinearDz) {
+        float a[V], s[V];
+        activate<kFast, true>(act, v[r], a, s, slope);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[r][e] = ok[r] ? o[r][e] * s[e] : 0.f;
+      } else if constexpr (MODE == kGated) {
+        activate<kFast, false>(act, v[r], v[r], sv, slope);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[r][e] *= w[r][e];
+      } else if constexpr (MODE == kGatedDz) {
+        float a[V], s[V];
+        activate<kFast, true>(act, v[r], a, s, slope);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[r][e] = ok[r] ? o[r][e] * w[r][e] * s[e] : 0.f;
+          w[r][e] = ok[r] ? o[r][e] * a[e] : 0.f;
+        }
+      }
+      if constexpr (kDz && CI) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sv[e] += v[r][e];
+          if (kPair) sw[e] += w[r][e];
+        }
+      } else if constexpr (kDz) {
+        if (g.sums) {
+          float s = 0.f, t = 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            s += v[r][e];
+            if (kPair) t += w[r][e];
+          }
+#pragma unroll
+          for (int d = U / 2; d > 0; d >>= 1) {
+            s += __shfl_xor(s, d, 64);
+            if (kPair) t += __shfl_xor(t, d, 64);
+          }
+          if (ul == 0) {
+            f.row_sums[rj] += s;
+            if (kPair) f.row_sums[ROWS + rj] += t;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NB; ++r) {
+      T* p = out + (long long)(f.j0 + uj + (r0 + r) * RS) * ldo + i;
+      if (!ok[r]) continue;
+      store_values<T, V>(p, v[r]);
+      if (MODE == kGatedDz) store_values<T, V>(p + (CI ? (long long)g.pair : g.pair * ldo), w[r]);
+    }
+  }
+  if constexpr (kDz && CI) {
+    if (g.sums) {
+      float* sums = g.sums + (long long)sum_row * (kPair ? 2 * g.pair : g.I);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+#pragma unroll
+        for (int d = U; d < 64; d <<= 1) {
+          sv[e] += __shfl_xor(sv[e], d, 64);
+          if (kPair) sw[e] += __shfl_xor(sw[e], d, 64);
+        }
+        if (uj == 0 && column) {
+          sums[i + e] = sv[e];
+          if (kPair) sums[g.pair + i + e] = sw[e];
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int MODE, bool CI, int WI, int WJ>
+__device__ __forceinline__ void finish_tile(const ProductArgs& g, const float* tile,
+                                            float* row_sums, int i0, int j0, int z, int sum_row) {
+  constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
+  constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
+  constexpr int E = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 63;
+  if constexpr (MODE == kPartial) {
+    if (g.splits > 1) {
+      float* out = (float*)g.out + (long long)z * g.I * g.J;
+#pragma unroll 4
+      for (int u = lane; u < WI / 4 * WJ; u += 64) {
+        const int i = i0 + u % (WI / 4) * 4, j = j0 + u / (WI / 4);
+        float v[4];
+        turned<WI, 4>(tile, u / (WI / 4), u % (WI / 4) * 4, v);
+        if (j >= g.J) continue;
+        if (i + 4 <= g.I) {
+          store_values<float, 4>(out + (long long)j * g.I + i, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < g.I) out[(long long)j * g.I + i + e] = v[e];
+        }
+      }
+      return;
+    }
+  }
+  Finish f;
+  f.tile = tile;
+  f.row_sums = row_sums;
+  f.i0 = kPair && CI ? i0 / 2 : i0;
+  f.j0 = kPair && !CI ? j0 / 2 : j0;
+  f.i_end = kPair && CI ? g.pair : g.I;
+  f.j_end = kPair && !CI ? g.pair : g.J;
+  constexpr int COLS = kPair && CI ? WI / 2 : WI, ROWS = kPair && !CI ? WJ / 2 : WJ;
+  if constexpr (kDz && !CI) {
+    for (int r = lane; r < (kPair ? 2 : 1) * ROWS; r += 64) row_sums[r] = 0.f;
+    __builtin_amdgcn_wave_barrier();
+  }
+  const int batch = MODE == kPartial ? 0 : z;
+  T* out = (T*)g.out + batch * g.out_batch;
+  const T* other = g.other ? (const T*)g.other + batch * g.other_batch : nullptr;
+  // one instance of the body for whole pieces, one for what is left of a row
+  constexpr int M = MODE == kPartial ? kPlain : MODE;
+  const int have = min(COLS, f.i_end - f.i0);
+  if (have >= E) finish_columns<T, M, CI, WI, WJ, E>(g, f, out, other, sum_row);
+  if (have > 0 && have % E) finish_columns<T, M, CI, WI, WJ, 1>(g, f, out, other, sum_row);
+  if constexpr (kDz && !CI) {
+    if (g.sums) {
+      __builtin_amdgcn_wave_barrier();
+      float* sums = g.sums + (long long)sum_row * (kPair ? 2 * g.pair : g.J);
+      for (int r = lane; r < ROWS; r += 64)
+        if (f.j0 + r < f.j_end) {
+          sums[f.j0 + r] = row_sums[r];
+          if (kPair) sums[g.pair + f.j0 + r] = row_sums[ROWS + r];
+        }
+    }
+  }
+}
+
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
+          bool DIRECT>
+__global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void product(const ProductArgs g) {
+  constexpr int NW = NWI * NWJ;
+  constexpr bool PART = MODE == kPartial, CI = BKC && AKC && !PART;  // channels along i: tokens
+  constexpr int WI = BI / NWI, WJ = BJ / NWJ, FI = WI / 16, FJ = WJ / 16;
+  constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
+  typedef Tile<T, BI, AKC, NW> TA;
+  typedef Tile<T, BJ, BKC, NW> TB;
+  typedef typename Frag<T>::type frag_t;
+  // Four buffers, four variables: the compiler then sees that a read of one does not have to wait
+  // for the direct loads that are under way into another.
+  __shared__ __attribute__((aligned(16))) char a0[TA::BYTES], b0[TB::BYTES], a1[TA::BYTES],
+      b1[TB::BYTES];
+  __shared__ float row_sums[NW][WJ];
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+  const int wi = (wave % NWI) * WI, wj = (wave / NWI) * WJ;
+
+  // tile (ti, tj) of batch / k split z; neighbouring tiles on one XCD
+  // (4 tiles along j at a time: 32 tiles in flight on an XCD share 8 tiles of A and 4 of B)
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int plane = g.tiles_i * g.tiles_j, z = id / plane, at = id - z * plane;
+  const int group = at / (4 * g.tiles_i), first = group * 4, in = at - group * 4 * g.tiles_i;
+  const int deep = min(4, g.tiles_j - first);
+  const int ti = in / deep, tj = first + in % deep;
+  const int i0 = ti * BI, j0 = tj * BJ;
+  const int batch = PART ? 0 : z;
+
+  Loader<T, BI, AKC, NW, DIRECT> la;
+  Loader<T, BJ, BKC, NW, DIRECT> lb;
+  la.init((const T*)g.a + batch * g.a_batch, g.lda, g.K, i0, g.I, kPair && CI ? g.pair : 0);
+  lb.init((const T*)g.b + batch * g.b_batch, g.ldb, g.K, j0, g.J, kPair && !CI ? g.pair : 0);
+
+  // steps of this block: all of K, or its share of the segments' steps
+  const int per_seg = (g.K + TA::KS - 1) / TA::KS;
+  const int total = g.segments * per_seg;
+  int s = 0, end = total;
+  if (PART) {
+    s = (int)((long long)total * z / g.splits);
+    end = (int)((long long)total * (z + 1) / g.splits);
+  }
+  // the step whose loads start next
+  int seg = s / per_seg, k0 = (s - seg * per_seg) * TA::KS, next = s;
+  auto start = [&](char* pa, char* pb) __attribute__((always_inline)) {
+    // past the end every chunk is outside: zeros, without an access to memory
+    const int k = next < end ? k0 : 0x3fffffff;
+    la.load(pa, seg * g.a_segment, k);
+    lb.load(pb, seg * g.b_segment, k);
+    ++next;
+    k0 += TA::KS;
+    if (k0 >= g.K) {
+      k0 = 0;
+      ++seg;
+    }
+  };
+  // the started loads are in LDS, and this wave's reads so far are done
+  auto settle = [&](char* pa, char* pb) __attribute__((always_inline)) {
+    la.finish(pa);
+    lb.finish(pb);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  f32x4 acc[FI][FJ];
+#pragma unroll
+  for (int j = 0; j < FJ; ++j)
+#pragma unroll
+    for (int i = 0; i < FI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Two fragment sets: while one is multiplied the other is read.  A step has two halves of k:
+  //   read half 1 | multiply half 0 | wait for the next step's loads, barrier |
+  //   read half 0 of the next step | start the loads of the step after it into the buffer that
+  //   all waves have read | multiply half 1
+  // so the loads have a whole step, the reads half a step, and one barrier a step is enough.
+  frag_t fa[2][FI], fb[2][FJ];
+  auto read = [&](const char* pa, const char* pb, int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) fb[kk][j] = TB::frag(pb, wj + j * 16, kk);
+#pragma unroll
+    for (int i = 0; i < FI; ++i) fa[kk][i] = TA::frag(pa, wi + i * 16, kk);
+  };
+  auto multiply = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+        if constexpr (FI * FJ >= 64)
+          mma_pinned(fa[kk][i], fb[kk][j], acc[i][j], T());
+        else
+          acc[i][j] = mma(fa[kk][i], fb[kk][j], acc[i][j], T());
+      }
+  };
+  auto step = [&](char* ca, char* cb, char* na, char* nb) __attribute__((always_inline)) {
+    read(ca, cb, 1);
+    multiply(0);
+    __builtin_amdgcn_sched_barrier(0);
+    settle(na, nb);
+    __builtin_amdgcn_sched_barrier(0);
+    read(na, nb, 0);
+    start(ca, cb);
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // written sums before the first matrix instruction reads them
+  if constexpr (FI * FJ >= 64) asm volatile("s_nop 7" ::: "memory");
+  start(a0, b0);
+  settle(a0, b0);
+  read(a0, b0, 0);
+  start(a1, b1);
+  if constexpr (FI * FJ >= 64) {
+    // (a step past the end multiplies zeros)
+    for (; s < end; s += 2) {
+      step(a0, b0, a1, b1);
+      step(a1, b1, a0, b0);
+    }
+  } else {
+    char *ca = a0, *cb = b0, *na = a1, *nb = b1;
+    for (; s < end; ++s) {
+      step(ca, cb, na, nb);
+      char* t = ca;
+      ca = na;
+      na = t;
+      t = cb;
+      cb = nb;
+      nb = t;
+    }
+  }
+  // the last matrix instructions, 8 passes of 4 cycles, before their sums are read
+  if constexpr (FI * FJ >= 64) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  // what is still under way into LDS (zeros, or nothing) arrives before LDS is used otherwise
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // lane (l, q) holds i = 16 fi + 4 q + r, j = 16 fj + l
+  // the sums turn through this wave's own part of LDS, HJ of the FJ columns of fragments at a time
+  constexpr int HJ = FJ / PASSES;
+  constexpr int SHARE = WI * HJ * 16 * 4;
+  static_assert(NW == 4 && SHARE <= (TA::BYTES < TB::BYTES ? TA::BYTES : TB::BYTES), "a buffer a wave");
+  float* tile = (float*)(wave == 0 ? a0 : wave == 1 ? b0 : wave == 2 ? a1 : b1);
+  auto pass = [&](auto which) __attribute__((always_inline)) {
+    constexpr int h = decltype(which)::value;
+#pragma unroll
+    for (int fj = 0; fj < HJ; ++fj)
+#pragma unroll
+      for (int fi = 0; fi < FI; ++fi) {
+        const int j = fj * 16 + l;
+        *(f32x4*)(tile + j * WI + swz_turn<WI>(j, fi * 4 + q) * 4) = acc[fi][h * HJ + fj];
+      }
+    __builtin_amdgcn_wave_barrier();
+    // this wave's row of the bias gradient's partial sums
+    const int row = CI ? (tj * NWJ + wave / NWI) * PASSES + h
+                       : (z * g.tiles_i + ti) * NWI + wave % NWI;
+    finish_tile<T, MODE, CI, WI, HJ * 16>(g, tile, row_sums[wave], i0 + wi, j0 + wj + h * HJ * 16, z, row);
+    __builtin_amdgcn_wave_barrier();
+  };
+  static_assert(PASSES <= 2, "passes are written out: the sums have to stay in registers");
+  pass(std::integral_constant<int, 0>());
+  if constexpr (PASSES == 2) pass(std::integral_constant<int, 1>());
+}
+
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
+          bool DIRECT>
+static hipError_t launch(ProductArgs g, hipStream_t stream) {
+  constexpr bool kPair = MODE == kGated || MODE == kGatedDz, CI = AKC && BKC;
+  const long long pairs = (g.pair + 15) / 16 * 32;
+  g.tiles_i = (int)(((kPair && CI ? pairs : g.I) + BI - 1) / BI);
+  g.tiles_j = (int)(((kPair && !CI ? pairs : g.J) + BJ - 1) / BJ);
+  const long long blocks =
+      (long long)g.tiles_i * g.tiles_j * (g.mode == kPartial ? g.splits : g.batches);
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+  product<T, BI, BJ, NWI, NWJ, PASSES, AKC, BKC, MODE, DIRECT>
+      <<<(unsigned)blocks, NWI * NWJ * 64, 0, stream>>>(g);
+  return hipGetLastError();
+}
+
+// the combinations of operands and epilogues that the calls use
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool DIRECT>
+static hipError_t by_operands(const ProductArgs& g, hipStream_t stream) {
+#define PRODUCT(AKC, BKC, MODE) \
+  return launch<T, BI, BJ, NWI, NWJ, PASSES, AKC, BKC, MODE, DIRECT>(g, stream)
+  if (g.a_k && g.b_k) switch (g.mode) {
+      case kLinear: PRODUCT(true, true, kLinear);
+      case kLinearDz: PRODUCT(true, true, kLinearDz);
+      case kGated: PRODUCT(true, true, kGated);
+      case kGatedDz: PRODUCT(true, true, kGatedDz);
+      case kPartial: PRODUCT(true, true, kPartial);
+    }
+  else if (g.b_k) switch (g.mode) {
+      case kLinear: PRODUCT(false, true, kLinear);
+      case kLinearDz: PRODUCT(false, true, kLinearDz);
+      case kGated: PRODUCT(false, true, kGated);
+      case kGatedDz: PRODUCT(false, true, kGatedDz);
+      case kPlain: PRODUCT(false, true, kPlain);
+    }
+  else switch (g.mode) {
+      case kPlain: PRODUCT(false, false, kPlain);
+      case kPartial: PRODUCT(false, false, kPartial);
+    }
+#undef PRODUCT
+  return hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t product_t(const ProductArgs& g, TileShape t, bool direct, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (t.bi == 256) return by_operands<T, 256, 256, 2, 2, 2, true>(g, stream);
+  }
+  return direct ? by_operands<T, 128, 128, 2, 2, 1, true>(g, stream)
+                : by_operands<T, 128, 128, 2, 2, 1, false>(g, stream);
+}
+
+}  // namespace feat
+}  // namespace pwc

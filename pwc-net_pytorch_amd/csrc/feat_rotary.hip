@@ -68,8 +68,8 @@ __global__ __launch_bounds__(256) void rotary_rows(const RotaryArgs a) {
     if constexpr (V == 1) {
       const int p = INTER ? 2 * j0 : j0, q = INTER ? p + 1 : a.R + j0;
       const float f = to_f32(xp[p]), g = to_f32(xp[q]);
-      yp[p] = from_f32<T>(f * c[0] - g * s[0]);
-      yp[q] = from_f32<T>(f * s[0] + g * c[0]);
+      yp[p] = narrow<T>(f * c[0] - g * s[0]);
+      yp[q] = narrow<T>(f * s[0] + g * c[0]);
     } else {
       const int p = INTER ? 2 * j0 : j0, q = INTER ? p + V : a.R + j0;
       Pack<T, V> f = *(const Pack<T, V>*)(xp + p), g = *(const Pack<T, V>*)(xp + q);
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(256) void rotary_rows(const RotaryArgs a) {
         T& tu = INTER ? (2 * e < V ? f.v[2 * e % V] : g.v[2 * e % V]) : f.v[e];
         T& tv = INTER ? (2 * e < V ? f.v[(2 * e + 1) % V] : g.v[(2 * e + 1) % V]) : g.v[e];
         const float fu = to_f32(tu), fv = to_f32(tv);
-        tu = from_f32<T>(fu * c[e] - fv * s[e]);
-        tv = from_f32<T>(fu * s[e] + fv * c[e]);
+        tu = narrow<T>(fu * c[e] - fv * s[e]);
+        tv = narrow<T>(fu * s[e] + fv * c[e]);
       }
       *(Pack<T, V>*)(yp + p) = f;
       *(Pack<T, V>*)(yp + q) = g;
@@ -116,8 +116,8 @@ __global__ __launch_bounds__(256) void rotary_pixels(const RotaryArgs a) {
     if constexpr (V == 1) {
       const float f = to_f32(x[p * a.xs_d]), g = q < a.D ? to_f32(x[q * a.xs_d]) : 0.f;
       // a passing value is not multiplied: infinity times zero is none
-      y[p * a.ys_d] = turned ? from_f32<T>(f * c[0] - g * s[0]) : x[p * a.xs_d];
-      if (q < a.D) y[q * a.ys_d] = turned ? from_f32<T>(f * s[0] + g * c[0]) : x[q * a.xs_d];
+      y[p * a.ys_d] = turned ? narrow<T>(f * c[0] - g * s[0]) : x[p * a.xs_d];
+      if (q < a.D) y[q * a.ys_d] = turned ? narrow<T>(f * s[0] + g * c[0]) : x[q * a.xs_d];
     } else {
       Pack<T, V> f = *(const Pack<T, V>*)(x + p * a.xs_d), g;
       if (q < a.D) g = *(const Pack<T, V>*)(x + q * a.xs_d);
@@ -125,8 +125,8 @@ __global__ __launch_bounds__(256) void rotary_pixels(const RotaryArgs a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float fu = to_f32(f.v[e]), fv = to_f32(g.v[e]);
-          f.v[e] = from_f32<T>(fu * c[e] - fv * s[e]);
-          g.v[e] = from_f32<T>(fu * s[e] + fv * c[e]);
+          f.v[e] = narrow<T>(fu * c[e] - fv * s[e]);
+          g.v[e] = narrow<T>(fu * s[e] + fv * c[e]);
         }
       }
       *(Pack<T, V>*)(y + p * a.ys_d) = f;

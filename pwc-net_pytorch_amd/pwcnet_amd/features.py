@@ -321,8 +321,7 @@ def _product_backward(what, gated, x, weight, bias, grad_out, activation, negati
         raise ValueError(f"{what}: grad_output shape {tuple(grad_out.shape)} != {tuple(shape)}")
     grad_out = grad_out.contiguous()
     gx = torch.empty(like, dtype=x.dtype, device=x.device) if needs[0] else None
-    # the bias gradient is summed by the weight gradient's kernel
-    gw = torch.empty_like(weight) if needs[1] or needs[2] else None
+    gw = torch.empty_like(weight) if needs[1] else None
     gb = torch.empty(weight.shape[0], dtype=x.dtype, device=x.device) if needs[2] else None
     lib, dt = _lib.load(), _lib.DTYPE_CODES[x.dtype]
     if gated:
@@ -336,7 +335,7 @@ def _product_backward(what, gated, x, weight, bias, grad_out, activation, negati
                     _opt(gb), *geo, stride, code, float(negative_slope), dt, wsp, size,
                     _stream(x.device)), what)
     del ws
-    return gx, gw if needs[1] else None, gb
+    return gx, gw, gb
 
 
 def linear_forward(x, weight, bias=None, residual=None, activation="none", negative_slope=0.1,
