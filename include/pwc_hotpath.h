@@ -305,7 +305,8 @@ PWC_API int pwc_corr_forward_group(const pwc_corr_problem* problems, int count, 
  *   PWC_LAYOUT_TOKENS  x[P][C] (B = 1); token m starts at x + m * x_stride elements (>= C)
  * Only the first input may be strided that way; every other tensor is dense in the same layout.
  * Weights, biases and activations share one `dtype`; sums, statistics and activations are fp32,
- * every output is rounded once.  Any alignment of a pointer to its element type is accepted.
+ * every output is rounded once.  Any alignment of a pointer to its element type is accepted;
+ * workspaces are aligned to 256 bytes.
  * Empty batches return 1 (weight gradients over no tokens are written as zeros). */
 #define PWC_LAYOUT_MAP 0
 #define PWC_LAYOUT_TOKENS 1

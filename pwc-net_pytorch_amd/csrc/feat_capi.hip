@@ -94,32 +94,61 @@ ProductArgs forward_args(const Problem& p, const void* x, const void* w, const v
 bool needs_z(const Problem& p) { return p.gated || p.act != kActNone; }
 size_t elem(int dtype) { return dtype == 0 ? 4 : 2; }
 
-struct BackwardSpace {
-  size_t part, sums, total;  // bytes from the start; dz lies at 0
-  int splits, rows;          // rows of partial bias gradients
-};
 ProductArgs dz_args(const Problem& p, const void* x, const void* w, const void* bias,
                     const void* dy, void* dz) {
   return forward_args(p, x, w, bias, dy, dz, p.gated ? kGatedDz : kLinearDz, p.rows);
 }
-// The pointers matter for their alignment alone: without them the larger space.
-BackwardSpace backward_space(const Problem& p, const void* x, const void* w) {
+// dW = dz^T x in 32-bit parts (`out`), or itself where there is one split
+ProductArgs dw_args(const Problem& p, const void* x, const void* dz, void* out) {
+  ProductArgs g = blank();
+  g.mode = kPartial;
+  g.out = out;
+  g.I = p.K;
+  g.J = p.rows;
+  g.ldo = p.K;
+  if (p.layout == PWC_LAYOUT_TOKENS) {
+    g.K = (int)p.M;
+    g.a = x, g.lda = p.x_stride, g.a_k = 0;
+    g.b = dz, g.ldb = p.rows, g.b_k = 0;
+  } else {
+    g.K = (int)p.P;
+    g.segments = (int)p.B;
+    g.a = x, g.lda = p.P, g.a_segment = p.x_stride, g.a_k = 1;
+    g.b = dz, g.ldb = p.P, g.b_segment = (long long)p.rows * p.P, g.b_k = 1;
+  }
+  return g;
+}
+
+struct BackwardSpace {
+  size_t part, sums, total;  // bytes from the start; dz lies at 0
+  int splits, rows;          // rows of partial bias gradients
+};
+BackwardSpace backward_space(const Problem& p, int splits, int rows) {
   BackwardSpace s = {};
-  s.splits = p.layout == PWC_LAYOUT_MAP
-                 ? product_splits(p.K, p.rows, (int)p.B, p.P, p.dtype)
-                 : product_splits(p.K, p.rows, 1, p.M, p.dtype);
-  s.rows = needs_z(p) ? product_sum_rows(dz_args(p, x, w, nullptr, nullptr, nullptr), p.dtype)
-                      : product_column_parts(p.layout, p.B, p.P, p.rows);
+  s.splits = splits;
+  s.rows = rows;
   s.part = needs_z(p) ? align256((size_t)p.M * p.rows * elem(p.dtype)) : 0;
-  s.sums = s.part + (s.splits > 1 ? align256((size_t)s.splits * p.rows * p.K * 4) : 0);
-  s.total = s.sums + align256((size_t)s.rows * p.rows * 4);
+  s.sums = s.part + (splits > 1 ? align256((size_t)splits * p.rows * p.K * 4) : 0);
+  s.total = s.sums + align256((size_t)rows * p.rows * 4);
   return s;
+}
+// (of the pointers only the alignment matters)
+int dw_splits(const Problem& p, const void* x, const void* dz) {
+  return product_plan(dw_args(p, x, dz, nullptr), p.dtype).splits;
+}
+int db_rows(const Problem& p, const void* x, const void* w) {
+  return needs_z(p) ? product_sum_rows(dz_args(p, x, w, nullptr, nullptr, nullptr), p.dtype)
+                    : product_column_parts(p.layout, p.B, p.P, p.rows);
 }
 size_t most_backward_space(const Problem& p) {
   if (bad_problem(p) || p.M == 0) return 0;
-  const size_t a = backward_space(p, nullptr, nullptr).total;
-  const size_t b = backward_space(p, (const void*)1, (const void*)1).total;
-  return a > b ? a : b;
+  int splits = 0, rows = 0;
+  for (const void* at : {(const void*)nullptr, (const void*)1}) {
+    const int s = dw_splits(p, at, at), r = db_rows(p, at, at);
+    if (s > splits) splits = s;
+    if (r > rows) rows = r;
+  }
+  return backward_space(p, splits, rows).total;
 }
 
 int product_backward(const char* fn, const Problem& p, const void* x, const void* w,
@@ -134,8 +163,10 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
   }
   if (!x || !w || !dy) return api_fail(fn, "null buffer");
   if (!dx && !dw && !db) return api_launch(fn, hipSuccess);
-  const BackwardSpace s = backward_space(p, x, w);
-  if (!workspace || bytes < s.total) return api_fail(fn, "workspace too small");
+  const BackwardSpace s = backward_space(
+      p, dw ? dw_splits(p, x, needs_z(p) ? nullptr : dy) : 1, db ? db_rows(p, x, w) : 0);
+  if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
+  if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
   char* ws = (char*)workspace;
   const void* dz = dy;
   if (needs_z(p)) {
@@ -165,23 +196,8 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     if (e != hipSuccess) return api_launch(fn, e);
   }
   if (dw) {
-    ProductArgs g = blank();
-    g.mode = kPartial;
+    ProductArgs g = dw_args(p, x, dz, s.splits > 1 ? (void*)(ws + s.part) : dw);
     g.splits = s.splits;
-    g.out = s.splits > 1 ? (void*)(ws + s.part) : dw;
-    g.I = p.K;
-    g.J = p.rows;
-    g.ldo = p.K;
-    if (p.layout == PWC_LAYOUT_TOKENS) {
-      g.K = (int)p.M;
-      g.a = x, g.lda = p.x_stride, g.a_k = 0;
-      g.b = dz, g.ldb = p.rows, g.b_k = 0;
-    } else {
-      g.K = (int)p.P;
-      g.segments = (int)p.B;
-      g.a = x, g.lda = p.P, g.a_segment = p.x_stride, g.a_k = 1;
-      g.b = dz, g.ldb = p.P, g.b_segment = dz_image, g.b_k = 1;
-    }
     hipError_t e = product_launch(g, p.dtype, stream);
     if (e == hipSuccess && s.splits > 1)
       e = product_add_splits((const float*)(ws + s.part), dw, (long long)p.rows * p.K, s.splits,

@@ -35,18 +35,31 @@ struct ProductArgs {
   int tiles_i, tiles_j;  // set by the launcher
 };
 
-struct TileShape {
-  int bi, bj, passes;
+// The kernels (direct loads from aligned rows, or Any).
+enum ProductKernel : int {
+  kFew16,  // passes over W for at most 16, 32, 64 tokens
+  kFew32,
+  kFew64,
+  kTile64,
+  kTile64Any,
+  kTile128,
+  kTile128Any,
+  kTile256,
 };
+struct ProductPlan {
+  int kernel;
+  int tile, passes;  // edge of the tile; column halves that the epilogue takes it in
+  int splits;        // kPartial
+};
+ProductPlan product_plan(const ProductArgs& g, int dtype);
 template <typename T>
-hipError_t product_t(const ProductArgs& g, TileShape t, bool direct, hipStream_t stream);
+hipError_t product_t(const ProductArgs& g, const ProductPlan& p, hipStream_t stream);
 
 hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream);
 int product_sum_rows(const ProductArgs& g, int dtype);
 int product_column_parts(int layout, long long B, long long P, int C);
 hipError_t product_column_sums(const void* dy, float* part, int layout, long long B, long long P,
                                int C, int parts, int dtype, hipStream_t stream);
-int product_splits(long long I, long long J, int segments, long long K, int dtype);
 hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
                               hipStream_t stream);
 

@@ -26,8 +26,7 @@
 // bytes a lane: eight k of one row (16 bits, one 16x16x32 instruction) or four (32 bits, four
 // 16x16x4 instructions).  The order of k within a fragment does not matter as long as both
 // operands share it; N tiles of 16 bits are turned by the transposing LDS read.
-#include <cstdlib>
-
+#include "feat_norm.cuh"
 #include "feat_product.cuh"
 
 namespace pwc {
@@ -60,13 +59,65 @@ template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int
          fits(g.b, g.ldb, g.b_batch, g.b_segment, g.b_k, g.J, bj, g.channel_i ? 0 : g.pair);
 }
 
-static TileShape tile_shape(const ProductArgs& g, int dtype) {
-  const char* env = getenv("TILE");
-  if (dtype != 0 && env && atoi(env) == 2 &&
-      (dtype == 1 ? direct_loads<__half>(g, 256, 256)
-                  : direct_loads<__hip_bfloat16>(g, 256, 256)))
-    return {256, 256, 2};
-  return {128, 128, 1};
+// Which kernel: the one with the least modelled time.  A step of 128 bytes of k costs a block at
+// least `lag` (loads, barrier, latency), and the blocks of a CU share its matrix units, `work` a
+// block; a tile's epilogue and start cost `fixed` for every round of tiles over the card.  The
+// figures are measured (us; bf16: 8192 x K -> 4096 and 64 x 4096 -> 4096 tokens; fp32: 4096 x 1024
+// -> 1024 and 1000 x 1000 -> 1000): 256-tiles do 1430 TFLOP/s where there are enough of them, 128
+// are the best for some hundred, 64 for less.
+struct TileCost {
+  int tile, blocks;  // blocks that a CU holds
+  double lag, work, fixed;
+};
+static constexpr TileCost kCost16[] = {
+    {64, 4, 0.56, 0.18, 3.3}, {128, 2, 0.80, 0.50, 6.5}, {256, 1, 1.40, 1.50, 16.0}};
+static constexpr TileCost kCost32[] = {{64, 4, 0.65, 0.53, 4.0}, {128, 2, 2.00, 2.00, 8.0}};
+constexpr int kCUs = 256;
+
+static bool direct_any(const ProductArgs& g, int tile, int dtype) {
+  return dtype == 0   ? direct_loads<float>(g, tile, tile)
+         : dtype == 1 ? direct_loads<__half>(g, tile, tile)
+                      : direct_loads<__hip_bfloat16>(g, tile, tile);
+}
+
+ProductPlan product_plan(const ProductArgs& g, int dtype) {
+  const bool pair = g.mode == kGated || g.mode == kGatedDz;
+  // A pass over W reads it once at memory speed, the tiles a block's share of it at a CU's pace.
+  // (tokens alone: their W lies along k, and a kernel of one pass has one batch)
+  if (g.channel_i && (g.mode == kLinear || g.mode == kGated) && g.J <= 64)
+    return {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 1, 1};
+  const long long pairs = ((long long)g.pair + 15) / 16 * 32;
+  const long long ri = pair && g.channel_i ? pairs : g.I, rj = pair && !g.channel_i ? pairs : g.J;
+  const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
+  const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
+  ProductPlan best = {};
+  double least = 1e300;
+  const TileCost* costs = dtype == 0 ? kCost32 : kCost16;
+  for (int n = 0; n < (dtype == 0 ? 2 : 3); ++n) {
+    const TileCost& c = costs[n];
+    const bool direct = direct_any(g, c.tile, dtype);
+    if (c.tile == 256 && !direct) break;
+    const double tiles =
+        (double)((ri + c.tile - 1) / c.tile) * ((rj + c.tile - 1) / c.tile) * g.batches;
+    for (int splits = 1; splits <= (g.mode == kPartial ? 512 : 1); splits *= 2) {
+      if (splits > 1 && splits * 4 > steps) break;  // some steps each
+      const double blocks = tiles * splits, each = steps / splits;
+      const double rounds = blocks / (kCUs * c.blocks);
+      double t = each * c.lag;
+      if (t < blocks / kCUs * each * c.work) t = blocks / kCUs * each * c.work;
+      t += c.fixed * (rounds < 1 ? 1 : rounds);
+      // the partial sums go out and come back, and one more launch
+      if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 5e6;
+      if (t < least) {
+        least = t;
+        const int kernel = c.tile == 64 ? (direct ? kTile64 : kTile64Any)
+                           : c.tile == 128 ? (direct ? kTile128 : kTile128Any)
+                                           : kTile256;
+        best = {kernel, c.tile, c.tile == 256 ? 2 : 1, splits};
+      }
+    }
+  }
+  return best;
 }
 
 template <typename T>
@@ -78,22 +129,18 @@ static hipError_t add_splits_t(const float* part, void* out, long long n, int sp
   return hipGetLastError();
 }
 
-template <typename T>
-static hipError_t dispatch(const ProductArgs& g, TileShape t, hipStream_t stream) {
-  return product_t<T>(g, t, direct_loads<T>(g, t.bi, t.bj), stream);
-}
 hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream) {
-  const TileShape t = tile_shape(g, dtype);
-  return dtype == 0   ? dispatch<float>(g, t, stream)
-         : dtype == 1 ? dispatch<__half>(g, t, stream)
-                      : dispatch<__hip_bfloat16>(g, t, stream);
+  const ProductPlan p = product_plan(g, dtype);
+  return dtype == 0   ? product_t<float>(g, p, stream)
+         : dtype == 1 ? product_t<__half>(g, p, stream)
+                      : product_t<__hip_bfloat16>(g, p, stream);
 }
 
 // Rows of partial sums that a kLinearDz / kGatedDz launch writes.
 int product_sum_rows(const ProductArgs& g, int dtype) {
-  const TileShape t = tile_shape(g, dtype);
-  if (g.channel_i) return (g.J + t.bj - 1) / t.bj * 2 * t.passes;
-  return (g.I + t.bi - 1) / t.bi * 2 * g.batches;
+  const ProductPlan p = product_plan(g, dtype);
+  if (g.channel_i) return (g.J + p.tile - 1) / p.tile * 2 * p.passes;
+  return (g.I + p.tile - 1) / p.tile * 2 * g.batches;
 }
 
 // Partial column sums of dy, for a linear without an activation: tokens [M][C], a wave V channels
@@ -170,18 +217,10 @@ hipError_t product_column_sums(const void* dy, float* part, int layout, long lon
                       : column_sums_t<__hip_bfloat16>(dy, part, layout, B, P, C, parts, stream);
 }
 
-// Blocks that share a weight gradient's k: enough for every CU, a step or more each.
-int product_splits(long long I, long long J, int segments, long long K, int dtype) {
-  const int ks = dtype == 0 ? 32 : 64;
-  const long long tiles = ((I + 127) / 128) * ((J + 127) / 128);
-  const long long steps = segments * ((K + ks - 1) / ks);
-  long long splits = (512 + tiles - 1) / tiles;
-  if (splits > (steps + 3) / 4) splits = (steps + 3) / 4;
-  return (int)(splits < 1 ? 1 : splits);
-}
-
 hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
                               hipStream_t stream) {
+  // many splits of few values: 32 threads share a value's splits
+  if (splits > 8 && n <= (1 << 20)) return sum_rows(part, out, (int)n, splits, dtype, stream);
   return dtype == 0   ? add_splits_t<float>(part, out, n, splits, stream)
          : dtype == 1 ? add_splits_t<__half>(part, out, n, splits, stream)
                       : add_splits_t<__hip_bfloat16>(part, out, n, splits, stream);

@@ -3,6 +3,6 @@
 
 namespace pwc {
 namespace feat {
-template hipError_t product_t<float>(const ProductArgs&, TileShape, bool, hipStream_t);
+template hipError_t product_t<float>(const ProductArgs&, const ProductPlan&, hipStream_t);
 }  // namespace feat
 }  // namespace pwc

@@ -593,6 +593,138 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void pro
   if constexpr (PASSES == 2) pass(std::integral_constant<int, 1>());
 }
 
+// ---- few tokens: a pass over W ----
+// At most 16 JB tokens: the time is W's bytes.  A block takes 16 FR output channels (gated: of each
+// half) and its 8 waves take an eighth of k each, straight from memory into fragments -- W is used
+// once, LDS would only delay it -- with DEPTH loads of 32 bytes a row under way; then the waves'
+// sums are added in their order.
+constexpr int kFewWaves = 8;
+
+template <typename T, int FR, int JB, int MODE>
+__global__ __launch_bounds__(kFewWaves * 64) void few_tokens(const ProductArgs g) {
+  constexpr bool kPair = MODE == kGated;
+  constexpr int E = 16 / (int)sizeof(T), HALVES = kPair ? 2 : 1, FA = FR * HALVES;
+  constexpr int STEP = 8 * E;  // k of a step: two chunks of each of the four lane groups
+  constexpr int DEPTH = FA * JB >= 8 ? 1 : FA * JB >= 4 ? 2 : 4;
+  typedef typename Frag<T>::type frag_t;
+  __shared__ f32x4 join[kFewWaves][FA * JB][64];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
+  const int outs = kPair ? g.pair : g.I, i0 = blockIdx.x * 16 * FR;
+
+  const T* pa[FA];
+  bool oa[FA];
+#pragma unroll
+  for (int f = 0; f < FA; ++f) {
+    const int i = i0 + f / HALVES * 16 + l;
+    oa[f] = i < outs;
+    pa[f] = (const T*)g.a + ((long long)(kPair && f % 2 ? g.pair : 0) + (oa[f] ? i : 0)) * g.lda;
+  }
+  const T* pb[JB];
+  bool ob[JB];
+#pragma unroll
+  for (int f = 0; f < JB; ++f) {
+    ob[f] = f * 16 + l < g.J;
+    pb[f] = (const T*)g.b + (ob[f] ? f * 16 + l : 0) * g.ldb;
+  }
+  f32x4 acc[FA][JB];
+#pragma unroll
+  for (int f = 0; f < FA; ++f)
+#pragma unroll
+    for (int j = 0; j < JB; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // whole steps in turns of DEPTH, then what is left of k value by value
+  const u32x4 none = {0u, 0u, 0u, 0u};
+  auto take = [&](int k, bool whole, u32x4(&va)[FA][2], u32x4(&vb)[JB][2])
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int at = k + (q * 2 + c) * E, have = whole ? E : g.K - at;
+#pragma unroll
+      for (int f = 0; f < FA; ++f) {
+        va[f][c] = none;
+        if (oa[f] && have >= E) va[f][c] = load16(pa[f] + at);
+        if (!whole && oa[f] && have > 0 && have < E) va[f][c] = load_some(pa[f] + at, have);
+      }
+#pragma unroll
+      for (int f = 0; f < JB; ++f) {
+        vb[f][c] = none;
+        if (ob[f] && have >= E) vb[f][c] = load16(pb[f] + at);
+        if (!whole && ob[f] && have > 0 && have < E) vb[f][c] = load_some(pb[f] + at, have);
+      }
+    }
+  };
+  auto use = [&](u32x4(&va)[FA][2], u32x4(&vb)[JB][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int f = 0; f < FA; ++f)
+#pragma unroll
+        for (int j = 0; j < JB; ++j)
+          acc[f][j] = mma(__builtin_bit_cast(frag_t, va[f][c]), __builtin_bit_cast(frag_t, vb[j][c]),
+                          acc[f][j], T());
+  };
+  const int steps = (g.K + STEP - 1) / STEP, whole = g.K / STEP;
+  int s = steps * wave / kFewWaves;
+  const int end = steps * (wave + 1) / kFewWaves, fast = min(end, whole);
+  for (; s + DEPTH <= fast; s += DEPTH) {
+    u32x4 va[DEPTH][FA][2], vb[DEPTH][JB][2];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) take((s + d) * STEP, true, va[d], vb[d]);
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) use(va[d], vb[d]);
+  }
+  for (; s < end; ++s) {
+    u32x4 va[FA][2], vb[JB][2];
+    take(s * STEP, false, va, vb);
+    use(va, vb);
+  }
+
+#pragma unroll
+  for (int f = 0; f < FA; ++f)
+#pragma unroll
+    for (int j = 0; j < JB; ++j) join[wave][f * JB + j][lane] = acc[f][j];
+  __syncthreads();
+  // one wave a fragment; lane (l, q) holds token 16 fj + l, channels 16 fi + 4 q + 0..3
+  for (int u = wave; u < FR * JB; u += kFewWaves) {
+    const int fi = u / JB, fj = u % JB, j = fj * 16 + l, i = i0 + fi * 16 + q * 4;
+    f32x4 a = join[0][fi * HALVES * JB + fj][lane], b = a;
+    for (int w = 1; w < kFewWaves; ++w) a += join[w][fi * HALVES * JB + fj][lane];
+    if (kPair) {
+      b = join[0][(fi * 2 + 1) * JB + fj][lane];
+      for (int w = 1; w < kFewWaves; ++w) b += join[w][(fi * 2 + 1) * JB + fj][lane];
+    }
+    if (j >= g.J) continue;
+    const T* bias = (const T*)g.bias;
+    const T* res = (const T*)g.other;
+    T* out = (T*)g.out + (long long)j * g.ldo;
+    float z[4], v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[r] = a[r] + (bias && i + r < outs ? to_f32(bias[i + r]) : 0.f);
+    activate<sizeof(T) == 2, false>(g.act, z, v, v, g.slope);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (i + r >= outs) continue;
+      if (kPair)
+        v[r] *= b[r] + (bias ? to_f32(bias[g.pair + i + r]) : 0.f);
+      else if (res)
+        v[r] += to_f32(res[(long long)j * g.ldother + i + r]);
+      out[i + r] = narrow<T>(v[r]);
+    }
+  }
+}
+
+template <typename T, int FR, int JB>
+static hipError_t launch_few(const ProductArgs& g, hipStream_t stream) {
+  const bool gated = g.mode == kGated;
+  const unsigned blocks = (unsigned)(((gated ? g.pair : g.I) + 16 * FR - 1) / (16 * FR));
+  if (gated)
+    few_tokens<T, FR, JB, kGated><<<blocks, kFewWaves * 64, 0, stream>>>(g);
+  else
+    few_tokens<T, FR, JB, kLinear><<<blocks, kFewWaves * 64, 0, stream>>>(g);
+  return hipGetLastError();
+}
+
 template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
           bool DIRECT>
 static hipError_t launch(ProductArgs g, hipStream_t stream) {
@@ -636,12 +768,19 @@ static hipError_t by_operands(const ProductArgs& g, hipStream_t stream) {
 }
 
 template <typename T>
-hipError_t product_t(const ProductArgs& g, TileShape t, bool direct, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
-    if (t.bi == 256) return by_operands<T, 256, 256, 2, 2, 2, true>(g, stream);
+hipError_t product_t(const ProductArgs& g, const ProductPlan& p, hipStream_t stream) {
+  switch (p.kernel) {
+    case kFew16: return launch_few<T, 1, 1>(g, stream);
+    case kFew32: return launch_few<T, 1, 2>(g, stream);
+    case kFew64: return launch_few<T, 1, 4>(g, stream);
+    case kTile64: return by_operands<T, 64, 64, 2, 2, 1, true>(g, stream);
+    case kTile64Any: return by_operands<T, 64, 64, 2, 2, 1, false>(g, stream);
+    case kTile128: return by_operands<T, 128, 128, 2, 2, 1, true>(g, stream);
+    case kTile128Any: return by_operands<T, 128, 128, 2, 2, 1, false>(g, stream);
+    case kTile256:
+      if constexpr (sizeof(T) == 2) return by_operands<T, 256, 256, 2, 2, 2, true>(g, stream);
   }
-  return direct ? by_operands<T, 128, 128, 2, 2, 1, true>(g, stream)
-                : by_operands<T, 128, 128, 2, 2, 1, false>(g, stream);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace feat

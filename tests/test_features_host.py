@@ -98,8 +98,10 @@ def test_product_entries_refuse():
         assert bwd(gw=z, gb=z, P=0) == 1
     assert lib.pwc_linear_backward_workspace_size(0, 1, 4, 8, 6, 0, 9) == 0
     assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 4, 0, 6, 0) == 0
-    # dz [4, 12] and the split sums of dW [12, 8]
-    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 4, 8, 6, 0) >= 4 * 12 * 4 + 12 * 8 * 4
+    # dz [4, 12], and the sums of dW [12, 8] where k is split
+    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 4, 8, 6, 0) >= 4 * 12 * 4
+    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 10 ** 6, 8, 6, 0) >= \
+        10 ** 6 * 12 * 4 + 2 * 12 * 8 * 4
 
 
 def test_rotary_entry_refuses():
