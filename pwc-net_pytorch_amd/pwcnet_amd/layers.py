@@ -158,35 +158,22 @@ def _traced(x):
     return torch.compiler.is_compiling() or type(x) not in (torch.Tensor, nn.Parameter)
 
 
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=1):
     """(x - mean) / sqrt(var + eps) * weight + bias over the channels of each pixel of a map
     [B, C, *spatial] (``channel_dim=1``) or of each token [..., C] (``channel_dim=-1``)."""
     if _traced(x):
         return _library.layer_norm(x, weight, bias, eps, channel_dim)[0]
-    if _wants_grad(x, weight, bias):
-        return _features.LayerNormFunction.apply(x, weight, bias, eps, channel_dim)
-    with _features._on(x):
-        return _features.layer_norm_forward(x, weight, bias, eps, channel_dim)[0]
+    return _features._ext.layer_norm(x, weight, bias, eps, channel_dim)
 
 
 def rotary(x, inv_freq, axis, positions=None, grid=None, origin=None, interleaved=False):
     """x [B, N, heads, D] with its channel pairs turned by position[axis[j]] * inv_freq[j]; see
     ``features.rotary_forward``.  ``inv_freq`` and ``axis`` come from ``rotary_frequencies``."""
-    if positions is not None and positions.requires_grad:
-        raise ValueError("rotary: positions have no gradient")
     if _traced(x):
         grid = None if grid is None else list(grid)
         origin = None if origin is None else list(origin)
         return _library.rotary(x, inv_freq, axis, positions, grid, origin, interleaved, False)
-    if _wants_grad(x):
-        return _features.RotaryFunction.apply(x, inv_freq, axis, positions, grid, origin,
-                                              interleaved)
-    with _features._on(x):
-        return _features.rotary_forward(x, inv_freq, axis, positions, grid, origin, interleaved)
+    return _features._ext.rotary(x, inv_freq, axis, positions, grid, origin, interleaved)
 
 
 def linear(x, weight, bias=None, residual=None, activation="none", negative_slope=0.1,
@@ -196,12 +183,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", negative_slop
     activation = activation or "none"
     if _traced(x):
         return _library.linear(x, weight, bias, residual, activation, negative_slope, channel_dim)
-    if _wants_grad(x, weight, bias, residual):
-        return _features.LinearFunction.apply(x, weight, bias, residual, activation,
-                                              negative_slope, channel_dim)
-    with _features._on(x):
-        return _features.linear_forward(x, weight, bias, residual, activation, negative_slope,
-                                        channel_dim)
+    return _features._ext.linear(x, weight, bias, residual, activation, negative_slope,
+                                 channel_dim)
 
 
 def gated_linear(x, weight, bias=None, activation="silu", negative_slope=0.1, channel_dim=1):
@@ -210,12 +193,7 @@ def gated_linear(x, weight, bias=None, activation="silu", negative_slope=0.1, ch
     activation = activation or "none"
     if _traced(x):
         return _library.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
-    if _wants_grad(x, weight, bias):
-        return _features.GatedLinearFunction.apply(x, weight, bias, activation, negative_slope,
-                                                   channel_dim)
-    with _features._on(x):
-        return _features.gated_linear_forward(x, weight, bias, activation, negative_slope,
-                                              channel_dim)
+    return _features._ext.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
 
 
 class LayerNorm(nn.Module):

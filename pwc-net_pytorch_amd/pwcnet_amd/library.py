@@ -193,8 +193,7 @@ def _tokens(x, channel_dim):
 def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
     """(y, mean, rstd)"""
-    with _on(x):
-        return _features.layer_norm_forward(x, weight, bias, eps, channel_dim, stats=True)
+    return _features.layer_norm_forward(x, weight, bias, eps, channel_dim, True)
 
 
 @layer_norm.register_fake
@@ -207,8 +206,7 @@ def _(x, weight, bias, eps, channel_dim):
 @torch.library.custom_op(f"{_NS}::layer_norm_backward", mutates_args=())
 def layer_norm_backward(x: Tensor, weight: Optional[Tensor], grad: Tensor, mean: Tensor,
                         rstd: Tensor, channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
-    with _on(x):
-        return _features.layer_norm_backward(x, weight, grad, mean, rstd, channel_dim)
+    return _features.layer_norm_backward(x, weight, grad, mean, rstd, channel_dim)
 
 
 @layer_norm_backward.register_fake
@@ -236,9 +234,8 @@ layer_norm.register_autograd(_norm_bwd, setup_context=_norm_setup)
 def rotary(x: Tensor, inv_freq: Tensor, axis: Tensor, positions: Optional[Tensor],
            grid: Optional[List[int]], origin: Optional[List[int]], interleaved: bool,
            inverse: bool) -> Tensor:
-    with _on(x):
-        return _features.rotary_forward(x, inv_freq, axis, positions, grid, origin, interleaved,
-                                        inverse)
+    return _features.rotary_forward(x, inv_freq, axis, positions, grid, origin, interleaved,
+                                    inverse)
 
 
 @rotary.register_fake
@@ -270,9 +267,8 @@ def _product_fake(x, weight, channel_dim, halves):
 @torch.library.custom_op(f"{_NS}::linear", mutates_args=())
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor],
            activation: str, negative_slope: float, channel_dim: int) -> Tensor:
-    with _on(x):
-        return _features.linear_forward(x, weight, bias, residual, activation, negative_slope,
-                                        channel_dim)
+    return _features.linear_forward(x, weight, bias, residual, activation, negative_slope,
+                                    channel_dim)
 
 
 @linear.register_fake
@@ -284,17 +280,15 @@ def _(x, weight, bias, residual, activation, negative_slope, channel_dim):
 def linear_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], grad: Tensor,
                     activation: str, negative_slope: float,
                     channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
-    with _on(x):
-        return _features.linear_backward(x, weight, bias, grad, activation, negative_slope,
-                                         channel_dim)
+    return _features.linear_backward(x, weight, bias, grad, activation, negative_slope,
+                                     channel_dim)
 
 
 @torch.library.custom_op(f"{_NS}::gated_linear", mutates_args=())
 def gated_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: str,
                  negative_slope: float, channel_dim: int) -> Tensor:
-    with _on(x):
-        return _features.gated_linear_forward(x, weight, bias, activation, negative_slope,
-                                              channel_dim)
+    return _features.gated_linear_forward(x, weight, bias, activation, negative_slope,
+                                          channel_dim)
 
 
 @gated_linear.register_fake
@@ -306,9 +300,8 @@ def _(x, weight, bias, activation, negative_slope, channel_dim):
 def gated_linear_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], grad: Tensor,
                           activation: str, negative_slope: float,
                           channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
-    with _on(x):
-        return _features.gated_linear_backward(x, weight, bias, grad, activation, negative_slope,
-                                               channel_dim)
+    return _features.gated_linear_backward(x, weight, bias, grad, activation, negative_slope,
+                                           channel_dim)
 
 
 def _product_backward_fake(x, weight, *args):

@@ -156,35 +156,33 @@ def test_functions_refuse_host_tensors_and_bad_arguments():
         P.RotaryPosition((2,))(x)
 
 
-def test_shapes_and_strides_are_checked_before_the_device():
-    """The geometry helpers, on host tensors."""
+def test_geometry():
+    """How shapes and strides are taken, on host tensors: (taken as is, layout, B, P, C, stride)."""
     from pwcnet_amd import features as F
-    for dim in (0, 2, -2, 3):
-        if dim == 3:
-            assert F._by_rows((2, 3, 4, 5), dim, "x")
-            continue
+    by_rows, matrix = F._ext.by_rows, F._ext.matrix
+    for dim in (0, 2, -2):
         with pytest.raises(ValueError, match="channel_dim"):
-            F._by_rows((2, 3, 4, 5), dim, "x")
-    with pytest.raises(ValueError, match="channel_dim"):
-        F._by_rows((3,), 1, "x")
-    assert F._by_rows((3,), -1, "x") and F._by_rows((5, 3), 1, "x")
-    assert not F._by_rows((5, 3, 2), 1, "x")
+            by_rows((2, 3, 4, 5), dim, "x")
+    assert by_rows((2, 3, 4, 5), 3, "x")
+    for shape in ((3,), ()):
+        with pytest.raises(ValueError, match="channel_dim"):
+            by_rows(shape, 1, "x")
+    assert by_rows((3,), -1, "x") and by_rows((5, 3), 1, "x")
+    assert not by_rows((5, 3, 2), 1, "x")
     base = torch.zeros(6, 10, 12)
     for t, stride in ((base, 12), (base[..., :8], 12), (base[:, 2:3], 120), (base[:1, ::2], 24),
                       (base.transpose(0, 1), None), (base[..., ::2], None),
                       (base[:, :5, :7], None), (torch.zeros(1, 12).expand(4, 12), None),
-                      (torch.zeros(4, 1).expand(4, 1), 1)):
-        v, layout, B, P, C, got = F._matrix(t, True)
-        assert (layout, B, P, C) == (F.TOKENS, 1, t.numel() // t.shape[-1], t.shape[-1])
-        assert got == (t.shape[-1] if stride is None else stride)
-        assert (v is t) == (stride is not None)
+                      (torch.zeros(4, 1).expand(4, 1), 1), (torch.zeros(4, 2)[:, :1], 2)):
+        got = matrix(t, True)
+        assert got == (stride is not None, F.TOKENS, 1, t.numel() // t.shape[-1], t.shape[-1],
+                       t.shape[-1] if stride is None else stride)
     for t, stride in ((base, 120), (base[:, 2:7], 120), (base[::2], 240),
                       (base.transpose(1, 2), None), (base[..., 1:], None),
                       (base[:1].expand(3, 10, 12), None)):
-        v, layout, B, P, C, got = F._matrix(t, False)
-        assert (layout, B, C, P) == (F.MAP, *t.shape)
-        assert got == (t.shape[1] * t.shape[2] if stride is None else stride)
-        assert (v is t) == (stride is not None)
+        got = matrix(t, False)
+        assert got == (stride is not None, F.MAP, t.shape[0], t.shape[2], t.shape[1],
+                       t.shape[1] * t.shape[2] if stride is None else stride)
 
 
 def test_frequencies():

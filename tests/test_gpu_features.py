@@ -815,3 +815,91 @@ def test_net_with_refined_features():
     for name, p in net.named_parameters():
         if name.startswith("FeatureBlocks"):
             assert torch.isfinite(p.grad).all() and p.grad.abs().max() > 0, name
+
+
+def test_refusals_on_the_device():
+    """Shapes, types and places that the Python functions refuse, and a second derivative."""
+    import pwcnet_amd as P
+    x, w, b = (torch.zeros(2, 4, 3, 3, device=DEV), torch.zeros(6, 4, device=DEV),
+               torch.zeros(6, device=DEV))
+    f, a = P.rotary_frequencies((2,), device=DEV)
+    h = torch.zeros(1, 9, 2, 4, device=DEV)
+    for call, error, text in (
+            (lambda: P.linear(x, w[:, :3]), ValueError, "weight shape"),
+            (lambda: P.linear(x, w[0]), ValueError, "weight shape"),
+            (lambda: P.linear(x, w[:0]), ValueError, "weight shape"),
+            (lambda: P.linear(x, w, b[:5]), ValueError, "bias shape"),
+            (lambda: P.linear(x, w, b, x), ValueError, "residual shape"),
+            (lambda: P.linear(x, w, activation="swish"), ValueError, "activation"),
+            (lambda: P.linear(x, w.half()), TypeError, "mixed dtypes"),
+            (lambda: P.linear(x.double(), w.double()), TypeError, "unsupported dtype"),
+            (lambda: P.linear(x, w.cpu()), RuntimeError, "HIP devices"),
+            (lambda: P.linear(x, w, channel_dim=2), ValueError, "channel_dim"),
+            (lambda: P.gated_linear(x, w[:5]), ValueError, "odd number"),
+            (lambda: P.layer_norm(x, b), ValueError, "weight shape"),
+            (lambda: P.layer_norm(x, eps=-1.0), ValueError, "eps"),
+            (lambda: P.layer_norm(x[:, :0]), ValueError, "no channels"),
+            (lambda: P.rotary(x[0], f, a, grid=(3,)), ValueError, "expected"),
+            (lambda: P.rotary(h, f.float(), a, grid=(9,)), TypeError, "fp64"),
+            (lambda: P.rotary(h, f, a.long(), grid=(9,)), TypeError, "int32"),
+            (lambda: P.rotary(h[..., :3], f, a, grid=(9,)), ValueError, "pairs"),
+            (lambda: P.rotary(h, f, a), ValueError, "positions or grid"),
+            (lambda: P.rotary(h, f, a, f, grid=(9,)), ValueError, "positions or grid"),
+            (lambda: P.rotary(h, f, a, grid=(2, 4)), ValueError, "grid"),
+            (lambda: P.rotary(h, f, a, grid=(9,), origin=(1, 2)), ValueError, "grid"),
+            (lambda: P.rotary(h, f, a, grid=(-3, -3)), ValueError, "grid"),
+            (lambda: P.rotary(h, f, a, torch.zeros(8, 1, device=DEV)), ValueError, "positions"),
+            (lambda: P.rotary(h, f, a, torch.zeros(9, 5, device=DEV)), ValueError, "positions"),
+            (lambda: P.rotary(h, f, a, torch.zeros(9, 1, device=DEV).double()), TypeError,
+             "positions"),
+            (lambda: P.rotary(h, f, a, torch.zeros(9, 1)), RuntimeError, "different devices")):
+        with pytest.raises(error, match=text):
+            call()
+    v = torch.randn(5, 4, device=DEV, requires_grad=True)
+    for y in (P.linear(v, w, activation="silu", channel_dim=-1), P.gated_linear(v, w, channel_dim=-1),
+              P.layer_norm(v, channel_dim=-1)):
+        g, = torch.autograd.grad(y.square().sum(), v, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiat"):
+            g.sum().backward()
+
+
+def test_threads_and_inplace_changes():
+    """Two threads at once, and a saved input that was changed before its backward pass."""
+    import threading
+    import pwcnet_amd as P
+    gen = _gen("threads")
+    x, w, g = _rand(gen, 64, 48), _rand(gen, 32, 48), _rand(gen, 64, 32)
+
+    def step(stream):
+        with torch.cuda.stream(stream):
+            a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            y = P.linear(a, b, activation="gelu", channel_dim=-1)
+            out = [y.detach(), *torch.autograd.grad(y, (a, b), g)]
+            stream.synchronize()
+            return out
+
+    want = step(torch.cuda.current_stream())
+    got = {}
+
+    def work(k):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.default_stream())
+        for _ in range(20):
+            got[k] = step(s)
+            assert all(torch.equal(p, q) for p, q in zip(got[k], want))
+        got[k] = "done"
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got == {0: "done", 1: "done"}
+    a = x.clone().requires_grad_(True)
+    c = a * 1
+    y = P.linear(c, w, activation="gelu", channel_dim=-1)
+    with torch.no_grad():
+        c.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
