@@ -46,16 +46,20 @@ template <typename T> __device__ __forceinline__ u32x4 load_some(const T* p, int
   }
   return v;
 }
+// V values of 16 bytes as floats
+template <typename T, int V> __device__ __forceinline__ void as_floats(u32x4 p, float (&v)[V]) {
+  static_assert(V * sizeof(T) == 16, "");
+  const Pack<T, V> o = __builtin_bit_cast(Pack<T, V>, p);
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = to_f32(o.v[e]);
+}
 // V values (16 bytes, or one) as floats
 template <typename T, int V>
 __device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
   if constexpr (V == 1) {
     v[0] = to_f32(*p);
   } else {
-    static_assert(V * sizeof(T) == 16, "");
-    const Pack<T, V> o = __builtin_bit_cast(Pack<T, V>, load16(p));
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = to_f32(o.v[e]);
+    as_floats<T, V>(load16(p), v);
   }
 }
 template <typename T, int V>

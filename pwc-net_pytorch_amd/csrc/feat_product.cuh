@@ -48,7 +48,7 @@ enum ProductKernel : int {
 };
 struct ProductPlan {
   int kernel;
-  int tile, passes;  // edge of the tile; column halves that the epilogue takes it in
+  int bi, bj, passes;  // the tile; column halves that the epilogue takes it in
   int splits;        // kPartial
 };
 ProductPlan product_plan(const ProductArgs& g, int dtype);

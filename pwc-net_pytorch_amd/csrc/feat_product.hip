@@ -26,6 +26,8 @@
 // bytes a lane: eight k of one row (16 bits, one 16x16x32 instruction) or four (32 bits, four
 // 16x16x4 instructions).  The order of k within a fragment does not matter as long as both
 // operands share it; N tiles of 16 bits are turned by the transposing LDS read.
+#include <cstdlib>
+
 #include "feat_norm.cuh"
 #include "feat_product.cuh"
 
@@ -66,18 +68,20 @@ template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int
 // -> 1024 and 1000 x 1000 -> 1000): 256-tiles do 1430 TFLOP/s where there are enough of them, 128
 // are the best for some hundred, 64 for less.
 struct TileCost {
-  int tile, blocks;  // blocks that a CU holds
+  int kernel, bi, bj, passes, blocks;  // blocks that a CU holds
   double lag, work, fixed;
 };
-static constexpr TileCost kCost16[] = {
-    {64, 4, 0.56, 0.18, 3.3}, {128, 2, 0.80, 0.50, 6.5}, {256, 1, 1.40, 1.50, 16.0}};
-static constexpr TileCost kCost32[] = {{64, 4, 0.65, 0.53, 4.0}, {128, 2, 2.00, 2.00, 8.0}};
+static constexpr TileCost kCost16[] = {{kTile64, 64, 64, 1, 4, 0.56, 0.18, 3.3},
+                                       {kTile128, 128, 128, 1, 2, 0.80, 0.50, 6.5},
+                                       {kTile256, 256, 256, 2, 1, 1.40, 1.50, 16.0}};
+static constexpr TileCost kCost32[] = {{kTile64, 64, 64, 1, 4, 0.65, 0.53, 4.0},
+                                       {kTile128, 128, 128, 1, 2, 2.00, 2.00, 8.0}};
 constexpr int kCUs = 256;
 
-static bool direct_any(const ProductArgs& g, int tile, int dtype) {
-  return dtype == 0   ? direct_loads<float>(g, tile, tile)
-         : dtype == 1 ? direct_loads<__half>(g, tile, tile)
-                      : direct_loads<__hip_bfloat16>(g, tile, tile);
+static bool direct_any(const ProductArgs& g, const TileCost& c, int dtype) {
+  return dtype == 0   ? direct_loads<float>(g, c.bi, c.bj)
+         : dtype == 1 ? direct_loads<__half>(g, c.bi, c.bj)
+                      : direct_loads<__hip_bfloat16>(g, c.bi, c.bj);
 }
 
 ProductPlan product_plan(const ProductArgs& g, int dtype) {
@@ -85,20 +89,24 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
   // A pass over W reads it once at memory speed, the tiles a block's share of it at a CU's pace.
   // (tokens alone: their W lies along k, and a kernel of one pass has one batch)
   if (g.channel_i && (g.mode == kLinear || g.mode == kGated) && g.J <= 64)
-    return {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 1, 1};
+    return {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 16, 1, 1};
   const long long pairs = ((long long)g.pair + 15) / 16 * 32;
   const long long ri = pair && g.channel_i ? pairs : g.I, rj = pair && !g.channel_i ? pairs : g.J;
-  const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
-  const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
   ProductPlan best = {};
   double least = 1e300;
   const TileCost* costs = dtype == 0 ? kCost32 : kCost16;
+  const char* env = getenv("TILE");
+  int pick = env ? atoi(env) : -1;
+  if (pick >= 0 && (pick >= (dtype == 0 ? 2 : 3) || (pick >= 2 && !direct_any(g, costs[pick], dtype)))) pick = -1;
   for (int n = 0; n < (dtype == 0 ? 2 : 3); ++n) {
     const TileCost& c = costs[n];
-    const bool direct = direct_any(g, c.tile, dtype);
-    if (c.tile == 256 && !direct) break;
+    if (pick >= 0 && pick != n) continue;
+    const bool direct = direct_any(g, c, dtype);
+    if (!direct && c.bi > 128) break;
+    const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
+    const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
     const double tiles =
-        (double)((ri + c.tile - 1) / c.tile) * ((rj + c.tile - 1) / c.tile) * g.batches;
+        (double)((ri + c.bi - 1) / c.bi) * ((rj + c.bj - 1) / c.bj) * g.batches;
     for (int splits = 1; splits <= (g.mode == kPartial ? 512 : 1); splits *= 2) {
       if (splits > 1 && splits * 4 > steps) break;  // some steps each
       const double blocks = tiles * splits, each = steps / splits;
@@ -110,14 +118,18 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
       if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 5e6;
       if (t < least) {
         least = t;
-        const int kernel = c.tile == 64 ? (direct ? kTile64 : kTile64Any)
-                           : c.tile == 128 ? (direct ? kTile128 : kTile128Any)
-                                           : kTile256;
-        best = {kernel, c.tile, c.tile == 256 ? 2 : 1, splits};
+        best = {c.kernel + (direct || c.bi > 128 ? 0 : 1), c.bi, c.bj, c.passes, splits};
       }
     }
   }
   return best;
+}
+
+hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream) {
+  const ProductPlan p = product_plan(g, dtype);
+  return dtype == 0   ? product_t<float>(g, p, stream)
+         : dtype == 1 ? product_t<__half>(g, p, stream)
+                      : product_t<__hip_bfloat16>(g, p, stream);
 }
 
 template <typename T>
@@ -129,18 +141,11 @@ static hipError_t add_splits_t(const float* part, void* out, long long n, int sp
   return hipGetLastError();
 }
 
-hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream) {
-  const ProductPlan p = product_plan(g, dtype);
-  return dtype == 0   ? product_t<float>(g, p, stream)
-         : dtype == 1 ? product_t<__half>(g, p, stream)
-                      : product_t<__hip_bfloat16>(g, p, stream);
-}
-
 // Rows of partial sums that a kLinearDz / kGatedDz launch writes.
 int product_sum_rows(const ProductArgs& g, int dtype) {
   const ProductPlan p = product_plan(g, dtype);
-  if (g.channel_i) return (g.J + p.tile - 1) / p.tile * 2 * p.passes;
-  return (g.I + p.tile - 1) / p.tile * 2 * g.batches;
+  if (g.channel_i) return (g.J + p.bj - 1) / p.bj * 2 * p.passes;
+  return (g.I + p.bi - 1) / p.bi * 2 * g.batches;
 }
 
 // Partial column sums of dy, for a linear without an activation: tokens [M][C], a wave V channels

@@ -49,7 +49,7 @@ constexpr int kStepBytes = 128;           // bytes of k in a step
 constexpr uint32_t kOOB = 0x80000000u;    // beyond every buffer range: the load returns zeros
 
 // The chunk (16 bytes) of row `r` where logical chunk c lies.
-// K tile: 8 chunks a row; a wave's 16-byte reads take 16 rows at one logical chunk.
+// K tile: a wave's 16-byte reads take 16 rows at one logical chunk of the 8 of a row.
 __device__ __forceinline__ int swz_k(int r, int c) { return c ^ ((r >> 1) & 7); }
 // N tile, 16 bits: a transposing read takes, per 16 lanes, 4 rows of 32 bytes; lanes 0-31 take
 // rows 0-3 and 8-11.  32 bits: rows q*4+s of the four lane groups q, 64 bytes each.
@@ -265,6 +265,21 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
 #pragma unroll
   for (int e = 0; e < V; ++e) sv[e] = sw[e] = 0.f;
 
+  // the residual or output gradient, a batch ahead
+  constexpr bool kOther = MODE != kGated && MODE != kPlain;
+  u32x4 ahead[kOther && V > 1 ? NB : 1];
+  auto fetch = [&](int r0) __attribute__((always_inline)) {
+    if constexpr (kOther && V > 1) {
+#pragma unroll
+      for (int r = 0; r < NB; ++r) {
+        const int j = f.j0 + uj + (r0 + r) * RS;
+        ahead[r] = u32x4{0u, 0u, 0u, 0u};
+        if (other && column && r0 < N && j < f.j_end)
+          ahead[r] = load16(other + (long long)j * ldother + i);
+      }
+    }
+  };
+  fetch(0);
 #pragma unroll 1
   for (int r0 = 0; r0 < N; r0 += NB) {
     float v[NB][V], w[NB][V], o[NB][V], bj[NB], cj[NB];
@@ -280,9 +295,13 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) o[r][e] = 0.f;
-      if (MODE != kGated && other && ok[r])
-        load_values<T, V>(other + (long long)j * ldother + i, o[r]);
+      if constexpr (kOther && V > 1) {
+        as_floats<T, V>(ahead[r], o[r]);
+      } else if constexpr (kOther) {
+        if (other && ok[r]) o[r][0] = to_f32(other[(long long)j * ldother + i]);
+      }
     }
+    fetch(r0 + NB);
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
       const int rj = uj + (r0 + r) * RS;
@@ -432,7 +451,8 @@ __device__ __forceinline__ void finish_tile(const ProductArgs& g, const float* t
 
 template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
           bool DIRECT>
-__global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void product(const ProductArgs g) {
+__global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
+    void product(const ProductArgs g) {
   constexpr int NW = NWI * NWJ;
   constexpr bool PART = MODE == kPartial, CI = BKC && AKC && !PART;  // channels along i: tokens
   constexpr int WI = BI / NWI, WJ = BJ / NWJ, FI = WI / 16, FJ = WJ / 16;
@@ -440,7 +460,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void pro
   typedef Tile<T, BI, AKC, NW> TA;
   typedef Tile<T, BJ, BKC, NW> TB;
   typedef typename Frag<T>::type frag_t;
-  // Four buffers, four variables: the compiler then sees that a read of one does not have to wait
+  // Two buffers as four variables: the compiler then sees that a read of one does not have to wait
   // for the direct loads that are under way into another.
   __shared__ __attribute__((aligned(16))) char a0[TA::BYTES], b0[TB::BYTES], a1[TA::BYTES],
       b1[TB::BYTES];
@@ -536,12 +556,31 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void pro
     multiply(1);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // written sums before the first matrix instruction reads them
-  if constexpr (FI * FJ >= 64) asm volatile("s_nop 7" ::: "memory");
+  // (the sums stand in their registers before the wait, and are taken from them behind the next)
+  auto pin = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) asm volatile("" : "+a"(acc[i][j]));
+  };
+  if constexpr (FI * FJ >= 64) {
+    // written sums before the first matrix instruction reads them
+    pin();
+    asm volatile("s_nop 7" ::: "memory");
+  }
   start(a0, b0);
-  settle(a0, b0);
-  read(a0, b0, 0);
-  start(a1, b1);
+  if constexpr (DIRECT) {
+    // the second step's loads follow at once; the first is there when only they are under way
+    start(a1, b1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TA::LOADS + TB::LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(a0, b0, 0);
+  } else {
+    settle(a0, b0);
+    read(a0, b0, 0);
+    start(a1, b1);
+  }
   if constexpr (FI * FJ >= 64) {
     // (a step past the end multiplies zeros)
     for (; s < end; s += 2) {
@@ -561,7 +600,10 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void pro
     }
   }
   // the last matrix instructions, 8 passes of 4 cycles, before their sums are read
-  if constexpr (FI * FJ >= 64) asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  if constexpr (FI * FJ >= 64) {
+    asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+    pin();
+  }
   // what is still under way into LDS (zeros, or nothing) arrives before LDS is used otherwise
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
@@ -570,7 +612,8 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2) void pro
   // the sums turn through this wave's own part of LDS, HJ of the FJ columns of fragments at a time
   constexpr int HJ = FJ / PASSES;
   constexpr int SHARE = WI * HJ * 16 * 4;
-  static_assert(NW == 4 && SHARE <= (TA::BYTES < TB::BYTES ? TA::BYTES : TB::BYTES), "a buffer a wave");
+  static_assert(NW == 4 && SHARE <= (TA::BYTES < TB::BYTES ? TA::BYTES : TB::BYTES),
+                "a buffer a wave");
   float* tile = (float*)(wave == 0 ? a0 : wave == 1 ? b0 : wave == 2 ? a1 : b1);
   auto pass = [&](auto which) __attribute__((always_inline)) {
     constexpr int h = decltype(which)::value;
