@@ -357,28 +357,43 @@ PWC_API int pwc_rotary(const void* x, void* y, const void* positions, const void
                        void* stream);
 
 /* y = act(x weight^T + bias) + residual; weight [O][K], bias [O] or NULL, residual like y or
- * NULL. */
+ * NULL.  The workspace holds copies of x and weight with rows at 16-byte places, where they are not
+ * and the call is large enough to gain by it (of the pointers given to the size functions only the
+ * alignment is looked at; a size of 0 means that none is used). */
+PWC_API size_t pwc_linear_forward_workspace_size(const void* x, const void* weight, int layout,
+                                                 long long B, long long P, int K, int O,
+                                                 long long x_stride, int dtype);
 PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bias,
                                const void* residual, void* y, int layout, long long B, long long P,
                                int K, int O, long long x_stride, int activation,
-                               float negative_slope, int dtype, void* stream);
-/* grad_x, grad_weight, grad_bias (each may be NULL: not computed).  The residual's
- * gradient is grad_out itself.  Deterministic. */
-PWC_API size_t pwc_linear_backward_workspace_size(int layout, long long B, long long P, int K,
-                                                  int O, int activation, int dtype);
+                               float negative_slope, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* grad_x, grad_weight, grad_bias (each may be NULL: not computed).  The residual's gradient is
+ * grad_out itself.  Deterministic.  The size is that of all three. */
+PWC_API size_t pwc_linear_backward_workspace_size(const void* x, const void* weight,
+                                                  const void* grad_out, int layout, long long B,
+                                                  long long P, int K, int O, long long x_stride,
+                                                  int activation, int dtype);
 PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* bias,
                                 const void* grad_out, void* grad_x, void* grad_weight,
                                 void* grad_bias, int layout, long long B, long long P, int K,
                                 int O, long long x_stride, int activation, float negative_slope,
                                 int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
-/* y = act(x Wg^T + bg) * (x Wu^T + bu); weight [2 * O][K] = [Wg; Wu], bias [2 * O] or NULL. */
+/* y = act(x Wg^T + bg) * (x Wu^T + bu); weight [2 * O][K] = [Wg; Wu], bias [2 * O] or NULL;
+ * workspaces as above. */
+PWC_API size_t pwc_gated_linear_forward_workspace_size(const void* x, const void* weight,
+                                                       int layout, long long B, long long P, int K,
+                                                       int O, long long x_stride, int dtype);
 PWC_API int pwc_gated_linear_forward(const void* x, const void* weight, const void* bias, void* y,
                                      int layout, long long B, long long P, int K, int O,
                                      long long x_stride, int activation, float negative_slope,
-                                     int dtype, void* stream);
-PWC_API size_t pwc_gated_linear_backward_workspace_size(int layout, long long B, long long P,
-                                                        int K, int O, int dtype);
+                                     int dtype, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+PWC_API size_t pwc_gated_linear_backward_workspace_size(const void* x, const void* weight,
+                                                        const void* grad_out, int layout,
+                                                        long long B, long long P, int K, int O,
+                                                        long long x_stride, int dtype);
 PWC_API int pwc_gated_linear_backward(const void* x, const void* weight, const void* bias,
                                       const void* grad_out, void* grad_x, void* grad_weight,
                                       void* grad_bias, int layout, long long B, long long P, int K,

@@ -23,18 +23,19 @@ using torch::autograd::variable_list;
 namespace py = pybind11;
 
 // ---- the C entries ----
+#define PWC_ENTRIES(E)                                                                    \
+  E(pwc_last_error) E(pwc_rotary)                                                         \
+  E(pwc_layer_norm_forward) E(pwc_layer_norm_backward_workspace_size)                     \
+  E(pwc_layer_norm_backward)                                                              \
+  E(pwc_linear_forward_workspace_size) E(pwc_linear_forward)                              \
+  E(pwc_linear_backward_workspace_size) E(pwc_linear_backward)                            \
+  E(pwc_gated_linear_forward_workspace_size) E(pwc_gated_linear_forward)                  \
+  E(pwc_gated_linear_backward_workspace_size) E(pwc_gated_linear_backward)
+
 struct Entries {
-  decltype(&pwc_last_error) last_error = nullptr;
-  decltype(&pwc_layer_norm_forward) norm_forward = nullptr;
-  decltype(&pwc_layer_norm_backward_workspace_size) norm_backward_size = nullptr;
-  decltype(&pwc_layer_norm_backward) norm_backward = nullptr;
-  decltype(&pwc_rotary) rotary = nullptr;
-  decltype(&pwc_linear_forward) linear_forward = nullptr;
-  decltype(&pwc_linear_backward_workspace_size) linear_backward_size = nullptr;
-  decltype(&pwc_linear_backward) linear_backward = nullptr;
-  decltype(&pwc_gated_linear_forward) gated_forward = nullptr;
-  decltype(&pwc_gated_linear_backward_workspace_size) gated_backward_size = nullptr;
-  decltype(&pwc_gated_linear_backward) gated_backward = nullptr;
+#define E(name) decltype(&::name) name = nullptr;
+  PWC_ENTRIES(E)
+#undef E
 };
 Entries g_entries;
 std::atomic<bool> g_bound{false};
@@ -47,27 +48,25 @@ const Entries& entries() {
   return g_entries;
 }
 
-void bind(const py::dict& at) {
-  auto set = [&](const char* name, auto& entry) {
-    entry = reinterpret_cast<std::remove_reference_t<decltype(entry)>>(
-        at[name].cast<uintptr_t>());
+std::vector<std::string> entry_names() {
+  return {
+#define E(name) #name,
+      PWC_ENTRIES(E)
+#undef E
   };
-  set("pwc_last_error", g_entries.last_error);
-  set("pwc_layer_norm_forward", g_entries.norm_forward);
-  set("pwc_layer_norm_backward_workspace_size", g_entries.norm_backward_size);
-  set("pwc_layer_norm_backward", g_entries.norm_backward);
-  set("pwc_rotary", g_entries.rotary);
-  set("pwc_linear_forward", g_entries.linear_forward);
-  set("pwc_linear_backward_workspace_size", g_entries.linear_backward_size);
-  set("pwc_linear_backward", g_entries.linear_backward);
-  set("pwc_gated_linear_forward", g_entries.gated_forward);
-  set("pwc_gated_linear_backward_workspace_size", g_entries.gated_backward_size);
-  set("pwc_gated_linear_backward", g_entries.gated_backward);
+}
+
+void bind(const py::dict& at) {
+  Entries e;
+#define E(name) e.name = reinterpret_cast<decltype(e.name)>(at[#name].cast<uintptr_t>());
+  PWC_ENTRIES(E)
+#undef E
+  g_entries = e;
   g_bound.store(true, std::memory_order_release);
 }
 
 void called(int ok, const char* what) {
-  TORCH_CHECK(ok == 1, what, " aborting: ", g_entries.last_error());
+  TORCH_CHECK(ok == 1, what, " aborting: ", g_entries.pwc_last_error());
 }
 
 // ---- checks ----
@@ -203,7 +202,7 @@ Norm norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps,
     r.rstd = at::empty({m.B * m.P}, x.options().dtype(at::kFloat));
   }
   if (r.y.numel())
-    called(entries().norm_forward(ptr(m.x), ptr(wv), ptr(bv), out(r.y), out(r.mean), out(r.rstd),
+    called(entries().pwc_layer_norm_forward(ptr(m.x), ptr(wv), ptr(bv), out(r.y), out(r.mean), out(r.rstd),
                                   m.layout, m.B, m.P, to_int(m.C, what), m.stride, (float)eps,
                                   dtype_code(x.scalar_type()), stream_of(x)),
            "LayerNorm_forward");
@@ -236,9 +235,9 @@ Grads norm_backward(const Tensor& x, const Tensor& w, const Tensor& dy, const Te
   const Entries& e = entries();
   const int dt = dtype_code(x.scalar_type()), C = to_int(m.C, what);
   const size_t bytes =
-      needs.w || needs.b ? e.norm_backward_size(m.layout, m.B, m.P, C, dt) : 0;
+      needs.w || needs.b ? e.pwc_layer_norm_backward_workspace_size(m.layout, m.B, m.P, C, dt) : 0;
   const Tensor ws = workspace(bytes, x);
-  called(e.norm_backward(ptr(m.x), ptr(wv), ptr(g), ptr(mean), ptr(rstd), out(r.x), out(r.w),
+  called(e.pwc_layer_norm_backward(ptr(m.x), ptr(wv), ptr(g), ptr(mean), ptr(rstd), out(r.x), out(r.w),
                          out(r.b), m.layout, m.B, m.P, C, m.stride, dt, out(ws), bytes,
                          stream_of(x)),
          "LayerNorm_backward");
@@ -312,7 +311,7 @@ Tensor rotary_forward(const Tensor& x, const Tensor& inv_freq, const Tensor& axi
     s.y_stride[k] = y.stride(k);
   }
   if (y.numel())
-    called(entries().rotary(ptr(x), out(y), ptr(positions), ptr(f), ptr(a), &s, inverse,
+    called(entries().pwc_rotary(ptr(x), out(y), ptr(positions), ptr(f), ptr(a), &s, inverse,
                             dtype_code(x.scalar_type()), stream_of(x)),
            what);
   return y;
@@ -371,11 +370,16 @@ Tensor product_forward(bool gated, const Tensor& x, const Tensor& w, const Tenso
   const int dt = dtype_code(x.scalar_type());
   const Matrix& m = p.m;
   const Entries& e = entries();
-  called(gated ? e.gated_forward(ptr(m.x), ptr(p.w), ptr(p.b), out(y), m.layout, m.B, m.P, p.K,
-                                 p.O, m.stride, (int)act, (float)slope, dt, stream_of(x))
-               : e.linear_forward(ptr(m.x), ptr(p.w), ptr(p.b), ptr(res), out(y), m.layout, m.B,
-                                  m.P, p.K, p.O, m.stride, (int)act, (float)slope, dt,
-                                  stream_of(x)),
+  const size_t bytes =
+      (gated ? e.pwc_gated_linear_forward_workspace_size : e.pwc_linear_forward_workspace_size)(
+          ptr(m.x), ptr(p.w), m.layout, m.B, m.P, p.K, p.O, m.stride, dt);
+  const Tensor ws = workspace(bytes, x);
+  called(gated ? e.pwc_gated_linear_forward(ptr(m.x), ptr(p.w), ptr(p.b), out(y), m.layout, m.B,
+                                            m.P, p.K, p.O, m.stride, (int)act, (float)slope, dt,
+                                            out(ws), bytes, stream_of(x))
+               : e.pwc_linear_forward(ptr(m.x), ptr(p.w), ptr(p.b), ptr(res), out(y), m.layout,
+                                      m.B, m.P, p.K, p.O, m.stride, (int)act, (float)slope, dt,
+                                      out(ws), bytes, stream_of(x)),
          what);
   return y;
 }
@@ -397,11 +401,13 @@ Grads product_backward(bool gated, const Tensor& x, const Tensor& w, const Tenso
   const Entries& e = entries();
   const Matrix& m = p.m;
   const int dt = dtype_code(x.scalar_type());
-  const size_t bytes = gated
-                           ? e.gated_backward_size(m.layout, m.B, m.P, p.K, p.O, dt)
-                           : e.linear_backward_size(m.layout, m.B, m.P, p.K, p.O, (int)act, dt);
+  const size_t bytes =
+      gated ? e.pwc_gated_linear_backward_workspace_size(ptr(m.x), ptr(p.w), ptr(g), m.layout, m.B,
+                                                         m.P, p.K, p.O, m.stride, dt)
+            : e.pwc_linear_backward_workspace_size(ptr(m.x), ptr(p.w), ptr(g), m.layout, m.B, m.P,
+                                                   p.K, p.O, m.stride, (int)act, dt);
   const Tensor ws = workspace(bytes, x);
-  const auto call = gated ? e.gated_backward : e.linear_backward;
+  const auto call = gated ? e.pwc_gated_linear_backward : e.pwc_linear_backward;
   called(call(ptr(m.x), ptr(p.w), ptr(p.b), ptr(g), out(r.x), out(r.w), out(r.b), m.layout, m.B,
               m.P, p.K, p.O, m.stride, (int)act, (float)slope, dt, out(ws), bytes, stream_of(x)),
          what);
@@ -565,6 +571,7 @@ PYBIND11_MODULE(_features_ext, m) {
   const auto nogil = py::call_guard<py::gil_scoped_release>();
   const All every(true, true, true);
   m.def("bind", &bind);
+  m.def("entries", &entry_names);
   m.def("by_rows", [](const std::vector<int64_t>& shape, int64_t dim, const std::string& what) {
     return by_rows(shape, dim, what.c_str());
   });

@@ -58,97 +58,200 @@ const char* bad_problem(const Problem& p) {
 
 Problem problem(int layout, long long B, long long P, int K, int O, long long x_stride, int act,
                 float slope, int dtype, int gated) {
-  Problem p = {layout, K, O, gated ? 2 * O : O, act, dtype, gated, B, P, 0, x_stride, slope};
+  Problem p = {layout, K, O, O, act, dtype, gated, B, P, 0, x_stride, slope};
+  if (gated && O > 0 && O <= (1 << 23)) p.rows = 2 * O;  // (larger ones are refused)
   p.M = layout == PWC_LAYOUT_MAP && B >= 0 && P >= 0 && B <= kIntMax && P <= kIntMax ? B * P : P;
   return p;
 }
 
+bool tokens(const Problem& p) { return p.layout == PWC_LAYOUT_TOKENS; }
+bool needs_z(const Problem& p) { return p.gated || p.act != kActNone; }
+size_t elem(int dtype) { return dtype == 0 ? 4 : 2; }
+
+// A matrix as the products read it: rows of `cols` values, `row` apart (tokens' channels, W's
+// channels, or a channel's pixels), images `image` apart; `padded`: zeros to the next 16 bytes.
+struct View {
+  const void* at;
+  long long row, image;
+  int padded;
+};
+View x_view(const Problem& p, const void* x) {
+  if (tokens(p)) return {x, p.x_stride, 0, 0};
+  return {x, p.P, p.x_stride, 0};
+}
+View w_view(const Problem& p, const void* w) { return {w, p.K, 0, 0}; }
+View dz_view(const Problem& p, const void* dz) {
+  if (tokens(p)) return {dz, p.rows, 0, 0};
+  return {dz, p.P, p.rows * p.P, 0};
+}
+
+// The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
+// not, large ones are laid out so first: rows of odd 16-bit lengths read through registers cost the
+// three backward products 2 to 7 times their time (8191 x 1023 -> 4095: 1.2 ms instead of 0.25),
+// the copies tens of microseconds.  Small calls, and 32-bit ones below 8 GFLOP, read them as they
+// lie.
+bool pads_pay(const Problem& p) {
+  return 2.0 * (double)p.M * p.rows * p.K >= (p.dtype == 0 ? 8e9 : 2e9);
+}
+long long whole(const Problem& p, long long cols) {
+  const long long e = 16 / (long long)elem(p.dtype);
+  return (cols + e - 1) / e * e;
+}
+bool lies_well(const Problem& p, const View& v, long long cols) {
+  return aligned_to(v.at, 16) && whole(p, v.row) == v.row && whole(p, v.image) == v.image &&
+         whole(p, cols) == cols;
+}
+long long x_cols(const Problem& p) { return tokens(p) ? p.K : p.P; }
+long long x_rows(const Problem& p) { return tokens(p) ? p.M : p.B * p.K; }
+long long dz_cols(const Problem& p) { return tokens(p) ? p.rows : p.P; }
+long long dz_rows(const Problem& p) { return tokens(p) ? p.M : p.B * p.rows; }
+View padded_x(const Problem& p, const void* at) {
+  const long long row = whole(p, x_cols(p));
+  return {at, row, tokens(p) ? 0 : p.K * row, 1};
+}
+View padded_w(const Problem& p, const void* at) { return {at, whole(p, p.K), 0, 1}; }
+View padded_dz(const Problem& p, const void* at) {
+  const long long row = whole(p, dz_cols(p));
+  return {at, row, tokens(p) ? 0 : p.rows * row, 1};
+}
+
 // z = x W^T + b into the epilogue `mode`, whose output has `out_rows` channels
-ProductArgs forward_args(const Problem& p, const void* x, const void* w, const void* bias,
-                         const void* other, void* out, int mode, int out_rows) {
+ProductArgs forward_args(const Problem& p, const View& x, const View& w, const void* bias,
+                         const void* other, const View& out, int mode) {
   ProductArgs g = blank();
   g.K = p.K;
   g.bias = bias;
   g.other = other;
-  g.out = out;
+  g.out = const_cast<void*>(out.at);
+  g.ldo = out.row;
+  g.out_batch = out.image;
   g.mode = mode;
   g.act = p.act;
   g.slope = p.slope;
   g.pair = p.gated ? p.O : 0;
-  if (p.layout == PWC_LAYOUT_TOKENS) {
-    g.a = w, g.lda = p.K, g.a_k = 1, g.I = p.rows;
-    g.b = x, g.ldb = p.x_stride, g.b_k = 1, g.J = (int)p.M;
-    g.ldo = out_rows;
+  if (tokens(p)) {
+    g.a = w.at, g.lda = w.row, g.a_pad = w.padded, g.a_k = 1, g.I = p.rows;
+    g.b = x.at, g.ldb = x.row, g.b_pad = x.padded, g.b_k = 1, g.J = (int)p.M;
     g.ldother = p.O;
     g.channel_i = 1;
   } else {
-    g.a = x, g.lda = p.P, g.a_batch = p.x_stride, g.a_k = 0, g.I = (int)p.P;
-    g.b = w, g.ldb = p.K, g.b_k = 1, g.J = p.rows;
+    g.a = x.at, g.lda = x.row, g.a_batch = x.image, g.a_pad = x.padded, g.a_k = 0, g.I = (int)p.P;
+    g.b = w.at, g.ldb = w.row, g.b_pad = w.padded, g.b_k = 1, g.J = p.rows;
     g.batches = (int)p.B;
-    g.ldo = p.P, g.out_batch = (long long)out_rows * p.P;
     g.ldother = p.P, g.other_batch = (long long)p.O * p.P;
   }
   return g;
 }
-
-bool needs_z(const Problem& p) { return p.gated || p.act != kActNone; }
-size_t elem(int dtype) { return dtype == 0 ? 4 : 2; }
-
-ProductArgs dz_args(const Problem& p, const void* x, const void* w, const void* bias,
-                    const void* dy, void* dz) {
-  return forward_args(p, x, w, bias, dy, dz, p.gated ? kGatedDz : kLinearDz, p.rows);
+ProductArgs y_args(const Problem& p, const View& x, const View& w, const void* bias,
+                   const void* res, void* y) {
+  View out = {y, p.O, 0, 0};
+  if (!tokens(p)) out.row = p.P, out.image = (long long)p.O * p.P;
+  return forward_args(p, x, w, bias, res, out, p.gated ? kGated : kLinear);
+}
+ProductArgs dz_args(const Problem& p, const View& x, const View& w, const void* bias,
+                    const void* dy, const View& dz) {
+  return forward_args(p, x, w, bias, dy, dz, p.gated ? kGatedDz : kLinearDz);
+}
+ProductArgs dx_args(const Problem& p, const View& dz, const View& w, void* dx) {
+  ProductArgs g = blank();
+  g.K = p.rows;
+  g.out = dx;
+  g.mode = kPlain;
+  if (tokens(p)) {
+    g.a = w.at, g.lda = w.row, g.a_pad = w.padded, g.a_k = 0, g.I = p.K;
+    g.b = dz.at, g.ldb = dz.row, g.b_pad = dz.padded, g.b_k = 1, g.J = (int)p.M;
+    g.ldo = p.K;
+  } else {
+    g.a = dz.at, g.lda = dz.row, g.a_batch = dz.image, g.a_pad = dz.padded, g.a_k = 0;
+    g.I = (int)p.P;
+    g.b = w.at, g.ldb = w.row, g.b_pad = w.padded, g.b_k = 0, g.J = p.K;
+    g.batches = (int)p.B;
+    g.ldo = p.P, g.out_batch = (long long)p.K * p.P;
+  }
+  return g;
 }
 // dW = dz^T x in 32-bit parts (`out`), or itself where there is one split
-ProductArgs dw_args(const Problem& p, const void* x, const void* dz, void* out) {
+ProductArgs dw_args(const Problem& p, const View& x, const View& dz, void* out) {
   ProductArgs g = blank();
   g.mode = kPartial;
   g.out = out;
   g.I = p.K;
   g.J = p.rows;
   g.ldo = p.K;
-  if (p.layout == PWC_LAYOUT_TOKENS) {
+  g.a = x.at, g.lda = x.row, g.a_pad = x.padded;
+  g.b = dz.at, g.ldb = dz.row, g.b_pad = dz.padded;
+  if (tokens(p)) {
     g.K = (int)p.M;
-    g.a = x, g.lda = p.x_stride, g.a_k = 0;
-    g.b = dz, g.ldb = p.rows, g.b_k = 0;
   } else {
     g.K = (int)p.P;
     g.segments = (int)p.B;
-    g.a = x, g.lda = p.P, g.a_segment = p.x_stride, g.a_k = 1;
-    g.b = dz, g.ldb = p.P, g.b_segment = (long long)p.rows * p.P, g.b_k = 1;
+    g.a_segment = x.image, g.a_k = 1;
+    g.b_segment = dz.image, g.b_k = 1;
   }
   return g;
 }
 
-struct BackwardSpace {
-  size_t part, sums, total;  // bytes from the start; dz lies at 0
-  int splits, rows;          // rows of partial bias gradients
+// ---- workspaces, as places from their start ----
+struct ForwardSpace {
+  bool pad_x, pad_w;
+  size_t w, total;  // the padded x lies at 0
 };
-BackwardSpace backward_space(const Problem& p, int splits, int rows) {
-  BackwardSpace s = {};
-  s.splits = splits;
-  s.rows = rows;
-  s.part = needs_z(p) ? align256((size_t)p.M * p.rows * elem(p.dtype)) : 0;
-  s.sums = s.part + (splits > 1 ? align256((size_t)splits * p.rows * p.K * 4) : 0);
-  s.total = s.sums + align256((size_t)rows * p.rows * 4);
+size_t bytes_of(const Problem& p, long long rows, long long cols) {
+  return align256((size_t)rows * whole(p, cols) * elem(p.dtype));
+}
+ForwardSpace forward_space(const Problem& p, const void* x, const void* w) {
+  ForwardSpace s = {};
+  const ProductPlan plan = product_plan(
+      y_args(p, x_view(p, x), w_view(p, w), nullptr, nullptr, nullptr), p.dtype);
+  const bool few = plan.kernel == kFew16 || plan.kernel == kFew32 || plan.kernel == kFew64;
+  if (few || !pads_pay(p)) return s;
+  s.pad_x = !lies_well(p, x_view(p, x), x_cols(p));
+  s.pad_w = !lies_well(p, w_view(p, w), p.K);
+  s.w = s.pad_x ? bytes_of(p, x_rows(p), x_cols(p)) : 0;
+  s.total = s.w + (s.pad_w ? bytes_of(p, p.rows, p.K) : 0);
   return s;
 }
-// (of the pointers only the alignment matters)
-int dw_splits(const Problem& p, const void* x, const void* dz) {
-  return product_plan(dw_args(p, x, dz, nullptr), p.dtype).splits;
-}
-int db_rows(const Problem& p, const void* x, const void* w) {
-  return needs_z(p) ? product_sum_rows(dz_args(p, x, w, nullptr, nullptr, nullptr), p.dtype)
-                    : product_column_parts(p.layout, p.B, p.P, p.rows);
-}
-size_t most_backward_space(const Problem& p) {
-  if (bad_problem(p) || p.M == 0) return 0;
-  int splits = 0, rows = 0;
-  for (const void* at : {(const void*)nullptr, (const void*)1}) {
-    const int s = dw_splits(p, at, at), r = db_rows(p, at, at);
-    if (s > splits) splits = s;
-    if (r > rows) rows = r;
+
+struct BackwardSpace {
+  bool pad_x, pad_w, pad_dz;
+  size_t x, w, part, sums, total;  // dz, or the padded dy, lies at 0
+  int splits, rows;                // rows of partial bias gradients
+  View xv, wv, dzv;                // as the products take them
+};
+BackwardSpace backward_space(const Problem& p, const void* x, const void* w, const void* dy,
+                             const char* ws, bool dx, bool dw, bool db) {
+  BackwardSpace s = {};
+  const bool z = needs_z(p), pay = pads_pay(p);
+  s.xv = x_view(p, x), s.wv = w_view(p, w), s.dzv = dz_view(p, z ? nullptr : dy);
+  s.pad_x = pay && (z || dw) && !lies_well(p, s.xv, x_cols(p));
+  s.pad_w = pay && (z || dx) && !lies_well(p, s.wv, p.K);
+  s.pad_dz = pay && (z || dx || dw) && !lies_well(p, s.dzv, dz_cols(p));
+  size_t at = 0;
+  if (s.pad_dz)
+    at += bytes_of(p, dz_rows(p), dz_cols(p));
+  else if (z)
+    at += align256((size_t)p.M * p.rows * elem(p.dtype));
+  s.x = at;
+  if (s.pad_x) at += bytes_of(p, x_rows(p), x_cols(p));
+  s.w = at;
+  if (s.pad_w) at += bytes_of(p, p.rows, p.K);
+  if (s.pad_x) s.xv = padded_x(p, ws + s.x);
+  if (s.pad_w) s.wv = padded_w(p, ws + s.w);
+  if (s.pad_dz)
+    s.dzv = padded_dz(p, ws);
+  else if (z)
+    s.dzv = dz_view(p, ws);
+  s.splits = dw ? product_plan(dw_args(p, s.xv, s.dzv, nullptr), p.dtype).splits : 1;
+  s.part = at;
+  if (s.splits > 1) at += align256((size_t)s.splits * p.rows * p.K * 4);
+  s.sums = at;
+  if (db) {
+    s.rows = z ? product_sum_rows(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype)
+               : product_column_parts(p.layout, p.B, p.P, p.rows);
+    at += align256((size_t)s.rows * p.rows * 4);
   }
-  return backward_space(p, splits, rows).total;
+  s.total = at;
+  return s;
 }
 
 int product_backward(const char* fn, const Problem& p, const void* x, const void* w,
@@ -163,66 +266,68 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
   }
   if (!x || !w || !dy) return api_fail(fn, "null buffer");
   if (!dx && !dw && !db) return api_launch(fn, hipSuccess);
-  const BackwardSpace s = backward_space(
-      p, dw ? dw_splits(p, x, needs_z(p) ? nullptr : dy) : 1, db ? db_rows(p, x, w) : 0);
+  char* ws = (char*)workspace;
+  const BackwardSpace s = backward_space(p, x, w, dy, ws, dx, dw, db);
   if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
   if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
-  char* ws = (char*)workspace;
-  const void* dz = dy;
-  if (needs_z(p)) {
-    ProductArgs g = dz_args(p, x, w, bias, dy, ws);
+  hipError_t e = hipSuccess;
+  if (s.pad_x)
+    e = product_pad(x_view(p, x).at, x_view(p, x).row, x_view(p, x).image, ws + s.x,
+                    tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype, stream);
+  if (s.pad_w && e == hipSuccess)
+    e = product_pad(w, p.K, 0, ws + s.w, p.rows, p.rows, p.K, p.dtype, stream);
+  if (e == hipSuccess && needs_z(p)) {
+    ProductArgs g = dz_args(p, s.xv, s.wv, bias, dy, s.dzv);
     g.sums = db ? (float*)(ws + s.sums) : nullptr;
-    const hipError_t e = product_launch(g, p.dtype, stream);
-    if (e != hipSuccess) return api_launch(fn, e);
-    dz = ws;
+    e = product_launch(g, p.dtype, stream);
+    if (s.pad_dz && e == hipSuccess)
+      e = product_zero_tails(ws, dz_rows(p), dz_cols(p), p.dtype, stream);
+  } else if (e == hipSuccess && s.pad_dz) {
+    const View v = dz_view(p, dy);
+    e = product_pad(dy, v.row, v.image, ws, tokens(p) ? p.M : p.rows, dz_rows(p), dz_cols(p),
+                    p.dtype, stream);
   }
-  const long long dz_image = (long long)p.rows * p.P;
-  if (dx) {
-    ProductArgs g = blank();
-    g.K = p.rows;
-    g.out = dx;
-    g.mode = kPlain;
-    if (p.layout == PWC_LAYOUT_TOKENS) {
-      g.a = w, g.lda = p.K, g.a_k = 0, g.I = p.K;
-      g.b = dz, g.ldb = p.rows, g.b_k = 1, g.J = (int)p.M;
-      g.ldo = p.K;
-    } else {
-      g.a = dz, g.lda = p.P, g.a_batch = dz_image, g.a_k = 0, g.I = (int)p.P;
-      g.b = w, g.ldb = p.K, g.b_k = 0, g.J = p.K;
-      g.batches = (int)p.B;
-      g.ldo = p.P, g.out_batch = (long long)p.K * p.P;
-    }
-    const hipError_t e = product_launch(g, p.dtype, stream);
-    if (e != hipSuccess) return api_launch(fn, e);
-  }
-  if (dw) {
-    ProductArgs g = dw_args(p, x, dz, s.splits > 1 ? (void*)(ws + s.part) : dw);
+  if (dx && e == hipSuccess) e = product_launch(dx_args(p, s.dzv, s.wv, dx), p.dtype, stream);
+  if (dw && e == hipSuccess) {
+    ProductArgs g = dw_args(p, s.xv, s.dzv, s.splits > 1 ? (void*)(ws + s.part) : dw);
     g.splits = s.splits;
-    hipError_t e = product_launch(g, p.dtype, stream);
+    e = product_launch(g, p.dtype, stream);
     if (e == hipSuccess && s.splits > 1)
       e = product_add_splits((const float*)(ws + s.part), dw, (long long)p.rows * p.K, s.splits,
                              p.dtype, stream);
-    if (e != hipSuccess) return api_launch(fn, e);
   }
-  if (db) {
+  if (db && e == hipSuccess) {
     float* sums = (float*)(ws + s.sums);
-    hipError_t e = hipSuccess;
     if (!needs_z(p))
       e = product_column_sums(dy, sums, p.layout, p.B, p.P, p.rows, s.rows, p.dtype, stream);
     if (e == hipSuccess) e = sum_rows(sums, db, p.rows, s.rows, p.dtype, stream);
-    if (e != hipSuccess) return api_launch(fn, e);
   }
-  return api_launch(fn, hipSuccess);
+  return api_launch(fn, e);
 }
 
 int product_forward(const char* fn, const Problem& p, const void* x, const void* w,
-                    const void* bias, const void* res, void* y, hipStream_t stream) {
+                    const void* bias, const void* res, void* y, void* workspace, size_t bytes,
+                    hipStream_t stream) {
   if (const char* e = bad_problem(p)) return api_fail(fn, e);
   if (p.M == 0) return api_launch(fn, hipSuccess);
   if (!x || !w || !y) return api_fail(fn, "null buffer");
-  return api_launch(fn, product_launch(forward_args(p, x, w, bias, res, y,
-                                                    p.gated ? kGated : kLinear, p.O),
-                                       p.dtype, stream));
+  const ForwardSpace s = forward_space(p, x, w);
+  if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
+  if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
+  char* ws = (char*)workspace;
+  View xv = x_view(p, x), wv = w_view(p, w);
+  hipError_t e = hipSuccess;
+  if (s.pad_x) {
+    e = product_pad(x, xv.row, xv.image, ws, tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype,
+                    stream);
+    xv = padded_x(p, ws);
+  }
+  if (s.pad_w && e == hipSuccess) {
+    e = product_pad(w, p.K, 0, ws + s.w, p.rows, p.rows, p.K, p.dtype, stream);
+    wv = padded_w(p, ws + s.w);
+  }
+  if (e == hipSuccess) e = product_launch(y_args(p, xv, wv, bias, res, y), p.dtype, stream);
+  return api_launch(fn, e);
 }
 
 NormArgs norm_args(int layout, long long B, long long P, int C, long long x_stride) {
@@ -355,20 +460,31 @@ PWC_API int pwc_rotary(const void* x, void* y, const void* positions, const void
   return api_launch(fn, rotary_launch(a, dtype, (hipStream_t)stream));
 }
 
+PWC_API size_t pwc_linear_forward_workspace_size(const void* x, const void* weight, int layout,
+                                                 long long B, long long P, int K, int O,
+                                                 long long x_stride, int dtype) {
+  const Problem p = problem(layout, B, P, K, O, x_stride, 0, 0.f, dtype, 0);
+  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight).total;
+}
+
 PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bias,
                                const void* residual, void* y, int layout, long long B, long long P,
                                int K, int O, long long x_stride, int activation,
-                               float negative_slope, int dtype, void* stream) {
+                               float negative_slope, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   return product_forward("pwc_linear_forward",
                          problem(layout, B, P, K, O, x_stride, activation, negative_slope, dtype, 0),
-                         x, weight, bias, residual, y, (hipStream_t)stream);
+                         x, weight, bias, residual, y, workspace, workspace_bytes,
+                         (hipStream_t)stream);
 }
 
-PWC_API size_t pwc_linear_backward_workspace_size(int layout, long long B, long long P, int K,
-                                                  int O, int activation, int dtype) {
-  const Problem p = problem(layout, B, P, K, O, layout == PWC_LAYOUT_MAP ? P * K : K, activation,
-                            0.f, dtype, 0);
-  return most_backward_space(p);
+PWC_API size_t pwc_linear_backward_workspace_size(const void* x, const void* weight,
+                                                  const void* grad_out, int layout, long long B,
+                                                  long long P, int K, int O, long long x_stride,
+                                                  int activation, int dtype) {
+  const Problem p = problem(layout, B, P, K, O, x_stride, activation, 0.f, dtype, 0);
+  if (bad_problem(p) || p.M == 0) return 0;
+  return backward_space(p, x, weight, grad_out, nullptr, true, true, true).total;
 }
 
 PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* bias,
@@ -383,20 +499,31 @@ PWC_API int pwc_linear_backward(const void* x, const void* weight, const void* b
                           workspace_bytes, (hipStream_t)stream);
 }
 
+PWC_API size_t pwc_gated_linear_forward_workspace_size(const void* x, const void* weight,
+                                                       int layout, long long B, long long P, int K,
+                                                       int O, long long x_stride, int dtype) {
+  const Problem p = problem(layout, B, P, K, O, x_stride, 0, 0.f, dtype, 1);
+  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight).total;
+}
+
 PWC_API int pwc_gated_linear_forward(const void* x, const void* weight, const void* bias, void* y,
                                      int layout, long long B, long long P, int K, int O,
                                      long long x_stride, int activation, float negative_slope,
-                                     int dtype, void* stream) {
+                                     int dtype, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
   return product_forward("pwc_gated_linear_forward",
                          problem(layout, B, P, K, O, x_stride, activation, negative_slope, dtype, 1),
-                         x, weight, bias, nullptr, y, (hipStream_t)stream);
+                         x, weight, bias, nullptr, y, workspace, workspace_bytes,
+                         (hipStream_t)stream);
 }
 
-PWC_API size_t pwc_gated_linear_backward_workspace_size(int layout, long long B, long long P,
-                                                        int K, int O, int dtype) {
-  const Problem p = problem(layout, B, P, K, O, layout == PWC_LAYOUT_MAP ? P * K : K, 0, 0.f,
-                            dtype, 1);
-  return most_backward_space(p);
+PWC_API size_t pwc_gated_linear_backward_workspace_size(const void* x, const void* weight,
+                                                        const void* grad_out, int layout,
+                                                        long long B, long long P, int K, int O,
+                                                        long long x_stride, int dtype) {
+  const Problem p = problem(layout, B, P, K, O, x_stride, 0, 0.f, dtype, 1);
+  if (bad_problem(p) || p.M == 0) return 0;
+  return backward_space(p, x, weight, grad_out, nullptr, true, true, true).total;
 }
 
 PWC_API int pwc_gated_linear_backward(const void* x, const void* weight, const void* bias,

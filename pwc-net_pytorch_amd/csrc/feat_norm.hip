@@ -173,118 +173,191 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
 }
 
 // ------------------------------------------------------------------------------ maps [B][C][P]
-// A block takes 64 pixels; wave g of G holds channels g, g + G, ... of them in registers.
-constexpr int kMapChannels = 16;  // of a thread; more channels (> 256) go by the loops below
+// A block takes 64 PV pixels, a lane PV neighbours (4 bytes of 16-bit values where P is even); wave
+// g of G holds NC channels g, g + G, ... in registers; more than 256 channels go by the loops below.
 
-template <int G> __device__ __forceinline__ float pixel_sum(float v, float (*red)[64]) {
+template <int G, int PV>
+__device__ __forceinline__ void pixel_sum(float (&v)[PV], float (*red)[64 * PV]) {
   if constexpr (G > 1) {
     const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
     __syncthreads();
-    red[g][l] = v;
-    __syncthreads();
-    v = 0.f;
 #pragma unroll
-    for (int k = 0; k < G; ++k) v += red[k][l];
+    for (int e = 0; e < PV; ++e) red[g][l * PV + e] = v[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PV; ++e) {
+      v[e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) v[e] += red[k][l * PV + e];
+    }
   }
-  return v;
+}
+// Sums over a wave of N values a lane (N a power of two): halves are exchanged, so N + 6 shuffles do
+// what 6 N would.  Lane l returns the sum of value l / (64 / N).
+template <int N> __device__ __forceinline__ float fold_lanes(float (&v)[N]) {
+  const int l = threadIdx.x & 63;
+  int bit = 32;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, bit /= 2) {
+    const bool up = l & bit;
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k)
+      if (k < n / 2) {
+        const float give = up ? v[k] : v[k + n / 2], keep = up ? v[k + n / 2] : v[k];
+        v[k] = keep + __shfl_xor(give, bit, 64);
+      }
+  }
+  float s = v[0];
+#pragma unroll
+  for (; bit > 0; bit /= 2) s += __shfl_xor(s, bit, 64);
+  return s;
+}
+template <typename T, int PV>
+__device__ __forceinline__ void load_pixels(const T* p, uint32_t at, bool ok, float (&v)[PV]) {
+  Pack<T, PV> o;
+#pragma unroll
+  for (int e = 0; e < PV; ++e) o.v[e] = narrow<T>(0.f);
+  if (ok) o = *(const Pack<T, PV>*)(p + at);
+#pragma unroll
+  for (int e = 0; e < PV; ++e) v[e] = to_f32(o.v[e]);
+}
+template <typename T, int PV>
+__device__ __forceinline__ void store_pixels(T* p, uint32_t at, const float (&v)[PV]) {
+  Pack<T, PV> o;
+#pragma unroll
+  for (int e = 0; e < PV; ++e) o.v[e] = narrow<T>(v[e]);
+  *(Pack<T, PV>*)(p + at) = o;
 }
 
-template <typename T, int G>
+template <typename T, int G, int NC, int PV>
 __global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
-  __shared__ float red[G][64];
-  const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const long long tiles = (a.P + 63) / 64;
-  const long long img = blockIdx.x / tiles, p = blockIdx.x % tiles * 64 + l;
-  const bool ok = p < a.P;
-  const T* x = (const T*)a.x + img * a.x_stride + p;
-  float v[kMapChannels];
-  float s = 0.f;
+  __shared__ float red[G][64 * PV];
+  const int l = threadIdx.x & 63;
+  const int g = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);  // channels: uniform
+  const uint32_t P = (uint32_t)a.P;  // (an image's offsets fit 32 bits)
+  const long long tiles = (a.P + 64 * PV - 1) / (64 * PV);
+  const long long img = blockIdx.x / tiles;
+  const uint32_t p = (uint32_t)((blockIdx.x % tiles * 64 + l) * PV);
+  const bool ok = p < P;
+  const T* x = (const T*)a.x + img * a.x_stride;
+  float v[NC][PV], s[PV], r[PV], mu[PV];
 #pragma unroll
-  for (int k = 0; k < kMapChannels; ++k) {
+  for (int e = 0; e < PV; ++e) s[e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
     const int c = k * G + g;
-    v[k] = ok && c < a.C ? to_f32(x[c * a.P]) : 0.f;
-    s += v[k];
-  }
-  const float mu = pixel_sum<G>(s, red) / a.C;
-  s = 0.f;
+    load_pixels<T, PV>(x, c * P + p, ok && c < a.C, v[k]);
 #pragma unroll
-  for (int k = 0; k < kMapChannels; ++k)
-    if (k * G + g < a.C) {
-      v[k] -= mu;
-      s += v[k] * v[k];
-    }
-  const float r = 1.f / sqrtf(pixel_sum<G>(s, red) / a.C + a.eps);
+    for (int e = 0; e < PV; ++e) s[e] += v[k][e];
+  }
+  pixel_sum<G, PV>(s, red);
+#pragma unroll
+  for (int e = 0; e < PV; ++e) {
+    mu[e] = s[e] / a.C;
+    s[e] = 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+    if (k * G + g < a.C)
+#pragma unroll
+      for (int e = 0; e < PV; ++e) {
+        v[k][e] -= mu[e];
+        s[e] += v[k][e] * v[k][e];
+      }
+  pixel_sum<G, PV>(s, red);
+#pragma unroll
+  for (int e = 0; e < PV; ++e) r[e] = 1.f / sqrtf(s[e] / a.C + a.eps);
   if (!ok) return;
-  if (a.mean && g == 0) {
-    a.mean[img * a.P + p] = mu;
-    a.rstd[img * a.P + p] = r;
-  }
-  T* y = (T*)a.y + img * a.C * a.P + p;
+  if (a.mean && g == 0)
 #pragma unroll
-  for (int k = 0; k < kMapChannels; ++k) {
+    for (int e = 0; e < PV; ++e) {
+      a.mean[img * a.P + p + e] = mu[e];
+      a.rstd[img * a.P + p + e] = r[e];
+    }
+  T* y = (T*)a.y + img * a.C * a.P;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
     const int c = k * G + g;
     if (c < a.C) {
       const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
       const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
-      y[c * a.P] = narrow<T>(v[k] * r * w + b);
+#pragma unroll
+      for (int e = 0; e < PV; ++e) v[k][e] = v[k][e] * r[e] * w + b;
+      store_pixels<T, PV>(y, c * P + p, v[k]);
     }
   }
 }
 
-template <typename T, int G>
+template <typename T, int G, int NC, int PV>
 __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
-  __shared__ float red[G][64];
-  const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const long long tiles = (a.P + 63) / 64;
-  float w[kMapChannels], dw[kMapChannels], db[kMapChannels];
+  __shared__ float red[G][64 * PV];
+  const int l = threadIdx.x & 63;
+  const int g = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);  // channels: uniform
+  const uint32_t P = (uint32_t)a.P;  // (an image's offsets fit 32 bits)
+  const long long tiles = (a.P + 64 * PV - 1) / (64 * PV);
+  float dw[NC], db[NC];
 #pragma unroll
-  for (int k = 0; k < kMapChannels; ++k) {
-    const int c = k * G + g;
-    w[k] = a.w && c < a.C ? to_f32(((const T*)a.w)[c]) : 1.f;
-    dw[k] = db[k] = 0.f;
-  }
+  for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.f;
   for (long long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
-    const long long img = t / tiles, p = t % tiles * 64 + l;
-    const bool ok = p < a.P;
-    const T* x = (const T*)a.x + img * a.x_stride + p;
-    const T* dy = (const T*)a.dy + img * a.C * a.P + p;
-    const float mu = ok ? a.mean[img * a.P + p] : 0.f, r = ok ? a.rstd[img * a.P + p] : 0.f;
-    float xh[kMapChannels], h[kMapChannels];
-    float s1 = 0.f, s2 = 0.f;
+    const long long img = t / tiles;
+    const uint32_t p = (uint32_t)((t % tiles * 64 + l) * PV);
+    const bool ok = p < P;
+    const T* x = (const T*)a.x + img * a.x_stride;
+    const T* dy = (const T*)a.dy + img * a.C * a.P;
+    float xh[NC][PV], h[NC][PV], mu[PV], r[PV], s1[PV], s2[PV];
 #pragma unroll
-    for (int k = 0; k < kMapChannels; ++k) {
-      const int c = k * G + g;
-      const bool have = ok && c < a.C;
-      xh[k] = have ? (to_f32(x[c * a.P]) - mu) * r : 0.f;
-      h[k] = have ? to_f32(dy[c * a.P]) : 0.f;
-      dw[k] += h[k] * xh[k];
-      db[k] += h[k];
-      h[k] *= w[k];
-      s1 += h[k];
-      s2 += h[k] * xh[k];
+    for (int k = 0; k < NC; ++k) {
+      const bool have = ok && k * G + g < a.C;
+      load_pixels<T, PV>(x, (k * G + g) * P + p, have, xh[k]);
+      load_pixels<T, PV>(dy, (k * G + g) * P + p, have, h[k]);
     }
-    s1 = pixel_sum<G>(s1, red) / a.C;
-    s2 = pixel_sum<G>(s2, red) / a.C;
-    if (ok && a.dx) {
-      T* dx = (T*)a.dx + img * a.C * a.P + p;
 #pragma unroll
-      for (int k = 0; k < kMapChannels; ++k) {
+    for (int e = 0; e < PV; ++e) {
+      mu[e] = ok ? a.mean[img * a.P + p + e] : 0.f;
+      r[e] = ok ? a.rstd[img * a.P + p + e] : 0.f;
+      s1[e] = s2[e] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (k * G + g < a.C) {
+        const float w = a.w ? to_f32(((const T*)a.w)[k * G + g]) : 1.f;
+#pragma unroll
+        for (int e = 0; e < PV; ++e) {
+          xh[k][e] = (xh[k][e] - mu[e]) * r[e];
+          dw[k] += h[k][e] * xh[k][e];
+          db[k] += h[k][e];
+          h[k][e] *= w;
+          s1[e] += h[k][e];
+          s2[e] += h[k][e] * xh[k][e];
+        }
+      }
+    pixel_sum<G, PV>(s1, red);
+    pixel_sum<G, PV>(s2, red);
+#pragma unroll
+    for (int e = 0; e < PV; ++e) {
+      s1[e] /= a.C;
+      s2[e] /= a.C;
+    }
+    if (ok && a.dx) {
+      T* dx = (T*)a.dx + img * a.C * a.P;
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
         const int c = k * G + g;
-        if (c < a.C) dx[c * a.P] = narrow<T>(r * (h[k] - s1 - xh[k] * s2));
+        if (c < a.C) {
+#pragma unroll
+          for (int e = 0; e < PV; ++e) h[k][e] = r[e] * (h[k][e] - s1[e] - xh[k][e] * s2[e]);
+          store_pixels<T, PV>(dx, c * P + p, h[k]);
+        }
       }
     }
   }
   if (!a.part) return;
-#pragma unroll
-  for (int k = 0; k < kMapChannels; ++k) {
-    const int c = k * G + g;
-    if (c < a.C) {
-      const float sw = lanes_sum<64>(dw[k]), sb = lanes_sum<64>(db[k]);
-      if (l == 0) {
-        a.part[(long long)blockIdx.x * a.C + c] = sw;
-        a.part[((long long)gridDim.x + blockIdx.x) * a.C + c] = sb;
-      }
-    }
+  const float sw = fold_lanes<NC>(dw), sb = fold_lanes<NC>(db);
+  constexpr int each = 64 / NC;  // lanes that hold a channel's sum
+  const int c = l / each * G + g;
+  if (l % each == 0 && c < a.C) {
+    a.part[(long long)blockIdx.x * a.C + c] = sw;
+    a.part[((long long)gridDim.x + blockIdx.x) * a.C + c] = sb;
   }
 }
 
@@ -316,8 +389,13 @@ template <bool MAP> __device__ __forceinline__ RowAt row_at(const NormArgs& a) {
   return r;
 }
 template <bool MAP> __device__ __forceinline__ float any_sum(float v, float (*red)[64]) {
-  if (MAP) return pixel_sum<4>(v, red);
-  return row_sum<256>(v, red[0]);
+  if constexpr (MAP) {
+    float s[1] = {v};
+    pixel_sum<4, 1>(s, red);
+    return s[0];
+  } else {
+    return row_sum<256>(v, red[0]);
+  }
 }
 
 template <typename T, bool MAP> __global__ __launch_bounds__(256) void norm_any(const NormArgs a) {
@@ -414,8 +492,10 @@ __global__ __launch_bounds__(1024) void norm_add_parts(const float* __restrict__
   const int c = blockIdx.x * 32 + l;
   const float* p = part + (long long)blockIdx.y * blocks * C;
   float s = 0.f;
-  if (c < C)
+  if (c < C) {
+#pragma unroll 8
     for (int b = g; b < blocks; b += 32) s += p[(long long)b * C + c];
+  }
   red[g][l] = s;
   __syncthreads();
   if (g == 0 && c < C) {
@@ -446,7 +526,10 @@ template <typename T> static bool vector_rows(const NormArgs& a) {
   return a.C % V == 0;
 }
 
-constexpr int kBlocksBackward = 1024;  // blocks that stay: four of 256 threads on each of 256 CUs
+// Blocks of the backward pass, each with a row of partial sums: tokens, four of 256 threads that stay
+// on each of 256 CUs; maps, twice that (a tile of 64 pixels each up to 131072 pixels: with 1024
+// blocks the l4 map's 1344 tiles took two turns, 24 us instead of 11).
+constexpr int kBlocksTokens = 1024, kBlocksMaps = 2048;
 
 int norm_parts(int layout, long long B, long long P, int C, int dtype) {
   const long long M = layout == kMap ? B * P : P;
@@ -459,7 +542,8 @@ int norm_parts(int layout, long long B, long long P, int C, int dtype) {
     if (p.tpr) rows = 256 / p.tpr;
   }
   const long long n = (M + rows - 1) / rows;
-  return (int)(n < kBlocksBackward ? n : kBlocksBackward);
+  const long long most = layout == kMap ? kBlocksMaps : kBlocksTokens;
+  return (int)(n < most ? n : most);
 }
 
 template <typename T, int TPR, int V, int NV = 1>
@@ -492,17 +576,34 @@ template <typename T> static bool tokens(const NormArgs& a, bool back, int parts
   return true;
 }
 
-template <typename T> static bool map(const NormArgs& a, bool back, int parts, hipStream_t s) {
-  if (a.C > 16 * kMapChannels) return false;
-  const unsigned grid = (unsigned)(a.B * ((a.P + 63) / 64));
-#define NORM_MAP(G)                                                        \
-  (back ? norm_map_backward<T, G><<<parts, 64 * G, 0, s>>>(a)              \
-        : norm_map<T, G><<<grid, 64 * G, 0, s>>>(a))
-  a.C <= kMapChannels       ? NORM_MAP(1)
-  : a.C <= 4 * kMapChannels ? NORM_MAP(4)
-  : a.C <= 8 * kMapChannels ? NORM_MAP(8)
-                            : NORM_MAP(16);
+template <typename T, int PV>
+static void map_pv(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.B * ((a.P + 64 * PV - 1) / (64 * PV)));
+#define NORM_MAP(G, NC)                                                    \
+  (back ? norm_map_backward<T, G, NC, PV><<<parts, 64 * G, 0, s>>>(a)      \
+        : norm_map<T, G, NC, PV><<<grid, 64 * G, 0, s>>>(a))
+  // eight channels a thread where eight waves hold them: the backward pass keeps five values a
+  // channel, and more of them leave fewer waves on a CU
+  a.C <= 8     ? NORM_MAP(1, 8)
+  : a.C <= 32  ? NORM_MAP(4, 8)
+  : a.C <= 64  ? NORM_MAP(8, 8)
+  : a.C <= 128 ? NORM_MAP(8, 16)
+               : NORM_MAP(8, 32);
 #undef NORM_MAP
+}
+template <typename T> static bool map(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  if (a.C > 256 || a.C * a.P >= 1LL << 30) return false;
+  if constexpr (sizeof(T) == 2) {
+    // (the backward pass of more channels would not fit the registers with pairs)
+    bool pairs = (a.C <= 128 || !back) && a.P % 2 == 0 && (a.B == 1 || a.x_stride % 2 == 0);
+    for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx})
+      pairs = pairs && aligned_to(p, 4);
+    if (pairs) {
+      map_pv<T, 2>(a, back, parts, s);
+      return true;
+    }
+  }
+  map_pv<T, 1>(a, back, parts, s);
   return true;
 }
 

@@ -28,6 +28,7 @@ struct ProductArgs {
   long long a_segment, b_segment;  // k runs over `segments` segments of K
   int I, J, K, segments, batches, splits;
   int a_k, b_k;        // the operand lies along k
+  int a_pad, b_pad;    // its rows are filled up with zeros to whole 16 bytes
   int pair;            // kGated*: W is [gate; up], `pair` rows each
   int channel_i;       // forward / dz: the channels lie along i (tokens) or j (maps)
   int mode, act;
@@ -60,6 +61,13 @@ int product_sum_rows(const ProductArgs& g, int dtype);
 int product_column_parts(int layout, long long B, long long P, int C);
 hipError_t product_column_sums(const void* dy, float* part, int layout, long long B, long long P,
                                int C, int parts, int dtype, hipStream_t stream);
+// dst: `rows` rows of `cols` values, zeros up to the next 16 bytes; src: rows `row` apart, groups of
+// `per_image` rows `image` apart
+hipError_t product_pad(const void* src, long long row, long long image, void* dst,
+                       long long per_image, long long rows, long long cols, int dtype,
+                       hipStream_t stream);
+hipError_t product_zero_tails(void* dst, long long rows, long long cols, int dtype,
+                              hipStream_t stream);
 hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
                               hipStream_t stream);
 

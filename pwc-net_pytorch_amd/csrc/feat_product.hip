@@ -51,14 +51,15 @@ __global__ __launch_bounds__(256) void add_splits(const float* __restrict__ part
 template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int bj) {
   constexpr int E = 16 / (int)sizeof(T);
   auto fits = [&](const void* p, long long ld, long long batch, long long seg, bool kc, int n,
-                  int rows, int pair) {
+                  int rows, int pair, int pad) {
     const long long far = (long long)(kc ? rows + pair : kStepBytes / (int)sizeof(T)) * ld;
     return aligned_to(p, 16) && ld % E == 0 && batch % E == 0 && seg % E == 0 &&
-           (kc ? g.K : n) % E == 0 && far * (long long)sizeof(T) < (1LL << 31) - (1 << 20);
+           (pad || (kc ? g.K : n) % E == 0) && far * (long long)sizeof(T) < (1LL << 31) - (1 << 20);
   };
   return fits(g.a, g.lda, g.a_batch, g.a_segment, g.a_k, g.I, bi,
-              g.channel_i ? g.pair : 0) &&
-         fits(g.b, g.ldb, g.b_batch, g.b_segment, g.b_k, g.J, bj, g.channel_i ? 0 : g.pair);
+              g.channel_i ? g.pair : 0, g.a_pad) &&
+         fits(g.b, g.ldb, g.b_batch, g.b_segment, g.b_k, g.J, bj, g.channel_i ? 0 : g.pair,
+              g.b_pad);
 }
 
 // Which kernel: the one with the least modelled time.  A step of 128 bytes of k costs a block at
@@ -146,6 +147,54 @@ int product_sum_rows(const ProductArgs& g, int dtype) {
   const ProductPlan p = product_plan(g, dtype);
   if (g.channel_i) return (g.J + p.bj - 1) / p.bj * 2 * p.passes;
   return (g.I + p.bi - 1) / p.bi * 2 * g.batches;
+}
+
+// ---- rows at 16-byte places ----
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, long long row,
+                                                long long image, T* __restrict__ dst,
+                                                long long per_image, long long rows,
+                                                long long cols) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const long long chunks = (cols + E - 1) / E;
+  for (long long id = blockIdx.x * 256LL + threadIdx.x; id < rows * chunks;
+       id += gridDim.x * 256LL) {
+    const long long r = id / chunks, c = (id - r * chunks) * E;
+    const long long m = r / per_image;
+    const T* p = src + m * image + (r - m * per_image) * row + c;
+    *(u32x4*)(dst + id * E) = cols - c >= E ? load16(p) : load_some(p, (int)(cols - c));
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void zero_tails(T* __restrict__ dst, long long rows,
+                                                  long long cols, long long pitch) {
+  for (long long r = blockIdx.x * 256LL + threadIdx.x; r < rows; r += gridDim.x * 256LL)
+    for (long long c = cols; c < pitch; ++c) dst[r * pitch + c] = narrow<T>(0.f);
+}
+static unsigned some_blocks(long long n) {
+  const long long b = (n + 255) / 256;
+  return (unsigned)(b < 16384 ? b : 16384);
+}
+hipError_t product_pad(const void* src, long long row, long long image, void* dst,
+                       long long per_image, long long rows, long long cols, int dtype,
+                       hipStream_t stream) {
+  if (dtype == 0)
+    pad_rows<float><<<some_blocks(rows * ((cols + 3) / 4)), 256, 0, stream>>>(
+        (const float*)src, row, image, (float*)dst, per_image, rows, cols);
+  else  // 16 bits are moved as they are
+    pad_rows<__half><<<some_blocks(rows * ((cols + 7) / 8)), 256, 0, stream>>>(
+        (const __half*)src, row, image, (__half*)dst, per_image, rows, cols);
+  return hipGetLastError();
+}
+hipError_t product_zero_tails(void* dst, long long rows, long long cols, int dtype,
+                              hipStream_t stream) {
+  const long long e = dtype == 0 ? 4 : 8, pitch = (cols + e - 1) / e * e;
+  if (pitch == cols) return hipSuccess;
+  if (dtype == 0)
+    zero_tails<float><<<some_blocks(rows), 256, 0, stream>>>((float*)dst, rows, cols, pitch);
+  else
+    zero_tails<__half><<<some_blocks(rows), 256, 0, stream>>>((__half*)dst, rows, cols, pitch);
+  return hipGetLastError();
 }
 
 // Partial column sums of dy, for a linear without an activation: tokens [M][C], a wave V channels

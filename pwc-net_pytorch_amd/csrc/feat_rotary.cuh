@@ -20,7 +20,8 @@ struct RotaryArgs {
   int H, D, R, axes, pos_type, interleaved;  // pos_type: 0 float, 1 int32, 2 int64
   long long grid[kMaxAxes], origin[kMaxAxes];
   float sign;              // 1 forward, -1 backward
-  int heads_each, head_groups;            // set by the launcher
+  uint32_t inner[kMaxAxes];               // set by the launcher
+  int heads_each, head_groups;
   long long batch_each, batch_groups;
 };
 

@@ -95,11 +95,13 @@ SYMBOLS = {
     "pwc_layer_norm_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I]),
     "pwc_layer_norm_backward": (_I, [_P] * 8 + [_I, _L, _L, _I, _L, _I, _P, _Z, _P]),
     "pwc_rotary": (_I, [_P] * 5 + [ctypes.POINTER(RotaryShape), _I, _I, _P]),
-    "pwc_linear_forward": (_I, [_P] * 5 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P]),
-    "pwc_linear_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I, _I, _I]),
+    "pwc_linear_forward_workspace_size": (_Z, [_P, _P, _I, _L, _L, _I, _I, _L, _I]),
+    "pwc_linear_forward": (_I, [_P] * 5 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z, _P]),
+    "pwc_linear_backward_workspace_size": (_Z, [_P] * 3 + [_I, _L, _L, _I, _I, _L, _I, _I]),
     "pwc_linear_backward": (_I, [_P] * 7 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z, _P]),
-    "pwc_gated_linear_forward": (_I, [_P] * 4 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P]),
-    "pwc_gated_linear_backward_workspace_size": (_Z, [_I, _L, _L, _I, _I, _I]),
+    "pwc_gated_linear_forward_workspace_size": (_Z, [_P, _P, _I, _L, _L, _I, _I, _L, _I]),
+    "pwc_gated_linear_forward": (_I, [_P] * 4 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z, _P]),
+    "pwc_gated_linear_backward_workspace_size": (_Z, [_P] * 3 + [_I, _L, _L, _I, _I, _L, _I]),
     "pwc_gated_linear_backward": (_I, [_P] * 7 + [_I, _L, _L, _I, _I, _L, _I, _F, _I, _P, _Z,
                                                   _P]),
 }

@@ -42,13 +42,7 @@ def _bind():
     """Give the module the C entries' addresses (it asks at its first call)."""
     lib = _lib.load()
     _ext.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-               for name in ("pwc_last_error", "pwc_rotary",
-                            "pwc_layer_norm_forward", "pwc_layer_norm_backward_workspace_size",
-                            "pwc_layer_norm_backward", "pwc_linear_forward",
-                            "pwc_linear_backward_workspace_size", "pwc_linear_backward",
-                            "pwc_gated_linear_forward",
-                            "pwc_gated_linear_backward_workspace_size",
-                            "pwc_gated_linear_backward")})
+               for name in _ext.entries()})
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, channel_dim=1, stats=False):

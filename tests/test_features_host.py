@@ -61,7 +61,7 @@ def test_product_entries_refuse():
     lib, p, z = _lib(), ctypes.c_void_p(64), None
 
     def fwd(x=p, w=p, y=p, layout=0, B=1, P=4, K=8, O=6, stride=32, act=0, dtype=0, gated=False):
-        geo = (layout, B, P, K, O, stride, act, 0.1, dtype, z)
+        geo = (layout, B, P, K, O, stride, act, 0.1, dtype, z, 0, z)
         return (lib.pwc_gated_linear_forward(x, w, z, y, *geo) if gated
                 else lib.pwc_linear_forward(x, w, z, z, y, *geo))
 
@@ -96,12 +96,27 @@ def test_product_entries_refuse():
         _refused(bwd(ws=z), "workspace too small")
         assert bwd(gx=z, gw=z, gb=z) == 1
         assert bwd(gw=z, gb=z, P=0) == 1
-    assert lib.pwc_linear_backward_workspace_size(0, 1, 4, 8, 6, 0, 9) == 0
-    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 4, 0, 6, 0) == 0
+    back, gated = lib.pwc_linear_backward_workspace_size, lib.pwc_gated_linear_backward_workspace_size
+    assert back(p, p, p, 0, 1, 4, 8, 6, 32, 0, 9) == 0
+    assert gated(p, p, p, 0, 1, 4, 0, 6, 32, 0) == 0
     # dz [4, 12], and the sums of dW [12, 8] where k is split
-    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 4, 8, 6, 0) >= 4 * 12 * 4
-    assert lib.pwc_gated_linear_backward_workspace_size(0, 1, 10 ** 6, 8, 6, 0) >= \
-        10 ** 6 * 12 * 4 + 2 * 12 * 8 * 4
+    assert gated(p, p, p, 0, 1, 4, 8, 6, 32, 0) >= 4 * 12 * 4
+    assert gated(p, p, p, 0, 1, 10 ** 6, 8, 6, 8 * 10 ** 6, 0) >= 10 ** 6 * 12 * 4 + 2 * 12 * 8 * 4
+    # large 16-bit products are given rows at 16-byte places: x, W (and dz) where theirs are not
+    fwd = lib.pwc_linear_forward_workspace_size
+    odd = ctypes.c_void_p(66)
+    assert fwd(p, p, 1, 1, 4096, 1024, 1024, 1024, 2) == 0
+    assert fwd(odd, p, 1, 1, 4096, 1024, 1024, 1024, 2) == 4096 * 1024 * 2
+    assert fwd(p, odd, 1, 1, 4096, 1024, 1024, 1024, 2) == 1024 * 1024 * 2
+    assert fwd(p, p, 1, 1, 4096, 1024, 1024, 1025, 2) == 4096 * 1024 * 2
+    assert fwd(p, p, 1, 1, 4096, 1023, 1024, 1023, 2) == (4096 + 1024) * 1024 * 2
+    assert fwd(p, p, 1, 1, 4096, 1023, 1024, 1023, 0) == (4096 + 1024) * 1024 * 4
+    assert fwd(p, p, 1, 1, 100, 99, 98, 99, 2) == 0
+    assert fwd(p, p, 1, 1, 16, 9999, 9999, 9999, 2) == 0  # a pass over W reads it as it lies
+    _refused(lib.pwc_linear_forward(p, p, z, z, p, 1, 1, 4096, 1023, 1024, 1023, 0, 0.1, 2, z, 0,
+                                    z), "workspace too small")
+    _refused(lib.pwc_linear_forward(p, p, z, z, p, 1, 1, 4096, 1023, 1024, 1023, 0, 0.1, 2, p,
+                                    1 << 30, z), "workspace not aligned")
 
 
 def test_rotary_entry_refuses():

@@ -245,6 +245,41 @@ def test_many_steps(dtype):
             _check_product(*case, "gelu", gated, 1 if is_map else -1)
 
 
+@pytest.mark.parametrize("dtype,is_map,dims,K,O,gated,act", [
+    (torch.bfloat16, False, (3001,), 517, 1021, False, "gelu"),
+    (torch.float16, False, (3001,), 520, 1021, False, "none"),
+    (torch.bfloat16, False, (2999,), 521, 1024, False, "none"),
+    (torch.float16, False, (4093,), 259, 517, True, "silu"),
+    (torch.bfloat16, True, (4, 61, 67), 131, 259, True, "silu"),
+    (torch.float16, True, (5, 61, 67), 136, 392, False, "none"),
+    (torch.bfloat16, True, (4, 62, 68), 133, 517, False, "gelu_tanh"),
+    (torch.float32, False, (4099,), 1021, 1019, False, "tanh")])
+def test_large_rows_at_odd_places(dtype, is_map, dims, K, O, gated, act):
+    """Large products whose rows are laid out at 16-byte places first."""
+    case = _product_case(is_map, dims, K, O, dtype, act, True, not gated, gated)
+    _check_product(*case, act, gated, 1 if is_map else -1)
+
+
+def test_large_rows_with_a_distance():
+    """A slice of a wider buffer (odd distance, odd start) gives its copy's values; what stands
+    between the rows is not read into the sums."""
+    import pwcnet_amd as P
+    gen = _gen("distance")
+    wide = torch.full((4100, 1051), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wide[2:4098, 3:1027] = _rand(gen, 4096, 1024, dtype=torch.bfloat16)
+    x = wide[2:4098, 3:1027]
+    w, g = (_rand(gen, 512, 1024, dtype=torch.bfloat16, scale=1 / 32),
+            _rand(gen, 4096, 512, dtype=torch.bfloat16))
+    want = None
+    for v in (x.contiguous(), x):
+        v = v.detach().requires_grad_(True)
+        u = w.clone().requires_grad_(True)
+        y = P.linear(v, u, activation="silu", channel_dim=-1)
+        got = [y.detach(), *torch.autograd.grad(y, (v, u), g)]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
 def test_large_tiles(dtype):
     """Enough rows and columns for the largest tiles, one short of and one past a tile."""
