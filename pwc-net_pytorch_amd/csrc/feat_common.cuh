@@ -106,17 +106,14 @@ template <bool FAST> __device__ __forceinline__ float recip(float x) {
 template <bool FAST> __device__ __forceinline__ float sigmoid_f(float z) {
   return recip<FAST>(1.f + exp_neg<FAST>(z));
 }
-// Phi(z), the normal distribution function.  FAST: erfc by the rational form of Abramowitz and
-// Stegun 7.1.26 (error 1.5e-7 absolute), whose factor exp(-z^2 / 2) the derivative needs as well.
-template <bool FAST> __device__ __forceinline__ float phi_f(float z, float gauss) {
-  if (!FAST) return 0.5f * erfcf(-0.7071067811865476f * z);
-  const float a = fabsf(z) * 0.7071067811865476f;
-  const float t = recip<true>(1.f + 0.3275911f * a);
-  const float p =
-      t * (0.254829592f +
-           t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * p * gauss;  // Phi(-|z|)
-  return z > 0.f ? 1.f - tail : tail;
+// Phi(-|z|), the normal distribution's tail, given gauss = exp(-z^2 / 2): half of erfc by the form of
+// Abramowitz and Stegun 7.1.26 (error 1.5e-7 absolute).
+__device__ __forceinline__ float tail_f(float z, float gauss) {
+  const float t = recip<true>(1.f + 0.3275911f * 0.7071067811865476f * fabsf(z));
+  const float p = t * (0.127414796f +
+                       t * (-0.142248368f +
+                            t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  return p * gauss;
 }
 
 constexpr float kSqrt2OverPi = 0.7978845608028654f;
@@ -136,10 +133,22 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
   } else if (act == kActGelu) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float g = FAST || SLOPE ? exp_neg<FAST>(0.5f * z[e] * z[e]) : 0.f;
-      const float p = phi_f<FAST>(z[e], g);
-      f[e] = z[e] * p;
-      if (SLOPE) d[e] = p + z[e] * 0.3989422804014327f * g;
+      const float z2 = z[e] * z[e];
+      if (FAST) {
+        const float g = __builtin_amdgcn_exp2f(-0.7213475204444817f * z2);
+        const float t = tail_f(z[e], g);
+        if constexpr (SLOPE) {
+          const float p = z[e] > 0.f ? 1.f - t : t;
+          f[e] = z[e] * p;
+          d[e] = p + z[e] * (0.3989422804014327f * g);
+        } else {
+          f[e] = fmaxf(z[e], 0.f) - fabsf(z[e]) * t;  // z Phi(z)
+        }
+      } else {
+        const float p = 0.5f * erfcf(-0.7071067811865476f * z[e]);
+        f[e] = z[e] * p;
+        if (SLOPE) d[e] = p + z[e] * 0.3989422804014327f * expf(-0.5f * z2);
+      }
     }
   } else if (act == kActGeluTanh) {
 #pragma unroll

@@ -72,9 +72,9 @@ struct TileCost {
   int kernel, bi, bj, passes, blocks;  // blocks that a CU holds
   double lag, work, fixed;
 };
-static constexpr TileCost kCost16[] = {{kTile64, 64, 64, 1, 4, 0.56, 0.18, 3.3},
-                                       {kTile128, 128, 128, 1, 2, 0.80, 0.50, 6.5},
-                                       {kTile256, 256, 256, 2, 1, 1.40, 1.50, 16.0}};
+static constexpr TileCost kCost16[] = {{kTile64, 64, 64, 1, 4, 0.56, 0.20, 3.3},
+                                       {kTile128, 128, 128, 1, 2, 0.85, 0.57, 6.5},
+                                       {kTile256, 256, 256, 2, 1, 1.60, 1.65, 16.0}};
 static constexpr TileCost kCost32[] = {{kTile64, 64, 64, 1, 4, 0.65, 0.53, 4.0},
                                        {kTile128, 128, 128, 1, 2, 2.00, 2.00, 8.0}};
 constexpr int kCUs = 256;
@@ -116,7 +116,7 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
       if (t < blocks / kCUs * each * c.work) t = blocks / kCUs * each * c.work;
       t += c.fixed * (rounds < 1 ? 1 : rounds);
       // the partial sums go out and come back, and one more launch
-      if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 5e6;
+      if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 6.5e6;
       if (t < least) {
         least = t;
         best = {c.kernel + (direct || c.bi > 128 ? 0 : 1), c.bi, c.bj, c.passes, splits};

@@ -256,7 +256,7 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
   float b[V], c[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) b[e] = c[e] = 0.f;
-  if (CI && bias && column) {
+  if (MODE != kPlain && CI && bias && column) {
     load_values<T, V>(bias + i, b);
     if (kPair) load_values<T, V>(bias + g.pair + i, c);
   }
@@ -289,7 +289,7 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
       const int j = f.j0 + uj + (r0 + r) * RS;
       ok[r] = column && j < f.j_end;
       bj[r] = cj[r] = 0.f;
-      if (!CI && bias && ok[r]) {
+      if (MODE != kPlain && !CI && bias && ok[r]) {
         bj[r] = to_f32(bias[j]);
         if (kPair) cj[r] = to_f32(bias[g.pair + j]);
       }
@@ -307,17 +307,21 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
       const int rj = uj + (r0 + r) * RS;
       const int tj = kPair && !CI ? (rj >> 4) * 32 + (rj & 15) : rj;
       turned<WI, V>(f.tile, tj, ti, v[r]);
+      if constexpr (MODE != kPlain) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[r][e] += b[e] + bj[r];
+        for (int e = 0; e < V; ++e) v[r][e] += CI ? b[e] : bj[r];
+      }
       if constexpr (kPair) {
         turned<WI, V>(f.tile, CI ? tj : tj + 16, CI ? ti + 16 : ti, w[r]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[r][e] += c[e] + cj[r];
+        for (int e = 0; e < V; ++e) w[r][e] += CI ? c[e] : cj[r];
       }
       if constexpr (MODE == kLinear) {
         if (act != kActNone) activate<kFast, false>(act, v[r], v[r], sv, slope);
+        if (other) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[r][e] += o[r][e];
+          for (int e = 0; e < V; ++e) v[r][e] += o[r][e];
+        }
       } else if constexpr (MODE == kLinearDz) {
         float a[V], s[V];
         activate<kFast, true>(act, v[r], a, s, slope);
