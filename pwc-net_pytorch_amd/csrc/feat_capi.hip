@@ -90,6 +90,8 @@ View dz_view(const Problem& p, const void* dz) {
 // three backward products 2 to 7 times their time (8191 x 1023 -> 4095: 1.2 ms instead of 0.25),
 // the copies tens of microseconds.  Small calls, and 32-bit ones below 8 GFLOP, read them as they
 // lie.
+constexpr double kKeepLow = 5e8;  // operations of a product
+
 bool pads_pay(const Problem& p) {
   return 2.0 * (double)p.M * p.rows * p.K >= (p.dtype == 0 ? 8e9 : 2e9);
 }
@@ -152,11 +154,15 @@ ProductArgs dz_args(const Problem& p, const View& x, const View& w, const void* 
                     const void* dy, const View& dz) {
   return forward_args(p, x, w, bias, dy, dz, p.gated ? kGatedDz : kLinearDz);
 }
-ProductArgs dx_args(const Problem& p, const View& dz, const View& w, void* dx) {
+// dx = dz W, for tokens in 32-bit parts (`out`) or itself where there is one split; `low`: from dz
+// to what its rounding took, one more segment of k
+ProductArgs dx_args(const Problem& p, const View& dz, long long low, const View& w, void* out) {
   ProductArgs g = blank();
   g.K = p.rows;
-  g.out = dx;
-  g.mode = kPlain;
+  g.out = out;
+  g.mode = tokens(p) ? kPartial : kPlain;
+  g.segments = low ? 2 : 1;
+  (tokens(p) ? g.b_segment : g.a_segment) = low;
   if (tokens(p)) {
     g.a = w.at, g.lda = w.row, g.a_pad = w.padded, g.a_k = 0, g.I = p.K;
     g.b = dz.at, g.ldb = dz.row, g.b_pad = dz.padded, g.b_k = 1, g.J = (int)p.M;
@@ -171,7 +177,7 @@ ProductArgs dx_args(const Problem& p, const View& dz, const View& w, void* dx) {
   return g;
 }
 // dW = dz^T x in 32-bit parts (`out`), or itself where there is one split
-ProductArgs dw_args(const Problem& p, const View& x, const View& dz, void* out) {
+ProductArgs dw_args(const Problem& p, const View& x, const View& dz, long long low, void* out) {
   ProductArgs g = blank();
   g.mode = kPartial;
   g.out = out;
@@ -182,11 +188,13 @@ ProductArgs dw_args(const Problem& p, const View& x, const View& dz, void* out) 
   g.b = dz.at, g.ldb = dz.row, g.b_pad = dz.padded;
   if (tokens(p)) {
     g.K = (int)p.M;
+    g.segments = low ? 2 : 1;
+    g.b_segment = low;
   } else {
     g.K = (int)p.P;
-    g.segments = (int)p.B;
-    g.a_segment = x.image, g.a_k = 1;
-    g.b_segment = dz.image, g.b_k = 1;
+    g.segments = (int)p.B * (low ? 2 : 1);
+    g.a_segment = x.image, g.a_k = 1, g.a_halves = low ? 1 : 0;
+    g.b_segment = low ? low : dz.image, g.b_k = 1;
   }
   return g;
 }
@@ -215,7 +223,8 @@ ForwardSpace forward_space(const Problem& p, const void* x, const void* w) {
 struct BackwardSpace {
   bool pad_x, pad_w, pad_dz;
   size_t x, w, part, sums, total;  // dz, or the padded dy, lies at 0
-  int splits, rows;                // rows of partial bias gradients
+  int dx_splits, splits, rows;     // rows: of partial bias gradients
+  long long low;                   // from dz to what its rounding took (maps: image by image), or 0
   View xv, wv, dzv;                // as the products take them
 };
 BackwardSpace backward_space(const Problem& p, const void* x, const void* w, const void* dy,
@@ -226,11 +235,17 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   s.pad_x = pay && (z || dw) && !lies_well(p, s.xv, x_cols(p));
   s.pad_w = pay && (z || dx) && !lies_well(p, s.wv, p.K);
   s.pad_dz = pay && (z || dx || dw) && !lies_well(p, s.dzv, dz_cols(p));
+  // dz in 16 bits is rounded once, which makes the gradients' error 1.4 times that of their own
+  // rounding; in small calls, where chance adds to that, what the rounding took follows as more k,
+  // at a cost that the launches hide.  (Only the kernels of such calls can write it.)
+  if (z && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
+      product_plan(dz_args(p, s.xv, s.wv, nullptr, dy, s.dzv), p.dtype).kernel <= kTile64Any)
+    s.low = tokens(p) ? p.M * p.rows : p.rows * p.P;
   size_t at = 0;
   if (s.pad_dz)
     at += bytes_of(p, dz_rows(p), dz_cols(p));
   else if (z)
-    at += align256((size_t)p.M * p.rows * elem(p.dtype));
+    at += align256((size_t)p.M * p.rows * elem(p.dtype) * (s.low ? 2 : 1));
   s.x = at;
   if (s.pad_x) at += bytes_of(p, x_rows(p), x_cols(p));
   s.w = at;
@@ -241,9 +256,14 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
     s.dzv = padded_dz(p, ws);
   else if (z)
     s.dzv = dz_view(p, ws);
-  s.splits = dw ? product_plan(dw_args(p, s.xv, s.dzv, nullptr), p.dtype).splits : 1;
+  if (s.low && !tokens(p)) s.dzv.image *= 2;
+  s.dx_splits = dx ? product_plan(dx_args(p, s.dzv, s.low, s.wv, nullptr), p.dtype).splits : 1;
+  s.splits = dw ? product_plan(dw_args(p, s.xv, s.dzv, s.low, nullptr), p.dtype).splits : 1;
+  // (dx's parts are added before dW's are written)
   s.part = at;
-  if (s.splits > 1) at += align256((size_t)s.splits * p.rows * p.K * 4);
+  const size_t dx_part = s.dx_splits > 1 ? align256((size_t)s.dx_splits * p.M * p.K * 4) : 0;
+  const size_t dw_part = s.splits > 1 ? align256((size_t)s.splits * p.rows * p.K * 4) : 0;
+  at += dx_part > dw_part ? dx_part : dw_part;
   s.sums = at;
   if (db) {
     s.rows = z ? product_sum_rows(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype)
@@ -279,6 +299,7 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
   if (e == hipSuccess && needs_z(p)) {
     ProductArgs g = dz_args(p, s.xv, s.wv, bias, dy, s.dzv);
     g.sums = db ? (float*)(ws + s.sums) : nullptr;
+    g.low = s.low;
     e = product_launch(g, p.dtype, stream);
     if (s.pad_dz && e == hipSuccess)
       e = product_zero_tails(ws, dz_rows(p), dz_cols(p), p.dtype, stream);
@@ -287,9 +308,16 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     e = product_pad(dy, v.row, v.image, ws, tokens(p) ? p.M : p.rows, dz_rows(p), dz_cols(p),
                     p.dtype, stream);
   }
-  if (dx && e == hipSuccess) e = product_launch(dx_args(p, s.dzv, s.wv, dx), p.dtype, stream);
+  if (dx && e == hipSuccess) {
+    ProductArgs g = dx_args(p, s.dzv, s.low, s.wv, s.dx_splits > 1 ? (void*)(ws + s.part) : dx);
+    g.splits = s.dx_splits;
+    e = product_launch(g, p.dtype, stream);
+    if (e == hipSuccess && s.dx_splits > 1)
+      e = product_add_splits((const float*)(ws + s.part), dx, p.M * p.K, s.dx_splits, p.dtype,
+                             stream);
+  }
   if (dw && e == hipSuccess) {
-    ProductArgs g = dw_args(p, s.xv, s.dzv, s.splits > 1 ? (void*)(ws + s.part) : dw);
+    ProductArgs g = dw_args(p, s.xv, s.dzv, s.low, s.splits > 1 ? (void*)(ws + s.part) : dw);
     g.splits = s.splits;
     e = product_launch(g, p.dtype, stream);
     if (e == hipSuccess && s.splits > 1)

@@ -26,6 +26,8 @@ struct ProductArgs {
   long long lda, ldb, ldo, ldother;
   long long a_batch, b_batch, out_batch, other_batch;
   long long a_segment, b_segment;  // k runs over `segments` segments of K
+  long long low;      // k*Dz in 16 bits, 64-tiles and few tokens: where what rounding took goes, or 0
+  int a_halves;       // pairs of segments share A's
   int I, J, K, segments, batches, splits;
   int a_k, b_k;        // the operand lies along k
   int a_pad, b_pad;    // its rows are filled up with zeros to whole 16 bytes
@@ -36,7 +38,7 @@ struct ProductArgs {
   int tiles_i, tiles_j;  // set by the launcher
 };
 
-// The kernels (direct loads from aligned rows, or Any).
+// The kernels.  Direct loads from aligned rows; Any reads through registers.
 enum ProductKernel : int {
   kFew16,  // passes over W for at most 16, 32, 64 tokens
   kFew32,
@@ -44,7 +46,6 @@ enum ProductKernel : int {
   kTile64,
   kTile64Any,
   kTile128,
-  kTile128Any,
   kTile256,
 };
 struct ProductPlan {

@@ -26,7 +26,6 @@
 // bytes a lane: eight k of one row (16 bits, one 16x16x32 instruction) or four (32 bits, four
 // 16x16x4 instructions).  The order of k within a fragment does not matter as long as both
 // operands share it; N tiles of 16 bits are turned by the transposing LDS read.
-#include <cstdlib>
 
 #include "feat_norm.cuh"
 #include "feat_product.cuh"
@@ -66,7 +65,7 @@ template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int
 // least `lag` (loads, barrier, latency), and the blocks of a CU share its matrix units, `work` a
 // block; a tile's epilogue and start cost `fixed` for every round of tiles over the card.  The
 // figures are measured (us; bf16: 8192 x K -> 4096 and 64 x 4096 -> 4096 tokens; fp32: 4096 x 1024
-// -> 1024 and 1000 x 1000 -> 1000): 256-tiles do 1430 TFLOP/s where there are enough of them, 128
+// -> 1024 and 1000 x 1000 -> 1000): 256-tiles do 1520 TFLOP/s where there are enough of them, 128
 // are the best for some hundred, 64 for less.
 struct TileCost {
   int kernel, bi, bj, passes, blocks;  // blocks that a CU holds
@@ -89,21 +88,17 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
   const bool pair = g.mode == kGated || g.mode == kGatedDz;
   // A pass over W reads it once at memory speed, the tiles a block's share of it at a CU's pace.
   // (tokens alone: their W lies along k, and a kernel of one pass has one batch)
-  if (g.channel_i && (g.mode == kLinear || g.mode == kGated) && g.J <= 64)
+  if (g.channel_i && g.J <= 64)
     return {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 16, 1, 1};
   const long long pairs = ((long long)g.pair + 15) / 16 * 32;
   const long long ri = pair && g.channel_i ? pairs : g.I, rj = pair && !g.channel_i ? pairs : g.J;
   ProductPlan best = {};
   double least = 1e300;
   const TileCost* costs = dtype == 0 ? kCost32 : kCost16;
-  const char* env = getenv("TILE");
-  int pick = env ? atoi(env) : -1;
-  if (pick >= 0 && (pick >= (dtype == 0 ? 2 : 3) || (pick >= 2 && !direct_any(g, costs[pick], dtype)))) pick = -1;
   for (int n = 0; n < (dtype == 0 ? 2 : 3); ++n) {
     const TileCost& c = costs[n];
-    if (pick >= 0 && pick != n) continue;
     const bool direct = direct_any(g, c, dtype);
-    if (!direct && c.bi > 128) break;
+    if (!direct && n > 0) break;  // through registers: the small tile alone
     const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
     const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
     const double tiles =
@@ -119,7 +114,7 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
       if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 6.5e6;
       if (t < least) {
         least = t;
-        best = {c.kernel + (direct || c.bi > 128 ? 0 : 1), c.bi, c.bj, c.passes, splits};
+        best = {direct ? c.kernel : kTile64Any, c.bi, c.bj, c.passes, splits};
       }
     }
   }
@@ -145,6 +140,7 @@ static hipError_t add_splits_t(const float* part, void* out, long long n, int sp
 // Rows of partial sums that a kLinearDz / kGatedDz launch writes.
 int product_sum_rows(const ProductArgs& g, int dtype) {
   const ProductPlan p = product_plan(g, dtype);
+  if (p.kernel <= kFew64) return 1 << (p.kernel - kFew16);
   if (g.channel_i) return (g.J + p.bj - 1) / p.bj * 2 * p.passes;
   return (g.I + p.bi - 1) / p.bi * 2 * g.batches;
 }

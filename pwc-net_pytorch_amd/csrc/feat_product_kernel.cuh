@@ -182,35 +182,34 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
     }
   }
 
-  // start loading the step at k0 of the segment at `seg` values from base
-  __device__ __forceinline__ void load(char* lds, long long seg, int k0) {
-    const T* b = base + seg + (KC ? (long long)k0 : (long long)k0 * ld);
+  // the step at k0 of the segment at `seg` values from base: where it lies, then its loads
+  const T* from;
+  int left_k;
+  __device__ __forceinline__ void aim(long long seg, int k0) {
+    from = base + seg + (KC ? (long long)k0 : (long long)k0 * ld);
+    left_k = K - k0;
+  }
+  __device__ __forceinline__ void load(char* lds, int n) {
     if constexpr (DIRECT) {
-      const uint64_t a = (uint64_t)(uintptr_t)b;
+      const uint64_t a = (uint64_t)(uintptr_t)from;
       const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
       const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           (void*)(uintptr_t)(((uint64_t)hi << 32) | lo), (short)0, 0x7fffffff, 0x00020000);
       const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-#pragma unroll
-      for (int n = 0; n < Tl::LOADS; ++n) {
-        const uint32_t o = at[n] < K - k0 ? off[n] : kOOB;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (__attribute__((address_space(3))) void*)(lds + (n * NW + wave) * 1024), 16, o, 0, 0,
-            0);
-      }
+      const uint32_t o = at[n] < left_k ? off[n] : kOOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(lds + (n * NW + wave) * 1024), 16, o, 0, 0,
+          0);
     } else {
-#pragma unroll
-      for (int n = 0; n < Tl::LOADS; ++n) {
-        // K: k0 + at .. < K;  N: row k0 + at < K, `left` values of it
-        const int have = KC ? (left[n] ? K - k0 - at[n] : 0) : (at[n] < K - k0 ? left[n] : 0);
-        const T* p = b + row[n];
-        if (have >= Tl::E) {
-          reg[n] = load16(p);
-        } else {
-          reg[n] = u32x4{0u, 0u, 0u, 0u};
-          if (have > 0) reg[n] = load_some(p, have);
-        }
+      // K: k0 + at .. < K;  N: row k0 + at < K, `left` values of it
+      const int have = KC ? (left[n] ? left_k - at[n] : 0) : (at[n] < left_k ? left[n] : 0);
+      const T* p = from + row[n];
+      if (have >= Tl::E) {
+        reg[n] = load16(p);
+      } else {
+        reg[n] = u32x4{0u, 0u, 0u, 0u};
+        if (have > 0) reg[n] = load_some(p, have);
       }
     }
   }
@@ -221,6 +220,15 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
     }
   }
 };
+
+// what rounding takes from the values; nothing where it gives an infinity or a NaN
+template <typename T, int V> __device__ __forceinline__ void rounded_off(float (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float h = to_f32(narrow<T>(v[e]));
+    v[e] = fabsf(h) < __builtin_inff() ? v[e] - h : 0.f;
+  }
+}
 
 // What the epilogue needs of one wave's sums: they lie in LDS as rows of i (`tile`, WI long).
 struct Finish {
@@ -238,6 +246,7 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
                                                const T* other, int sum_row) {
   constexpr bool kFast = sizeof(T) == 2, kPair = MODE == kGated || MODE == kGatedDz;
   constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
+  constexpr bool kLow = kDz && sizeof(T) == 2 && WI == 32;  // small tiles
   constexpr int E = 16 / (int)sizeof(T);                    // columns of a whole piece
   constexpr int COLS = kPair && CI ? WI / 2 : WI, ROWS = kPair && !CI ? WJ / 2 : WJ;
   constexpr int U = V == 1 ? E : COLS / V, RS = 64 / U, N = ROWS / RS;
@@ -370,8 +379,19 @@ __device__ __forceinline__ void finish_columns(const ProductArgs& g, const Finis
     for (int r = 0; r < NB; ++r) {
       T* p = out + (long long)(f.j0 + uj + (r0 + r) * RS) * ldo + i;
       if (!ok[r]) continue;
+      T* const up = p + (CI ? (long long)g.pair : g.pair * ldo);
       store_values<T, V>(p, v[r]);
-      if (MODE == kGatedDz) store_values<T, V>(p + (CI ? (long long)g.pair : g.pair * ldo), w[r]);
+      if (MODE == kGatedDz) store_values<T, V>(up, w[r]);
+      if constexpr (kLow) {
+        if (g.low) {
+          rounded_off<T, V>(v[r]);
+          store_values<T, V>(p + g.low, v[r]);
+          if (MODE == kGatedDz) {
+            rounded_off<T, V>(w[r]);
+            store_values<T, V>(up + g.low, w[r]);
+          }
+        }
+      }
     }
   }
   if constexpr (kDz && CI) {
@@ -461,6 +481,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   constexpr bool PART = MODE == kPartial, CI = BKC && AKC && !PART;  // channels along i: tokens
   constexpr int WI = BI / NWI, WJ = BJ / NWJ, FI = WI / 16, FJ = WJ / 16;
   constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
+  constexpr bool kPinned = FI * FJ >= 64;  // one block a CU, one wave a SIMD
   typedef Tile<T, BI, AKC, NW> TA;
   typedef Tile<T, BJ, BKC, NW> TB;
   typedef typename Frag<T>::type frag_t;
@@ -499,17 +520,24 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   }
   // the step whose loads start next
   int seg = s / per_seg, k0 = (s - seg * per_seg) * TA::KS, next = s;
-  auto start = [&](char* pa, char* pb) __attribute__((always_inline)) {
+  auto aim = [&]() __attribute__((always_inline)) {
     // past the end every chunk is outside: zeros, without an access to memory
     const int k = next < end ? k0 : 0x3fffffff;
-    la.load(pa, seg * g.a_segment, k);
-    lb.load(pb, seg * g.b_segment, k);
+    la.aim((seg >> g.a_halves) * g.a_segment, k);
+    lb.aim(seg * g.b_segment, k);
     ++next;
     k0 += TA::KS;
     if (k0 >= g.K) {
       k0 = 0;
       ++seg;
     }
+  };
+  auto start = [&](char* pa, char* pb) __attribute__((always_inline)) {
+    aim();
+#pragma unroll
+    for (int n = 0; n < TA::LOADS; ++n) la.load(pa, n);
+#pragma unroll
+    for (int n = 0; n < TB::LOADS; ++n) lb.load(pb, n);
   };
   // the started loads are in LDS, and this wave's reads so far are done
   auto settle = [&](char* pa, char* pb) __attribute__((always_inline)) {
@@ -527,10 +555,14 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
     for (int i = 0; i < FI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // Two fragment sets: while one is multiplied the other is read.  A step has two halves of k:
-  //   read half 1 | multiply half 0 | wait for the next step's loads, barrier |
-  //   read half 0 of the next step | start the loads of the step after it into the buffer that
-  //   all waves have read | multiply half 1
-  // so the loads have a whole step, the reads half a step, and one barrier a step is enough.
+  //   multiply half 0, reading half 1 | wait for the next step's loads, barrier |
+  //   multiply half 1, reading half 0 of the next step and starting the loads of the step after it
+  //   into the buffer that all waves have read
+  // so the loads have a whole step, the reads half a step, and one barrier a step is enough.  Where
+  // one wave a SIMD has to feed the matrix unit alone, reads and loads stand between its
+  // instructions, a row of fragments at a time: issued in one go they fill the queues and it waits
+  // behind them (8192 x K -> 4096 tokens: 1430 -> 1520 TFLOP/s).  With two waves a SIMD one
+  // multiplies while the other issues, and the same order costs a third of the rate.
   frag_t fa[2][FI], fb[2][FJ];
   auto read = [&](const char* pa, const char* pb, int kk) __attribute__((always_inline)) {
 #pragma unroll
@@ -538,27 +570,46 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 #pragma unroll
     for (int i = 0; i < FI; ++i) fa[kk][i] = TA::frag(pa, wi + i * 16, kk);
   };
-  auto multiply = [&](int kk) __attribute__((always_inline)) {
+  // half kk is multiplied, half 1 - kk is read from (pa, pb); LOAD: the next loads into (qa, qb)
+  auto half = [&](int kk, const char* pa, const char* pb, auto load, char* qa, char* qb)
+      __attribute__((always_inline)) {
+    constexpr bool LOAD = decltype(load)::value;
+    if constexpr (!kPinned) {
+      read(pa, pb, 1 - kk);
+      if (LOAD) start(qa, qb);
 #pragma unroll
-    for (int i = 0; i < FI; ++i)
+      for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) {
-        if constexpr (FI * FJ >= 64)
-          mma_pinned(fa[kk][i], fb[kk][j], acc[i][j], T());
-        else
-          acc[i][j] = mma(fa[kk][i], fb[kk][j], acc[i][j], T());
+        for (int j = 0; j < FJ; ++j) acc[i][j] = mma(fa[kk][i], fb[kk][j], acc[i][j], T());
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      if (LOAD) aim();
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+          if (j * FI / FJ == i) fb[1 - kk][j] = TB::frag(pb, wj + j * 16, 1 - kk);
+        fa[1 - kk][i] = TA::frag(pa, wi + i * 16, 1 - kk);
+        if (LOAD) {
+#pragma unroll
+          for (int n = 0; n < TA::LOADS; ++n)
+            if (n * FI / TA::LOADS == i) la.load(qa, n);
+#pragma unroll
+          for (int n = 0; n < TB::LOADS; ++n)
+            if (n * FI / TB::LOADS == i) lb.load(qb, n);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) mma_pinned(fa[kk][i], fb[kk][j], acc[i][j], T());
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
   };
   auto step = [&](char* ca, char* cb, char* na, char* nb) __attribute__((always_inline)) {
-    read(ca, cb, 1);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
+    half(0, ca, cb, std::false_type(), nullptr, nullptr);
     settle(na, nb);
     __builtin_amdgcn_sched_barrier(0);
-    read(na, nb, 0);
-    start(ca, cb);
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
+    half(1, na, nb, std::true_type(), ca, cb);
   };
   // (the sums stand in their registers before the wait, and are taken from them behind the next)
   auto pin = [&]() __attribute__((always_inline)) {
@@ -567,7 +618,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 #pragma unroll
       for (int j = 0; j < FJ; ++j) asm volatile("" : "+a"(acc[i][j]));
   };
-  if constexpr (FI * FJ >= 64) {
+  if constexpr (kPinned) {
     // written sums before the first matrix instruction reads them
     pin();
     asm volatile("s_nop 7" ::: "memory");
@@ -585,7 +636,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
     read(a0, b0, 0);
     start(a1, b1);
   }
-  if constexpr (FI * FJ >= 64) {
+  if constexpr (kPinned) {
     // (a step past the end multiplies zeros)
     for (; s < end; s += 2) {
       step(a0, b0, a1, b1);
@@ -604,7 +655,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
     }
   }
   // the last matrix instructions, 8 passes of 4 cycles, before their sums are read
-  if constexpr (FI * FJ >= 64) {
+  if constexpr (kPinned) {
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
     pin();
   }
@@ -632,7 +683,8 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
     // this wave's row of the bias gradient's partial sums
     const int row = CI ? (tj * NWJ + wave / NWI) * PASSES + h
                        : (z * g.tiles_i + ti) * NWI + wave % NWI;
-    finish_tile<T, MODE, CI, WI, HJ * 16>(g, tile, row_sums[wave], i0 + wi, j0 + wj + h * HJ * 16, z, row);
+    finish_tile<T, MODE, CI, WI, HJ * 16>(g, tile, row_sums[wave], i0 + wi,
+                                          j0 + wj + h * HJ * 16, z, row);
     __builtin_amdgcn_wave_barrier();
   };
   static_assert(PASSES <= 2, "passes are written out: the sums have to stay in registers");
@@ -649,7 +701,8 @@ constexpr int kFewWaves = 8;
 
 template <typename T, int FR, int JB, int MODE>
 __global__ __launch_bounds__(kFewWaves * 64) void few_tokens(const ProductArgs g) {
-  constexpr bool kPair = MODE == kGated;
+  constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
+  constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
   constexpr int E = 16 / (int)sizeof(T), HALVES = kPair ? 2 : 1, FA = FR * HALVES;
   constexpr int STEP = 8 * E;  // k of a step: two chunks of each of the four lane groups
   constexpr int DEPTH = FA * JB >= 8 ? 1 : FA * JB >= 4 ? 2 : 4;
@@ -741,34 +794,79 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_tokens(const ProductArgs g
       b = join[0][(fi * 2 + 1) * JB + fj][lane];
       for (int w = 1; w < kFewWaves; ++w) b += join[w][(fi * 2 + 1) * JB + fj][lane];
     }
-    if (j >= g.J) continue;
     const T* bias = (const T*)g.bias;
-    const T* res = (const T*)g.other;
+    const T* other = (const T*)g.other + (long long)j * g.ldother;
     T* out = (T*)g.out + (long long)j * g.ldo;
-    float z[4], v[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) z[r] = a[r] + (bias && i + r < outs ? to_f32(bias[i + r]) : 0.f);
-    activate<sizeof(T) == 2, false>(g.act, z, v, v, g.slope);
+    float z[4], v[4], w[4], d[4];
+    bool ok[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      if (i + r >= outs) continue;
-      if (kPair)
-        v[r] *= b[r] + (bias ? to_f32(bias[g.pair + i + r]) : 0.f);
-      else if (res)
-        v[r] += to_f32(res[(long long)j * g.ldother + i + r]);
-      out[i + r] = narrow<T>(v[r]);
+      ok[r] = j < g.J && i + r < outs;
+      z[r] = a[r] + (bias && i + r < outs ? to_f32(bias[i + r]) : 0.f);
+      w[r] = b[r];
+      if (kPair && bias && i + r < outs) w[r] += to_f32(bias[g.pair + i + r]);
+    }
+    activate<sizeof(T) == 2, kDz>(g.act, z, v, d, g.slope);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float o = g.other && ok[r] ? to_f32(other[i + r]) : 0.f;
+      if constexpr (MODE == kLinear) {
+        v[r] += o;
+      } else if constexpr (MODE == kGated) {
+        v[r] *= w[r];
+      } else if constexpr (MODE == kLinearDz) {
+        v[r] = ok[r] ? o * d[r] : 0.f;
+      } else {
+        const float dz = ok[r] ? o * w[r] * d[r] : 0.f;
+        w[r] = ok[r] ? o * v[r] : 0.f;
+        v[r] = dz;
+      }
+      if (kDz && g.sums) {
+        // the bias gradient's row of these 16 tokens
+        float sv = v[r], sw = w[r];
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) {
+          sv += __shfl_xor(sv, m, 64);
+          if (kPair) sw += __shfl_xor(sw, m, 64);
+        }
+        float* sums = g.sums + (long long)fj * (kPair ? 2 * g.pair : g.I);
+        if (l == 0 && i + r < outs) {
+          sums[i + r] = sv;
+          if (kPair) sums[g.pair + i + r] = sw;
+        }
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < (kDz && sizeof(T) == 2 ? 2 : 1); ++part) {
+      if (part && !g.low) break;
+      if (part) {
+        rounded_off<T, 4>(v);
+        rounded_off<T, 4>(w);
+        out += g.low;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (ok[r]) {
+          out[i + r] = narrow<T>(v[r]);
+          if (MODE == kGatedDz) out[g.pair + i + r] = narrow<T>(w[r]);
+        }
     }
   }
 }
 
 template <typename T, int FR, int JB>
 static hipError_t launch_few(const ProductArgs& g, hipStream_t stream) {
-  const bool gated = g.mode == kGated;
-  const unsigned blocks = (unsigned)(((gated ? g.pair : g.I) + 16 * FR - 1) / (16 * FR));
-  if (gated)
-    few_tokens<T, FR, JB, kGated><<<blocks, kFewWaves * 64, 0, stream>>>(g);
-  else
-    few_tokens<T, FR, JB, kLinear><<<blocks, kFewWaves * 64, 0, stream>>>(g);
+  const int outs = g.mode == kGated || g.mode == kGatedDz ? g.pair : g.I;
+  const unsigned blocks = (unsigned)((outs + 16 * FR - 1) / (16 * FR));
+#define FEW(MODE) few_tokens<T, FR, JB, MODE><<<blocks, kFewWaves * 64, 0, stream>>>(g)
+  switch (g.mode) {
+    case kLinear: FEW(kLinear); break;
+    case kLinearDz: FEW(kLinearDz); break;
+    case kGated: FEW(kGated); break;
+    case kGatedDz: FEW(kGatedDz); break;
+    default: return hipErrorInvalidValue;
+  }
+#undef FEW
   return hipGetLastError();
 }
 
@@ -804,7 +902,7 @@ static hipError_t by_operands(const ProductArgs& g, hipStream_t stream) {
       case kLinearDz: PRODUCT(false, true, kLinearDz);
       case kGated: PRODUCT(false, true, kGated);
       case kGatedDz: PRODUCT(false, true, kGatedDz);
-      case kPlain: PRODUCT(false, true, kPlain);
+      case kPartial: PRODUCT(false, true, kPartial);
     }
   else switch (g.mode) {
       case kPlain: PRODUCT(false, false, kPlain);
@@ -823,7 +921,6 @@ hipError_t product_t(const ProductArgs& g, const ProductPlan& p, hipStream_t str
     case kTile64: return by_operands<T, 64, 64, 2, 2, 1, true>(g, stream);
     case kTile64Any: return by_operands<T, 64, 64, 2, 2, 1, false>(g, stream);
     case kTile128: return by_operands<T, 128, 128, 2, 2, 1, true>(g, stream);
-    case kTile128Any: return by_operands<T, 128, 128, 2, 2, 1, false>(g, stream);
     case kTile256:
       if constexpr (sizeof(T) == 2) return by_operands<T, 256, 256, 2, 2, 2, true>(g, stream);
   }

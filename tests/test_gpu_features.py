@@ -79,6 +79,7 @@ class Product64:
 
     def __init__(self, x, w, b, act, slope, gated, dtype, res=None):
         self.x, self.w, self.gated, self.u = x.double(), w.double(), gated, u(dtype)
+        self.kept = u(dtype)  # what dz loses where the backward keeps it
         self.floor = _floor(dtype)
         self.act = act
         K = x.shape[1]
@@ -120,7 +121,7 @@ class Product64:
             e = dy.abs() * edf
         if self.gated or self.act != "none":  # kept in the storage type
             e = e + 3 * F32 * dz.abs()
-            e = e + self.u * (dz.abs() + e) + self.floor
+            e = e + self.kept * (dz.abs() + e) + self.floor
         M, rows = dz.shape
         a = dz.abs() + e
         out = {}
@@ -233,6 +234,49 @@ def test_few_tokens(tokens, dtype):
     for K, O, gated in ((1024, 520, False), (1536, 200, True), (777, 65, False), (129, 50, True)):
         case = _product_case(False, (tokens,), K, O, dtype, "silu", True, not gated, gated)
         _check_product(*case, "silu", gated, -1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("is_map,dims,K,O,gated", [
+    (False, (1,), 512, 96, False), (False, (7,), 264, 130, True), (False, (40,), 1000, 65, True),
+    (False, (3440,), 176, 8, True), (False, (777,), 65, 33, False), (True, (7, 3, 2), 1, 40, False),
+    (True, (3, 24, 28), 32, 48, True), (True, (2, 37, 53), 33, 17, True)])
+def test_small_gradients_keep_their_bits(is_map, dims, K, O, gated, dtype):
+    """In small 16-bit calls dz is kept in two parts, u^2 off instead of u (the second part of a
+    16-bit value is at most u of it and rounded itself; fp16's is off by the subnormal step too)."""
+    import pwcnet_amd as P
+    x, w, b, _, g = _product_case(is_map, dims, K, O, dtype, "silu", True, False, gated)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = (P.gated_linear if gated else P.linear)(x, w, b, activation="silu",
+                                               channel_dim=1 if is_map else -1)
+    grads = torch.autograd.grad(y, leaves, g)
+    with torch.no_grad():
+        ref = Product64(_tok(x, is_map), w, b, "silu", 0.1, gated, dtype)
+        ref.kept = u(dtype) ** 2
+        back = ref.backward(_tok(g, is_map))
+        _within("dx", _tok(grads[0], is_map), *back["dx"])
+        _within("dw", grads[1], *back["dw"])
+
+
+def test_small_gradients_beyond_the_type():
+    """A dz that rounds to infinity gives infinite gradients, no NaN."""
+    import pwcnet_amd as P
+    for tokens in (3, 70):
+        x = torch.full((tokens, 32), 4.0, dtype=torch.float16, device=DEV, requires_grad=True)
+        w = torch.full((48, 32), 0.25, dtype=torch.float16, device=DEV, requires_grad=True)
+        y = P.gated_linear(x, w, None, "silu", channel_dim=-1)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.full_like(y, 65504.0))
+        assert bool(torch.isposinf(dx).all()) and bool(torch.isposinf(dw).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_few_tokens_long_gradients(dtype):
+    """dx of few tokens over many output channels is summed in parts."""
+    for tokens, K, O, gated in ((1, 264, 2100, False), (7, 96, 1500, True), (64, 65, 1031, False),
+                                (65, 200, 1024, True)):
+        for act in ("none", "gelu"):
+            case = _product_case(False, (tokens,), K, O, dtype, act, True, False, gated)
+            _check_product(*case, act, gated, -1)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
