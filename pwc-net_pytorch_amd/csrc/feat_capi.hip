@@ -85,15 +85,21 @@ View dz_view(const Problem& p, const void* dz) {
   return {dz, p.P, p.rows * p.P, 0};
 }
 
-// The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
-// not, large ones are laid out so first: rows of odd 16-bit lengths read through registers cost the
-// three backward products 2 to 7 times their time (8191 x 1023 -> 4095: 1.2 ms instead of 0.25),
-// the copies tens of microseconds.  Small calls, and 32-bit ones below 8 GFLOP, read them as they
-// lie.
-constexpr double kKeepLow = 5e8;  // operations of a product
+constexpr double kKeepLow = 5e8;  // operations of a product whose dz is kept in two parts
 
-bool pads_pay(const Problem& p) {
-  return 2.0 * (double)p.M * p.rows * p.K >= (p.dtype == 0 ? 8e9 : 2e9);
+// The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
+// not, large ones are laid out so first.  Forward alone that is worth its launches from some GFLOP
+// on (us, as they lie / laid out first; 16 bits: 2047 x 1023 -> 1023, 4.3 GFLOP: 19 / 25;
+// 8191 x 1023 -> 4095: 164 / 103).  Backward the three products share the copies, and rows of odd
+// 16-bit lengths that are read across k cost most (act'; 1001 x 511 -> 511: 56 / 38, 2047 x 1023 ->
+// 1023: 137 / 65; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 60; fp32 2001 x 701 -> 1001: 160 / 131),
+// unless so few channels meet that the products are all traffic anyway (map 16 x 64 x 113 x 129 ->
+// 64: 81 / 88, fp32 136 / 155).
+bool pads_pay(const Problem& p, bool backward) {
+  const double operations = 2.0 * (double)p.M * p.rows * p.K;
+  if (!backward) return operations >= 8e9;
+  if (p.K < 96 || p.rows < 96) return operations >= 8e9;
+  return operations > (tokens(p) && p.dtype != 0 ? kKeepLow : 1e9);
 }
 long long whole(const Problem& p, long long cols) {
   const long long e = 16 / (long long)elem(p.dtype);
@@ -212,7 +218,7 @@ ForwardSpace forward_space(const Problem& p, const void* x, const void* w) {
   const ProductPlan plan = product_plan(
       y_args(p, x_view(p, x), w_view(p, w), nullptr, nullptr, nullptr), p.dtype);
   const bool few = plan.kernel == kFew16 || plan.kernel == kFew32 || plan.kernel == kFew64;
-  if (few || !pads_pay(p)) return s;
+  if (few || !pads_pay(p, false)) return s;
   s.pad_x = !lies_well(p, x_view(p, x), x_cols(p));
   s.pad_w = !lies_well(p, w_view(p, w), p.K);
   s.w = s.pad_x ? bytes_of(p, x_rows(p), x_cols(p)) : 0;
@@ -230,7 +236,7 @@ struct BackwardSpace {
 BackwardSpace backward_space(const Problem& p, const void* x, const void* w, const void* dy,
                              const char* ws, bool dx, bool dw, bool db) {
   BackwardSpace s = {};
-  const bool z = needs_z(p), pay = pads_pay(p);
+  const bool z = needs_z(p), pay = pads_pay(p, true);
   s.xv = x_view(p, x), s.wv = w_view(p, w), s.dzv = dz_view(p, z ? nullptr : dy);
   s.pad_x = pay && (z || dw) && !lies_well(p, s.xv, x_cols(p));
   s.pad_w = pay && (z || dx) && !lies_well(p, s.wv, p.K);
@@ -238,7 +244,7 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   // dz in 16 bits is rounded once, which makes the gradients' error 1.4 times that of their own
   // rounding; in small calls, where chance adds to that, what the rounding took follows as more k,
   // at a cost that the launches hide.  (Only the kernels of such calls can write it.)
-  if (z && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
+  if (z && !s.pad_dz && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
       product_plan(dz_args(p, s.xv, s.wv, nullptr, dy, s.dzv), p.dtype).kernel <= kTile64Any)
     s.low = tokens(p) ? p.M * p.rows : p.rows * p.P;
   size_t at = 0;
