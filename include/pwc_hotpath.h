@@ -304,6 +304,7 @@ PWC_API int pwc_corr_forward_group(const pwc_corr_problem* problems, int count, 
  *                      x + n * x_stride elements (>= C * P)
  *   PWC_LAYOUT_TOKENS  x[P][C] (B = 1); token m starts at x + m * x_stride elements (>= C)
  * Only the first input may be strided that way; every other tensor is dense in the same layout.
+ * No output overlaps an input, unless an entry allows it.
  * Weights, biases and activations share one `dtype`; sums, statistics and activations are fp32,
  * every output is rounded once.  Any alignment of a pointer to its element type is accepted;
  * workspaces are aligned to 256 bytes.
@@ -369,7 +370,9 @@ PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bi
                                float negative_slope, int dtype, void* workspace,
                                size_t workspace_bytes, void* stream);
 /* grad_x, grad_weight, grad_bias (each may be NULL: not computed).  The residual's gradient is
- * grad_out itself.  Deterministic.  The size is that of all three. */
+ * grad_out itself.  Deterministic.  The size is that of all three.  With an activation, the
+ * gradient of the sums is kept in `dtype` between the products, in small 16-bit calls as a value and
+ * what its rounding took; where x or weight is infinite a gradient is infinite or NaN. */
 PWC_API size_t pwc_linear_backward_workspace_size(const void* x, const void* weight,
                                                   const void* grad_out, int layout, long long B,
                                                   long long P, int K, int O, long long x_stride,

@@ -56,7 +56,8 @@ std::vector<std::string> entry_names() {
   };
 }
 
-void bind(const py::dict& at) {
+void bind(const py::dict& at) {  // (under the interpreter's lock: threads that ask at once, once)
+  if (g_bound.load(std::memory_order_acquire)) return;
   Entries e;
 #define E(name) e.name = reinterpret_cast<decltype(e.name)>(at[#name].cast<uintptr_t>());
   PWC_ENTRIES(E)
@@ -86,6 +87,7 @@ void check(const char* what, const Tensor& x, std::initializer_list<const Tensor
     TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), what, ": mixed dtypes ",
                      t.scalar_type(), " vs ", x.scalar_type());
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, ": dense tensors only");
+    TORCH_CHECK_TYPE(!t.is_neg(), what, ": negated views are not read: resolve_neg() first");
   };
   one(x);
   for (const Tensor* t : others)
@@ -416,6 +418,9 @@ Grads product_backward(bool gated, const Tensor& x, const Tensor& w, const Tenso
 
 // ---- autograd ----
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  // forward-mode derivatives go the same way: the node refuses them
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;

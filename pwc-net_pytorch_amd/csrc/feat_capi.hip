@@ -24,6 +24,14 @@ const char* bad_shape(int layout, long long B, long long P, long long C, int dty
   return nullptr;
 }
 
+// Images of one pixel are tokens: the kernels' tiles would take one pixel each.
+void by_tokens(int& layout, long long& B, long long& P) {
+  if (layout != PWC_LAYOUT_MAP || P != 1) return;
+  layout = PWC_LAYOUT_TOKENS;
+  P = B;
+  B = 1;
+}
+
 const char* bad_stride(int layout, long long B, long long P, long long C, long long stride) {
   const long long rows = layout == PWC_LAYOUT_MAP ? B : P;
   const long long least = layout == PWC_LAYOUT_MAP ? P * C : C;
@@ -58,6 +66,7 @@ const char* bad_problem(const Problem& p) {
 
 Problem problem(int layout, long long B, long long P, int K, int O, long long x_stride, int act,
                 float slope, int dtype, int gated) {
+  by_tokens(layout, B, P);
   Problem p = {layout, K, O, O, act, dtype, gated, B, P, 0, x_stride, slope};
   if (gated && O > 0 && O <= (1 << 23)) p.rows = 2 * O;  // (larger ones are refused)
   p.M = layout == PWC_LAYOUT_MAP && B >= 0 && P >= 0 && B <= kIntMax && P <= kIntMax ? B * P : P;
@@ -376,8 +385,6 @@ NormArgs norm_args(int layout, long long B, long long P, int C, long long x_stri
 }
 const char* bad_norm(int layout, long long B, long long P, int C, long long x_stride, int dtype) {
   if (const char* e = bad_shape(layout, B, P, C, dtype)) return e;
-  // one block a row (tokens) or a 64-pixel tile (maps)
-  if (B * ((P + 63) / 64) > kIntMax) return "dimension too large";
   return bad_stride(layout, B, P, C, x_stride);
 }
 }  // namespace
@@ -388,6 +395,7 @@ PWC_API int pwc_layer_norm_forward(const void* x, const void* weight, const void
                                    void* mean, void* rstd, int layout, long long B, long long P,
                                    int C, long long x_stride, float eps, int dtype, void* stream) {
   const char* fn = "pwc_layer_norm_forward";
+  by_tokens(layout, B, P);
   if (const char* e = bad_norm(layout, B, P, C, x_stride, dtype)) return api_fail(fn, e);
   if (!(eps >= 0.f)) return api_fail(fn, "eps must not be negative");
   if ((mean == nullptr) != (rstd == nullptr)) return api_fail(fn, "mean and rstd come together");
@@ -406,6 +414,7 @@ PWC_API int pwc_layer_norm_forward(const void* x, const void* weight, const void
 
 PWC_API size_t pwc_layer_norm_backward_workspace_size(int layout, long long B, long long P, int C,
                                                       int dtype) {
+  by_tokens(layout, B, P);
   if (bad_shape(layout, B, P, C, dtype)) return 0;
   return align256((size_t)2 * norm_parts(layout, B, P, C, dtype) * C * sizeof(float));
 }
@@ -416,6 +425,7 @@ PWC_API int pwc_layer_norm_backward(const void* x, const void* weight, const voi
                                     long long P, int C, long long x_stride, int dtype,
                                     void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "pwc_layer_norm_backward";
+  by_tokens(layout, B, P);
   if (const char* e = bad_norm(layout, B, P, C, x_stride, dtype)) return api_fail(fn, e);
   const bool sums = grad_weight || grad_bias;
   if (!grad_x && !sums) return api_launch(fn, hipSuccess);
@@ -449,6 +459,7 @@ PWC_API int pwc_rotary(const void* x, void* y, const void* positions, const void
   if (s.B < 0 || s.N < 0 || s.heads < 0 || s.D < 0) return api_fail(fn, "negative dimension");
   if (s.B > kIntMax || s.N > kIntMax || s.heads > (1 << 20) || s.D > (1 << 20))
     return api_fail(fn, "dimension too large");
+  if ((long long)s.heads * s.D > kIntMax) return api_fail(fn, "dimension too large");
   if (s.pairs < 0 || 2LL * s.pairs > s.D) return api_fail(fn, "more pairs than channels");
   if (s.axes < 1 || s.axes > kMaxAxes) return api_fail(fn, "1 to 4 axes");
   if (positions) {

@@ -174,7 +174,7 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
   } else if (act == kActTanh) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      // small z in 16 bits: 2 sigmoid(2 z) - 1 loses the digits that 1 has more than z
+      // (2 sigmoid(2 z) - 1 would lose a small z's digits)
       f[e] = tanhf(z[e]);
       if (SLOPE) d[e] = 1.f - f[e] * f[e];
     }
@@ -185,6 +185,16 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
       if (SLOPE) d[e] = 1.f;
     }
   }
+}
+
+// A grid of any number of blocks: one dimension holds 2^24 of 256 threads.  Blocks behind the last
+// have work of their own to check for.
+__device__ __forceinline__ long long block_id() {
+  return blockIdx.y * (long long)gridDim.x + blockIdx.x;
+}
+inline dim3 grid_of(long long blocks) {
+  const long long x = blocks < (1 << 20) ? blocks : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
 inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
   __shared__ float red[4];
   constexpr int RPB = 256 / TPR;
   const int t = threadIdx.x % TPR;
-  const long long m = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const long long m = block_id() * RPB + threadIdx.x / TPR;
   const bool row = m < a.M;
   const T* x = (const T*)a.x + (row ? m : 0) * a.x_stride;
   float v[NV][V];
@@ -236,9 +236,9 @@ __global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
   const int g = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);  // channels: uniform
   const uint32_t P = (uint32_t)a.P;  // (an image's offsets fit 32 bits)
   const long long tiles = (a.P + 64 * PV - 1) / (64 * PV);
-  const long long img = blockIdx.x / tiles;
-  const uint32_t p = (uint32_t)((blockIdx.x % tiles * 64 + l) * PV);
-  const bool ok = p < P;
+  const long long id = block_id(), img = id / tiles;
+  const uint32_t p = (uint32_t)((id % tiles * 64 + l) * PV);
+  const bool ok = p < P && img < a.B;
   const T* x = (const T*)a.x + img * a.x_stride;
   float v[NC][PV], s[PV], r[PV], mu[PV];
 #pragma unroll
@@ -372,18 +372,18 @@ struct RowAt {
 template <bool MAP> __device__ __forceinline__ RowAt row_at(const NormArgs& a) {
   RowAt r;
   if (MAP) {
-    const long long tiles = (a.P + 63) / 64, img = blockIdx.x / tiles;
-    const long long p = blockIdx.x % tiles * 64 + (threadIdx.x & 63);
-    r.ok = p < a.P;
-    r.base = img * a.x_stride + (r.ok ? p : 0);
-    r.y = img * a.C * a.P + (r.ok ? p : 0);
+    const long long tiles = (a.P + 63) / 64, id = block_id(), img = id / tiles;
+    const long long p = id % tiles * 64 + (threadIdx.x & 63);
+    r.ok = p < a.P && img < a.B;
+    r.base = r.ok ? img * a.x_stride + p : 0;
+    r.y = r.ok ? img * a.C * a.P + p : 0;
     r.stride = a.P;
     r.m = img * a.P + p;
   } else {
-    r.m = blockIdx.x;
-    r.ok = true;
-    r.base = r.m * a.x_stride;
-    r.y = r.m * a.C;
+    r.m = block_id();
+    r.ok = r.m < a.M;
+    r.base = r.ok ? r.m * a.x_stride : 0;
+    r.y = r.ok ? r.m * a.C : 0;
     r.stride = 1;
   }
   return r;
@@ -550,7 +550,7 @@ template <typename T, int TPR, int V, int NV = 1>
 static void tokens_nv(const NormArgs& a, int nv, bool back, int parts, hipStream_t s) {
   if constexpr (NV * V <= most_values(TPR)) {
     if (nv != NV) return tokens_nv<T, TPR, V, 2 * NV>(a, nv, back, parts, s);
-    const unsigned grid = (unsigned)((a.M + 256 / TPR - 1) / (256 / TPR));
+    const dim3 grid = grid_of((a.M + 256 / TPR - 1) / (256 / TPR));
     const size_t lds = 16 + (TPR < 256 ? 8 * sizeof(float) * a.C : 0);
     if (back)
       norm_tokens_backward<T, TPR, NV, V><<<parts, 256, lds, s>>>(a);
@@ -578,7 +578,7 @@ template <typename T> static bool tokens(const NormArgs& a, bool back, int parts
 
 template <typename T, int PV>
 static void map_pv(const NormArgs& a, bool back, int parts, hipStream_t s) {
-  const unsigned grid = (unsigned)(a.B * ((a.P + 64 * PV - 1) / (64 * PV)));
+  const dim3 grid = grid_of(a.B * ((a.P + 64 * PV - 1) / (64 * PV)));
 #define NORM_MAP(G, NC)                                                    \
   (back ? norm_map_backward<T, G, NC, PV><<<parts, 64 * G, 0, s>>>(a)      \
         : norm_map<T, G, NC, PV><<<grid, 64 * G, 0, s>>>(a))
@@ -611,9 +611,9 @@ template <typename T> static hipError_t forward_t(const NormArgs& a, hipStream_t
   const bool is_map = a.layout == kMap;
   if (is_map ? map<T>(a, false, 0, s) : tokens<T>(a, false, 0, s)) return hipGetLastError();
   if (is_map)
-    norm_any<T, true><<<(unsigned)(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
+    norm_any<T, true><<<grid_of(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
   else
-    norm_any<T, false><<<(unsigned)a.M, 256, 0, s>>>(a);
+    norm_any<T, false><<<grid_of(a.M), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -622,9 +622,9 @@ template <typename T> static hipError_t backward_t(const NormArgs& a, int parts,
   if (!(is_map ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s))) {
     if (a.dx) {
       if (is_map)
-        norm_any_dx<T, true><<<(unsigned)(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
+        norm_any_dx<T, true><<<grid_of(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
       else
-        norm_any_dx<T, false><<<(unsigned)a.M, 256, 0, s>>>(a);
+        norm_any_dx<T, false><<<grid_of(a.M), 256, 0, s>>>(a);
     }
     if (a.part) {
       if (is_map)

@@ -497,8 +497,9 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 
   // tile (ti, tj) of batch / k split z; neighbouring tiles on one XCD
   // (4 tiles along j at a time: 32 tiles in flight on an XCD share 8 tiles of A and 4 of B)
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int plane = g.tiles_i * g.tiles_j, z = id / plane, at = id - z * plane;
+  const int plane = g.tiles_i * g.tiles_j, blocks = plane * (PART ? g.splits : g.batches);
+  if (block_id() >= blocks) return;
+  const int id = xcd_remap((int)block_id(), blocks), z = id / plane, at = id - z * plane;
   const int group = at / (4 * g.tiles_i), first = group * 4, in = at - group * 4 * g.tiles_i;
   const int deep = min(4, g.tiles_j - first);
   const int ti = in / deep, tj = first + in % deep;
@@ -881,7 +882,7 @@ static hipError_t launch(ProductArgs g, hipStream_t stream) {
       (long long)g.tiles_i * g.tiles_j * (g.mode == kPartial ? g.splits : g.batches);
   if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
   product<T, BI, BJ, NWI, NWJ, PASSES, AKC, BKC, MODE, DIRECT>
-      <<<(unsigned)blocks, NWI * NWJ * 64, 0, stream>>>(g);
+      <<<grid_of(blocks), NWI * NWJ * 64, 0, stream>>>(g);
   return hipGetLastError();
 }
 

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void rotary_rows(const RotaryArgs a) {
   const int units = (a.R + V - 1) / V;                     // of a token's pairs
   const int rest = (a.D - 2 * a.R + 2 * V - 1) / (2 * V);  // units of the channels that pass
   const long long per = (units + rest) * (long long)a.head_groups;
-  const long long id = blockIdx.x * 256LL + threadIdx.x;
+  const long long id = block_id() * 256 + threadIdx.x;
   if (id >= a.B * a.N * per) return;
   const long long bn = id / per;
   const uint32_t in = (uint32_t)(id - bn * per);
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void rotary_rows(const RotaryArgs a) {
 template <typename T, int V>
 __global__ __launch_bounds__(256) void rotary_pixels(const RotaryArgs a) {
   const uint32_t nv = (uint32_t)((a.N + V - 1) / V);
-  const long long id = blockIdx.x * 256LL + threadIdx.x;
+  const long long id = block_id() * 256 + threadIdx.x;
   const int units = a.R + (a.D - 2 * a.R + 1) / 2;
   if (id >= (long long)nv * units * a.H * a.batch_groups) return;
   const long long rows = id / nv;
@@ -214,13 +214,13 @@ template <typename T> static hipError_t rotary_t(RotaryArgs a, hipStream_t strea
     a.heads_each = (int)((a.H + groups - 1) / groups);
     a.head_groups = (a.H + a.heads_each - 1) / a.heads_each;
     const long long blocks = (a.B * a.N * units * a.head_groups + 255) / 256;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    const dim3 grid = grid_of(blocks);
     if (a.interleaved)
-      vec ? rotary_rows<T, V, true><<<(unsigned)blocks, 256, 0, stream>>>(a)
-          : rotary_rows<T, 1, true><<<(unsigned)blocks, 256, 0, stream>>>(a);
+      vec ? rotary_rows<T, V, true><<<grid, 256, 0, stream>>>(a)
+          : rotary_rows<T, 1, true><<<grid, 256, 0, stream>>>(a);
     else
-      vec ? rotary_rows<T, V, false><<<(unsigned)blocks, 256, 0, stream>>>(a)
-          : rotary_rows<T, 1, false><<<(unsigned)blocks, 256, 0, stream>>>(a);
+      vec ? rotary_rows<T, V, false><<<grid, 256, 0, stream>>>(a)
+          : rotary_rows<T, 1, false><<<grid, 256, 0, stream>>>(a);
     return hipGetLastError();
   }
   const bool vec = base && a.xs_n == 1 && a.ys_n == 1 && a.N % V == 0 &&
@@ -235,9 +235,9 @@ template <typename T> static hipError_t rotary_t(RotaryArgs a, hipStream_t strea
   a.batch_each = (a.B + groups - 1) / groups;
   a.batch_groups = (a.B + a.batch_each - 1) / a.batch_each;
   const long long blocks = (one * a.batch_groups + 255) / 256;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-  vec ? rotary_pixels<T, V><<<(unsigned)blocks, 256, 0, stream>>>(a)
-      : rotary_pixels<T, 1><<<(unsigned)blocks, 256, 0, stream>>>(a);
+  const dim3 grid = grid_of(blocks);
+  vec ? rotary_pixels<T, V><<<grid, 256, 0, stream>>>(a)
+      : rotary_pixels<T, 1><<<grid, 256, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -155,7 +155,8 @@ class CostVolumeLayer(nn.Module):
 # ---------------------------------------------------------------------------------------
 def _traced(x):
     """Tracers see one opaque torch.ops.pwcnet node; eager calls go straight to the kernels."""
-    return torch.compiler.is_compiling() or type(x) not in (torch.Tensor, nn.Parameter)
+    return (type(x) not in (torch.Tensor, nn.Parameter) or torch.compiler.is_compiling()
+            or torch._C._len_torch_dispatch_stack() > 0)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=1):

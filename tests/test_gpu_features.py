@@ -982,3 +982,96 @@ def test_threads_and_inplace_changes():
         c.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+def test_images_of_one_pixel_are_tokens():
+    """[B, C, 1, 1] gives the values and gradients of [B, C], from a strided batch too."""
+    import pwcnet_amd as P
+    for dtype in DTYPES:
+        gen = _gen("pixel", str(dtype))
+        w, b, g = (_rand(gen, 96, 40, dtype=dtype, scale=0.2), _rand(gen, 96, dtype=dtype),
+                   _rand(gen, 70, 48, dtype=dtype))
+        wide = _rand(gen, 70, 43, dtype=dtype)
+        for x in (wide[:, :40].contiguous(), wide[:, 3:]):
+            got = []
+            for shape, dim in (((70, 40), -1), ((70, 40, 1, 1), 1)):
+                v = x.detach().reshape(70, 40) if dim == -1 else x.detach()[:, :, None, None]
+                leaves = [v.requires_grad_(True), w.clone().requires_grad_(True),
+                          b.clone().requires_grad_(True)]
+                n = P.layer_norm(leaves[0], channel_dim=dim)
+                y = P.gated_linear(n, *leaves[1:], channel_dim=dim)
+                assert y.shape == (70, 48, *shape[2:])
+                grads = torch.autograd.grad(y, leaves, g.reshape(y.shape))
+                got.append([t.reshape(70, -1) if t.shape[0] == 70 else t for t in (y, *grads)])
+            assert all(torch.equal(p.detach(), q.detach()) for p, q in zip(*got))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values: the last rows equal a call on them alone."""
+    import pwcnet_amd as P
+    M, C, last = 2 ** 20 + 70, 2056, 66
+    x = torch.empty(M, C, dtype=torch.bfloat16, device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(5))
+    gen = _gen("far")
+    w = _rand(gen, 24, C, dtype=torch.bfloat16, scale=C ** -0.5)
+    b = _rand(gen, C, dtype=torch.bfloat16)
+    assert torch.equal(P.layer_norm(x, b, b, channel_dim=-1)[-last:],
+                       P.layer_norm(x[-last:], b, b, channel_dim=-1))
+    inv, axis = P.rotary_frequencies((C // 8,), device=DEV)
+    at = torch.arange(M, device=DEV)[:, None]
+    assert torch.equal(P.rotary(x.view(1, M, 4, C // 4), inv, axis, at)[:, -last:],
+                       P.rotary(x[-last:].view(1, last, 4, C // 4), inv, axis, at[-last:]))
+    # (the whole and the part may take other kernels: sums of the same products in another order)
+    whole, part = P.linear(x, w, channel_dim=-1)[-last:], P.linear(x[-last:], w, channel_dim=-1)
+    bound = x[-last:].float().abs() @ w.float().abs().t()
+    _within("linear", whole, part, 2 * C * F32 * bound
+            + 2 * u(torch.bfloat16) * (part.abs().float() + 2 * C * F32 * bound))
+    dy = _rand(gen, M, 24, dtype=torch.bfloat16)
+    from pwcnet_amd import features
+    gx = features.linear_backward(x, w, None, dy, channel_dim=-1, needs=(True, False, False))[0]
+    ref = dy[-last:].double() @ w.double()
+    tol = 26 * F32 * (dy[-last:].double().abs() @ w.double().abs())
+    _within("dx", gx[-last:], ref, tol + u(torch.bfloat16) * (ref.abs() + tol))
+    del gx, whole
+    # a map whose image is that large
+    m, v = x.view(-1)[: 2 ** 31 + 64].view(1, 2, -1), _rand(gen, 3, 2, dtype=torch.bfloat16)
+    assert torch.equal(P.linear(m, v)[..., -64:], P.linear(m[..., -64:].contiguous(), v))
+    assert torch.equal(P.layer_norm(m)[..., -64:], P.layer_norm(m[..., -64:].contiguous()))
+
+
+def test_derivatives_that_there_are_not():
+    """Forward-mode derivatives and negated views are refused, not dropped."""
+    import torch.autograd.forward_ad as fwad
+    import pwcnet_amd as P
+    x, w = torch.randn(4, 8, device=DEV), torch.randn(6, 8, device=DEV)
+    inv, axis = P.rotary_frequencies((4,), device=DEV)
+    with fwad.dual_level():
+        d = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: P.layer_norm(d, channel_dim=-1), lambda: P.linear(d, w, channel_dim=-1),
+                     lambda: P.gated_linear(x, fwad.make_dual(w, w), channel_dim=-1),
+                     lambda: P.rotary(d[None, :, None], inv, axis, grid=(4,))):
+            with pytest.raises(RuntimeError):
+                call()
+    neg = torch.conj(torch.randn(1, 4, 1, 8, dtype=torch.complex64, device=DEV)).imag
+    with pytest.raises(TypeError, match="negated"):
+        P.rotary(neg, inv, axis, grid=(4,))
+    assert torch.equal(P.rotary(neg.resolve_neg(), inv, axis, grid=(4,)),
+                       P.rotary(neg.clone(), inv, axis, grid=(4,)))
+
+
+def test_dispatch_modes_see_single_nodes():
+    """Under a dispatch mode an eager call shows as its node."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    import pwcnet_amd as P
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+    x, w = torch.randn(4, 8, device=DEV), torch.randn(6, 8, device=DEV)
+    want = P.linear(x, w, activation="gelu", channel_dim=-1)
+    with Names():
+        got = P.linear(x, w, activation="gelu", channel_dim=-1)
+    assert torch.equal(got, want) and any("pwcnet.linear" in n for n in seen)
