@@ -215,23 +215,28 @@ ProductArgs dw_args(const Problem& p, const View& x, const View& dz, long long l
 }
 
 // ---- workspaces, as places from their start ----
-struct ForwardSpace {
-  bool pad_x, pad_w;
-  size_t w, total;  // the padded x lies at 0
-};
 size_t bytes_of(const Problem& p, long long rows, long long cols) {
   return align256((size_t)rows * whole(p, cols) * elem(p.dtype));
 }
-ForwardSpace forward_space(const Problem& p, const void* x, const void* w) {
+struct ForwardSpace {
+  bool pad_x, pad_w;
+  size_t w, part, total;  // the padded x lies at 0
+  View xv, wv;            // as the product takes them
+};
+ForwardSpace forward_space(const Problem& p, const void* x, const void* w, const char* ws) {
   ForwardSpace s = {};
-  const ProductPlan plan = product_plan(
-      y_args(p, x_view(p, x), w_view(p, w), nullptr, nullptr, nullptr), p.dtype);
-  const bool few = plan.kernel == kFew16 || plan.kernel == kFew32 || plan.kernel == kFew64;
-  if (few || !pads_pay(p, false)) return s;
-  s.pad_x = !lies_well(p, x_view(p, x), x_cols(p));
-  s.pad_w = !lies_well(p, w_view(p, w), p.K);
+  s.xv = x_view(p, x), s.wv = w_view(p, w);
+  const int kernel =
+      product_plan(y_args(p, s.xv, s.wv, nullptr, nullptr, nullptr), p.dtype).kernel;
+  if (kernel > kFew64 && pads_pay(p, false)) {
+    s.pad_x = !lies_well(p, s.xv, x_cols(p));
+    s.pad_w = !lies_well(p, s.wv, p.K);
+  }
   s.w = s.pad_x ? bytes_of(p, x_rows(p), x_cols(p)) : 0;
-  s.total = s.w + (s.pad_w ? bytes_of(p, p.rows, p.K) : 0);
+  s.part = s.w + (s.pad_w ? bytes_of(p, p.rows, p.K) : 0);
+  if (s.pad_x) s.xv = padded_x(p, ws);
+  if (s.pad_w) s.wv = padded_w(p, ws + s.w);
+  s.total = s.part + product_part_bytes(y_args(p, s.xv, s.wv, nullptr, nullptr, nullptr), p.dtype);
   return s;
 }
 
@@ -250,11 +255,13 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   s.pad_x = pay && (z || dw) && !lies_well(p, s.xv, x_cols(p));
   s.pad_w = pay && (z || dx) && !lies_well(p, s.wv, p.K);
   s.pad_dz = pay && (z || dx || dw) && !lies_well(p, s.dzv, dz_cols(p));
+  const ProductPlan dz_plan =
+      z ? product_plan(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype) : ProductPlan();
   // dz in 16 bits is rounded once, which makes the gradients' error 1.4 times that of their own
   // rounding; in small calls, where chance adds to that, what the rounding took follows as more k,
   // at a cost that the launches hide.  (Only the kernels of such calls can write it.)
   if (z && !s.pad_dz && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
-      product_plan(dz_args(p, s.xv, s.wv, nullptr, dy, s.dzv), p.dtype).kernel <= kTile64Any)
+      (dz_plan.kernel <= kTile64Any || dz_plan.splits > 1))
     s.low = tokens(p) ? p.M * p.rows : p.rows * p.P;
   size_t at = 0;
   if (s.pad_dz)
@@ -274,11 +281,16 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   if (s.low && !tokens(p)) s.dzv.image *= 2;
   s.dx_splits = dx ? product_plan(dx_args(p, s.dzv, s.low, s.wv, nullptr), p.dtype).splits : 1;
   s.splits = dw ? product_plan(dw_args(p, s.xv, s.dzv, s.low, nullptr), p.dtype).splits : 1;
-  // (dx's parts are added before dW's are written)
+  // (the parts of each product are added before the next one's are written)
   s.part = at;
-  const size_t dx_part = s.dx_splits > 1 ? align256((size_t)s.dx_splits * p.M * p.K * 4) : 0;
-  const size_t dw_part = s.splits > 1 ? align256((size_t)s.splits * p.rows * p.K * 4) : 0;
-  at += dx_part > dw_part ? dx_part : dw_part;
+  size_t most = 0;
+  auto parts = [&](int splits, long long values) {
+    if (splits > 1 && most < (size_t)splits * values) most = (size_t)splits * values;
+  };
+  parts(dz_plan.splits, p.M * p.rows);
+  parts(s.dx_splits, p.M * p.K);
+  parts(s.splits, (long long)p.rows * p.K);
+  at += align256(most * sizeof(float));
   s.sums = at;
   if (db) {
     s.rows = z ? product_sum_rows(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype)
@@ -315,6 +327,7 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     ProductArgs g = dz_args(p, s.xv, s.wv, bias, dy, s.dzv);
     g.sums = db ? (float*)(ws + s.sums) : nullptr;
     g.low = s.low;
+    g.part = (float*)(ws + s.part);
     e = product_launch(g, p.dtype, stream);
     if (s.pad_dz && e == hipSuccess)
       e = product_zero_tails(ws, dz_rows(p), dz_cols(p), p.dtype, stream);
@@ -354,22 +367,23 @@ int product_forward(const char* fn, const Problem& p, const void* x, const void*
   if (const char* e = bad_problem(p)) return api_fail(fn, e);
   if (p.M == 0) return api_launch(fn, hipSuccess);
   if (!x || !w || !y) return api_fail(fn, "null buffer");
-  const ForwardSpace s = forward_space(p, x, w);
+  char* ws = (char*)workspace;
+  const ForwardSpace s = forward_space(p, x, w, ws);
   if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
   if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
-  char* ws = (char*)workspace;
-  View xv = x_view(p, x), wv = w_view(p, w);
   hipError_t e = hipSuccess;
   if (s.pad_x) {
-    e = product_pad(x, xv.row, xv.image, ws, tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype,
+    const View v = x_view(p, x);
+    e = product_pad(x, v.row, v.image, ws, tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype,
                     stream);
-    xv = padded_x(p, ws);
   }
-  if (s.pad_w && e == hipSuccess) {
+  if (s.pad_w && e == hipSuccess)
     e = product_pad(w, p.K, 0, ws + s.w, p.rows, p.rows, p.K, p.dtype, stream);
-    wv = padded_w(p, ws + s.w);
+  if (e == hipSuccess) {
+    ProductArgs g = y_args(p, s.xv, s.wv, bias, res, y);
+    g.part = (float*)(ws + s.part);
+    e = product_launch(g, p.dtype, stream);
   }
-  if (e == hipSuccess) e = product_launch(y_args(p, xv, wv, bias, res, y), p.dtype, stream);
   return api_launch(fn, e);
 }
 
@@ -509,7 +523,7 @@ PWC_API size_t pwc_linear_forward_workspace_size(const void* x, const void* weig
                                                  long long B, long long P, int K, int O,
                                                  long long x_stride, int dtype) {
   const Problem p = problem(layout, B, P, K, O, x_stride, 0, 0.f, dtype, 0);
-  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight).total;
+  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight, nullptr).total;
 }
 
 PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bias,
@@ -548,7 +562,7 @@ PWC_API size_t pwc_gated_linear_forward_workspace_size(const void* x, const void
                                                        int layout, long long B, long long P, int K,
                                                        int O, long long x_stride, int dtype) {
   const Problem p = problem(layout, B, P, K, O, x_stride, 0, 0.f, dtype, 1);
-  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight).total;
+  return bad_problem(p) || p.M == 0 ? 0 : forward_space(p, x, weight, nullptr).total;
 }
 
 PWC_API int pwc_gated_linear_forward(const void* x, const void* weight, const void* bias, void* y,

@@ -75,6 +75,15 @@ __device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
   }
 }
 
+// what rounding takes from the values; nothing where it gives an infinity or a NaN
+template <typename T, int V> __device__ __forceinline__ void rounded_off(float (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float h = to_f32(narrow<T>(v[e]));
+    v[e] = fabsf(h) < __builtin_inff() ? v[e] - h : 0.f;
+  }
+}
+
 // Sum over the `W` neighbouring lanes (a power of two) that share a row.
 template <int W> __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll

@@ -22,6 +22,7 @@ struct ProductArgs {
   void* out;
   const void* bias;   // along the channels, or NULL
   const void* other;  // residual or output gradient, or NULL; at ldother
+  float* part;        // workspace of product_part_bytes: 32-bit sums of the splits of k
   float* sums;        // k*Dz: partial sums of dz over the tokens, product_sum_rows rows, or NULL
   long long lda, ldb, ldo, ldother;
   long long a_batch, b_batch, out_batch, other_batch;
@@ -51,13 +52,14 @@ enum ProductKernel : int {
 struct ProductPlan {
   int kernel;
   int bi, bj, passes;  // the tile; column halves that the epilogue takes it in
-  int splits;        // kPartial
+  int splits;        // of k: kPartial, or summed and finished by a kernel of its own
 };
 ProductPlan product_plan(const ProductArgs& g, int dtype);
 template <typename T>
 hipError_t product_t(const ProductArgs& g, const ProductPlan& p, hipStream_t stream);
 
 hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream);
+size_t product_part_bytes(const ProductArgs& g, int dtype);
 int product_sum_rows(const ProductArgs& g, int dtype);
 int product_column_parts(int layout, long long B, long long P, int C);
 hipError_t product_column_sums(const void* dy, float* part, int layout, long long B, long long P,

@@ -86,14 +86,19 @@ static bool direct_any(const ProductArgs& g, const TileCost& c, int dtype) {
 
 ProductPlan product_plan(const ProductArgs& g, int dtype) {
   const bool pair = g.mode == kGated || g.mode == kGatedDz;
-  // A pass over W reads it once at memory speed, the tiles a block's share of it at a CU's pace.
-  // (tokens alone: their W lies along k, and a kernel of one pass has one batch)
-  if (g.channel_i && g.J <= 64)
-    return {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 16, 1, 1};
   const long long pairs = ((long long)g.pair + 15) / 16 * 32;
   const long long ri = pair && g.channel_i ? pairs : g.I, rj = pair && !g.channel_i ? pairs : g.J;
   ProductPlan best = {};
   double least = 1e300;
+  if (g.channel_i && g.J <= 64) {
+    // A pass over W: a CU takes 50 bytes of W and x a ns (64 tokens, 4096 -> 4096: 13.6 us, by
+    // tiles 16.0; 4096 -> 16384: 45, by tiles 30), and up to 32 tokens nothing is faster.
+    best = {g.J <= 16 ? kFew16 : g.J <= 32 ? kFew32 : kFew64, 16, 16, 1, 1};
+    if (g.J <= 32) return best;
+    const int blocks = ((pair ? g.pair : g.I) + 15) / 16;
+    least = 2.0 + (double)((blocks + kCUs - 1) / kCUs) * (g.J + (pair ? 32 : 16)) * g.K *
+                      (dtype == 0 ? 4 : 2) / 50e3;
+  }
   const TileCost* costs = dtype == 0 ? kCost32 : kCost16;
   for (int n = 0; n < (dtype == 0 ? 2 : 3); ++n) {
     const TileCost& c = costs[n];
@@ -103,15 +108,17 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
     const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
     const double tiles =
         (double)((ri + c.bi - 1) / c.bi) * ((rj + c.bj - 1) / c.bj) * g.batches;
-    for (int splits = 1; splits <= (g.mode == kPartial ? 512 : 1); splits *= 2) {
+    for (int splits = 1; splits <= (g.mode == kPartial || g.channel_i ? 512 : 1); splits *= 2) {
       if (splits > 1 && splits * 4 > steps) break;  // some steps each
       const double blocks = tiles * splits, each = steps / splits;
       const double rounds = blocks / (kCUs * c.blocks);
       double t = each * c.lag;
       if (t < blocks / kCUs * each * c.work) t = blocks / kCUs * each * c.work;
       t += c.fixed * (rounds < 1 ? 1 : rounds);
-      // the partial sums go out and come back, and one more launch
-      if (splits > 1) t += 4.0 + (double)g.I * g.J * splits * 8 / 6.5e6;
+      // the partial sums go out and come back, and one more launch, with the epilogue if there is
+      // one (128 tokens, 4096 -> 4096: 40 us in one part, 20 in eight)
+      if (splits > 1)
+        t += (g.mode == kPartial ? 5.5 : 6.5) + (double)g.I * g.J * splits * 8 / 6.5e6;
       if (t < least) {
         least = t;
         best = {direct ? c.kernel : kTile64Any, c.bi, c.bj, c.passes, splits};
@@ -121,11 +128,157 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
   return best;
 }
 
+// The epilogue of a product that was summed in parts: a lane takes four channels, a wave 256 of a
+// token, `each` tokens of every fourth.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void finish_parts(const ProductArgs g, int splits, int each) {
+  constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
+  constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
+  __shared__ float red[kDz ? 3 : 1][kPair ? 2 : 1][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int outs = kPair ? g.pair : g.I, i = (blockIdx.x * 64 + lane) * 4, left = outs - i;
+  auto four = [&](const auto* p, int n, float(&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 0.f;
+    if (n >= 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = to_f32(p[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < n) v[e] = to_f32(p[e]);
+    }
+  };
+  const T* bias = (const T*)g.bias;
+  float b[4], c[4], sv[4], sw[4];
+  four(bias + i, bias ? left : 0, b);
+  four(bias + g.pair + i, bias && kPair ? left : 0, c);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sv[e] = sw[e] = 0.f;
+  for (int r = 0; r < each; ++r) {
+    const int j = (blockIdx.y * each + r) * 4 + wave;
+    if (j >= g.J || left <= 0) break;
+    float v[4], w[4], d[4], t[4], o[4];
+    four((const T*)g.other + (long long)j * g.ldother + i, g.other ? left : 0, o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = b[e];
+      w[e] = c[e];
+    }
+    const float* p = g.part + (long long)j * g.I + i;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s, p += (long long)g.I * g.J) {
+      four(p, left, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += t[e];
+      if constexpr (kPair) {
+        four(p + g.pair, left, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] += t[e];
+      }
+    }
+    float f[4];
+    activate<sizeof(T) == 2, kDz>(g.act, v, f, d, g.slope);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (MODE == kLinear) {
+        v[e] = f[e] + o[e];
+      } else if constexpr (MODE == kGated) {
+        v[e] = f[e] * w[e];
+      } else if constexpr (MODE == kLinearDz) {
+        v[e] = o[e] * d[e];
+      } else {
+        v[e] = o[e] * w[e] * d[e];
+        w[e] = o[e] * f[e];
+      }
+      if (kDz && e < left) {
+        sv[e] += v[e];
+        sw[e] += w[e];
+      }
+    }
+    T* out = (T*)g.out + (long long)j * g.ldo + i;
+#pragma unroll
+    for (int n = 0; n < (kDz && sizeof(T) == 2 ? 2 : 1); ++n) {
+      if (n && !g.low) break;
+      if (n) {
+        rounded_off<T, 4>(v);
+        rounded_off<T, 4>(w);
+        out += g.low;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) {
+          out[e] = narrow<T>(v[e]);
+          if (MODE == kGatedDz) out[g.pair + e] = narrow<T>(w[e]);
+        }
+    }
+  }
+  if constexpr (kDz) {
+    if (!g.sums) return;
+    if (wave)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        red[wave - 1][0][lane * 4 + e] = sv[e];
+        if (kPair) red[wave - 1][kPair][lane * 4 + e] = sw[e];
+      }
+    __syncthreads();
+    if (wave) return;
+    float* sums = g.sums + (long long)blockIdx.y * g.I + i;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= left) break;
+      sums[e] = sv[e] + red[0][0][lane * 4 + e] + red[1][0][lane * 4 + e] + red[2][0][lane * 4 + e];
+      if (kPair)
+        sums[g.pair + e] = sw[e] + red[0][kPair][lane * 4 + e] + red[1][kPair][lane * 4 + e] +
+                           red[2][kPair][lane * 4 + e];
+    }
+  }
+}
+// some blocks a CU where there are that many tokens
+static int finish_each(const ProductArgs& g) {
+  const int outs = g.mode == kGated || g.mode == kGatedDz ? g.pair : g.I;
+  const long long blocks = (outs + 255LL) / 256 * ((g.J + 3) / 4);
+  return (int)((blocks + 2047) / 2048);
+}
+static int finish_rows(const ProductArgs& g) {
+  const int each = finish_each(g) * 4;
+  return (g.J + each - 1) / each;
+}
+template <typename T>
+static hipError_t finish_t(const ProductArgs& g, int splits, hipStream_t stream) {
+  const int outs = g.mode == kGated || g.mode == kGatedDz ? g.pair : g.I;
+  const dim3 grid((outs + 255) / 256, finish_rows(g));
+  const int each = finish_each(g);
+#define FINISH(MODE) finish_parts<T, MODE><<<grid, 256, 0, stream>>>(g, splits, each)
+  switch (g.mode) {
+    case kLinear: FINISH(kLinear); break;
+    case kLinearDz: FINISH(kLinearDz); break;
+    case kGated: FINISH(kGated); break;
+    case kGatedDz: FINISH(kGatedDz); break;
+    default: return hipErrorInvalidValue;
+  }
+#undef FINISH
+  return hipGetLastError();
+}
+template <typename T>
+static hipError_t launch_t(const ProductArgs& g, const ProductPlan& p, hipStream_t stream) {
+  if (g.mode == kPartial || p.splits == 1) return product_t<T>(g, p, stream);
+  ProductArgs parts = g;
+  parts.mode = kPartial;
+  parts.out = g.part;
+  parts.splits = p.splits;
+  const hipError_t e = product_t<T>(parts, p, stream);
+  return e == hipSuccess ? finish_t<T>(g, p.splits, stream) : e;
+}
 hipError_t product_launch(const ProductArgs& g, int dtype, hipStream_t stream) {
   const ProductPlan p = product_plan(g, dtype);
-  return dtype == 0   ? product_t<float>(g, p, stream)
-         : dtype == 1 ? product_t<__half>(g, p, stream)
-                      : product_t<__hip_bfloat16>(g, p, stream);
+  return dtype == 0   ? launch_t<float>(g, p, stream)
+         : dtype == 1 ? launch_t<__half>(g, p, stream)
+                      : launch_t<__hip_bfloat16>(g, p, stream);
+}
+size_t product_part_bytes(const ProductArgs& g, int dtype) {
+  const int splits = product_plan(g, dtype).splits;
+  return splits > 1 ? align256((size_t)splits * g.I * g.J * sizeof(float)) : 0;
 }
 
 template <typename T>
@@ -140,6 +293,7 @@ static hipError_t add_splits_t(const float* part, void* out, long long n, int sp
 // Rows of partial sums that a kLinearDz / kGatedDz launch writes.
 int product_sum_rows(const ProductArgs& g, int dtype) {
   const ProductPlan p = product_plan(g, dtype);
+  if (p.splits > 1) return finish_rows(g);
   if (p.kernel <= kFew64) return 1 << (p.kernel - kFew16);
   if (g.channel_i) return (g.J + p.bj - 1) / p.bj * 2 * p.passes;
   return (g.I + p.bi - 1) / p.bi * 2 * g.batches;

@@ -221,15 +221,6 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
   }
 };
 
-// what rounding takes from the values; nothing where it gives an infinity or a NaN
-template <typename T, int V> __device__ __forceinline__ void rounded_off(float (&v)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float h = to_f32(narrow<T>(v[e]));
-    v[e] = fabsf(h) < __builtin_inff() ? v[e] - h : 0.f;
-  }
-}
-
 // What the epilogue needs of one wave's sums: they lie in LDS as rows of i (`tile`, WI long).
 struct Finish {
   const float* tile;
@@ -695,38 +686,46 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 
 // ---- few tokens: a pass over W ----
 // At most 16 JB tokens: the time is W's bytes.  A block takes 16 FR output channels (gated: of each
-// half) and its 8 waves take an eighth of k each, straight from memory into fragments -- W is used
-// once, LDS would only delay it -- with DEPTH loads of 32 bytes a row under way; then the waves'
-// sums are added in their order.
+// half) and its 8 waves take an eighth of k each; then the waves' sums are added in their order.
+// Eight lanes read 128 bytes of a row, whole lines, a group of steps ahead of its use, and a
+// wave turns them into fragments through its own part of LDS, without a barrier: read as the
+// fragments want them, four neighbouring lanes ask for four lines, and the L1 cache gives 16 of its
+// 64 bytes a cycle (4096 -> 4096 bf16: 1 token 8.6 us, 64 tokens 22).
 constexpr int kFewWaves = 8;
 
 template <typename T, int FR, int JB, int MODE>
-__global__ __launch_bounds__(kFewWaves * 64) void few_tokens(const ProductArgs g) {
+__global__ __launch_bounds__(kFewWaves * 64, JB < 4 ? 4 : 2) void few_tokens(const ProductArgs g) {
   constexpr bool kPair = MODE == kGated || MODE == kGatedDz;
   constexpr bool kDz = MODE == kLinearDz || MODE == kGatedDz;
   constexpr int E = 16 / (int)sizeof(T), HALVES = kPair ? 2 : 1, FA = FR * HALVES;
-  constexpr int STEP = 8 * E;  // k of a step: two chunks of each of the four lane groups
-  constexpr int DEPTH = FA * JB >= 8 ? 1 : FA * JB >= 4 ? 2 : 4;
+  constexpr int STEP = 8 * E;  // k of a step: 128 bytes of a row
+  constexpr int DEPTH = FA + JB > 2 ? 1 : 2;
+  constexpr int REGION = ((FA + JB) * 2 > FA * JB ? (FA + JB) * 2 : FA * JB) * 1024;
   typedef typename Frag<T>::type frag_t;
-  __shared__ f32x4 join[kFewWaves][FA * JB][64];
+  __shared__ __attribute__((aligned(16))) char lds[kFewWaves][REGION];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4;
   const int outs = kPair ? g.pair : g.I, i0 = blockIdx.x * 16 * FR;
 
-  const T* pa[FA];
-  bool oa[FA];
+  // this lane's chunk of rows 8 n + lane / 8 of each fragment
+  const T* pa[FA][2];
+  const T* pb[JB][2];
+  bool oa[FA][2], ob[JB][2];
 #pragma unroll
-  for (int f = 0; f < FA; ++f) {
-    const int i = i0 + f / HALVES * 16 + l;
-    oa[f] = i < outs;
-    pa[f] = (const T*)g.a + ((long long)(kPair && f % 2 ? g.pair : 0) + (oa[f] ? i : 0)) * g.lda;
-  }
-  const T* pb[JB];
-  bool ob[JB];
+  for (int n = 0; n < 2; ++n) {
+    const int r = n * 8 + lane / 8, at = lane % 8 * E;
 #pragma unroll
-  for (int f = 0; f < JB; ++f) {
-    ob[f] = f * 16 + l < g.J;
-    pb[f] = (const T*)g.b + (ob[f] ? f * 16 + l : 0) * g.ldb;
+    for (int f = 0; f < FA; ++f) {
+      const int i = i0 + f / HALVES * 16 + r;
+      oa[f][n] = i < outs;
+      pa[f][n] =
+          (const T*)g.a + ((long long)(kPair && f % 2 ? g.pair : 0) + (oa[f][n] ? i : 0)) * g.lda + at;
+    }
+#pragma unroll
+    for (int f = 0; f < JB; ++f) {
+      ob[f][n] = f * 16 + r < g.J;
+      pb[f][n] = (const T*)g.b + (ob[f][n] ? f * 16 + r : 0) * g.ldb + at;
+    }
   }
   f32x4 acc[FA][JB];
 #pragma unroll
@@ -734,66 +733,107 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_tokens(const ProductArgs g
 #pragma unroll
     for (int j = 0; j < JB; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // whole steps in turns of DEPTH, then what is left of k value by value
+  struct Step {
+    u32x4 a[FA][2], b[JB][2];
+  };
   const u32x4 none = {0u, 0u, 0u, 0u};
-  auto take = [&](int k, bool whole, u32x4(&va)[FA][2], u32x4(&vb)[JB][2])
-      __attribute__((always_inline)) {
+  auto take = [&](int k, bool whole, Step& v) __attribute__((always_inline)) {
+    const int have = whole ? E : g.K - k - lane % 8 * E;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int at = k + (q * 2 + c) * E, have = whole ? E : g.K - at;
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int f = 0; f < FA; ++f) {
-        va[f][c] = none;
-        if (oa[f] && have >= E) va[f][c] = load16(pa[f] + at);
-        if (!whole && oa[f] && have > 0 && have < E) va[f][c] = load_some(pa[f] + at, have);
+        v.a[f][n] = none;
+        if (oa[f][n] && have >= E) v.a[f][n] = load16(pa[f][n] + k);
+        if (!whole && oa[f][n] && have > 0 && have < E) v.a[f][n] = load_some(pa[f][n] + k, have);
       }
 #pragma unroll
       for (int f = 0; f < JB; ++f) {
-        vb[f][c] = none;
-        if (ob[f] && have >= E) vb[f][c] = load16(pb[f] + at);
-        if (!whole && ob[f] && have > 0 && have < E) vb[f][c] = load_some(pb[f] + at, have);
+        v.b[f][n] = none;
+        if (ob[f][n] && have >= E) v.b[f][n] = load16(pb[f][n] + k);
+        if (!whole && ob[f][n] && have > 0 && have < E) v.b[f][n] = load_some(pb[f][n] + k, have);
       }
     }
   };
-  auto use = [&](u32x4(&va)[FA][2], u32x4(&vb)[JB][2]) __attribute__((always_inline)) {
+  // a fragment is 16 rows of 128 bytes, its chunks exclusive-ored with the row
+  char* const mine = lds[wave];
+  const int put = lane / 8 * 128 + ((lane % 8) ^ (lane / 8)) * 16;
+  auto use = [&](const Step& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int f = 0; f < FA; ++f) *(u32x4*)(mine + f * 2048 + n * 1024 + put) = v.a[f][n];
+#pragma unroll
+      for (int f = 0; f < JB; ++f) *(u32x4*)(mine + (FA + f) * 2048 + n * 1024 + put) = v.b[f][n];
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    frag_t a[FA][2], b[JB][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int get = l * 128 + ((c * 4 + q) ^ (l & 7)) * 16;
+#pragma unroll
+      for (int f = 0; f < FA; ++f) a[f][c] = *(const frag_t*)(mine + f * 2048 + get);
+#pragma unroll
+      for (int f = 0; f < JB; ++f) b[f][c] = *(const frag_t*)(mine + (FA + f) * 2048 + get);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int f = 0; f < FA; ++f)
 #pragma unroll
-        for (int j = 0; j < JB; ++j)
-          acc[f][j] = mma(__builtin_bit_cast(frag_t, va[f][c]), __builtin_bit_cast(frag_t, vb[j][c]),
-                          acc[f][j], T());
+        for (int j = 0; j < JB; ++j) acc[f][j] = mma(a[f][c], b[j][c], acc[f][j], T());
   };
+  // whole steps in groups of DEPTH, the next group's loads before one is used; then what is left
   const int steps = (g.K + STEP - 1) / STEP, whole = g.K / STEP;
   int s = steps * wave / kFewWaves;
   const int end = steps * (wave + 1) / kFewWaves, fast = min(end, whole);
-  for (; s + DEPTH <= fast; s += DEPTH) {
-    u32x4 va[DEPTH][FA][2], vb[DEPTH][JB][2];
+  if (s + DEPTH <= fast) {
+    Step x[DEPTH], y[DEPTH];
+    auto group = [&](Step(&v)[DEPTH], int at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) take((s + d) * STEP, true, va[d], vb[d]);
+      for (int d = 0; d < DEPTH; ++d) take((at + d) * STEP, true, v[d]);
+    };
+    auto spend = [&](const Step(&v)[DEPTH]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) use(va[d], vb[d]);
+      for (int d = 0; d < DEPTH; ++d) use(v[d]);
+      s += DEPTH;
+    };
+    group(x, s);
+    for (;;) {
+      const bool more = s + 2 * DEPTH <= fast;
+      if (more) group(y, s + DEPTH);
+      spend(x);
+      if (!more) break;
+      const bool again = s + 2 * DEPTH <= fast;
+      if (again) group(x, s + DEPTH);
+      spend(y);
+      if (!again) break;
+    }
   }
   for (; s < end; ++s) {
-    u32x4 va[FA][2], vb[JB][2];
-    take(s * STEP, false, va, vb);
-    use(va, vb);
+    Step x;
+    take(s * STEP, false, x);
+    use(x);
   }
 
+  f32x4(*join)[REGION / 16] = (f32x4(*)[REGION / 16])lds;
 #pragma unroll
   for (int f = 0; f < FA; ++f)
 #pragma unroll
-    for (int j = 0; j < JB; ++j) join[wave][f * JB + j][lane] = acc[f][j];
+    for (int j = 0; j < JB; ++j) join[wave][(f * JB + j) * 64 + lane] = acc[f][j];
   __syncthreads();
   // one wave a fragment; lane (l, q) holds token 16 fj + l, channels 16 fi + 4 q + 0..3
   for (int u = wave; u < FR * JB; u += kFewWaves) {
     const int fi = u / JB, fj = u % JB, j = fj * 16 + l, i = i0 + fi * 16 + q * 4;
-    f32x4 a = join[0][fi * HALVES * JB + fj][lane], b = a;
-    for (int w = 1; w < kFewWaves; ++w) a += join[w][fi * HALVES * JB + fj][lane];
+    const int at = (fi * HALVES * JB + fj) * 64 + lane;
+    f32x4 a = join[0][at], b = a;
+    for (int w = 1; w < kFewWaves; ++w) a += join[w][at];
     if (kPair) {
-      b = join[0][(fi * 2 + 1) * JB + fj][lane];
-      for (int w = 1; w < kFewWaves; ++w) b += join[w][(fi * 2 + 1) * JB + fj][lane];
+      b = join[0][at + JB * 64];
+      for (int w = 1; w < kFewWaves; ++w) b += join[w][at + JB * 64];
     }
     const T* bias = (const T*)g.bias;
     const T* other = (const T*)g.other + (long long)j * g.ldother;

@@ -270,6 +270,16 @@ def test_small_gradients_beyond_the_type():
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tokens", [33, 48, 64, 100, 255, 513])
+def test_some_tokens(tokens, dtype):
+    """Too few tokens to fill the card: long rows are summed in parts, whatever follows."""
+    for K, O, gated, act in ((2048, 520, False, "gelu"), (1536, 200, True, "silu"),
+                             (2055, 67, False, "none"), (1032, 51, True, "gelu_tanh")):
+        case = _product_case(False, (tokens,), K, O, dtype, act, True, not gated, gated)
+        _check_product(*case, act, gated, -1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_few_tokens_long_gradients(dtype):
     """dx of few tokens over many output channels is summed in parts."""
     for tokens, K, O, gated in ((1, 264, 2100, False), (7, 96, 1500, True), (64, 65, 1031, False),
