@@ -101,14 +101,14 @@ constexpr double kKeepLow = 5e8;  // operations of a product whose dz is kept in
 // on (us, as they lie / laid out first; 16 bits: 2047 x 1023 -> 1023, 4.3 GFLOP: 19 / 25;
 // 8191 x 1023 -> 4095: 164 / 103).  Backward the three products share the copies, and rows of odd
 // 16-bit lengths that are read across k cost most (act'; 1001 x 511 -> 511: 56 / 38, 2047 x 1023 ->
-// 1023: 137 / 65; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 60; fp32 2001 x 701 -> 1001: 160 / 131),
+// 1023: 137 / 65, 301 x 511 -> 511 without one 43 / 29; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 60; fp32 2001 x 701 -> 1001: 160 / 131),
 // unless so few channels meet that the products are all traffic anyway (map 16 x 64 x 113 x 129 ->
 // 64: 81 / 88, fp32 136 / 155).
 bool pads_pay(const Problem& p, bool backward) {
   const double operations = 2.0 * (double)p.M * p.rows * p.K;
   if (!backward) return operations >= 8e9;
   if (p.K < 96 || p.rows < 96) return operations >= 8e9;
-  return operations > (tokens(p) && p.dtype != 0 ? kKeepLow : 1e9);
+  return operations > (tokens(p) && p.dtype != 0 ? 1e8 : 1e9);
 }
 long long whole(const Problem& p, long long cols) {
   const long long e = 16 / (long long)elem(p.dtype);
@@ -242,9 +242,9 @@ ForwardSpace forward_space(const Problem& p, const void* x, const void* w, const
 
 struct BackwardSpace {
   bool pad_x, pad_w, pad_dz;
-  size_t x, w, part, sums, total;  // dz, or the padded dy, lies at 0
+  size_t x, w, part, part_bytes, sums, total;  // dz, or the padded dy, lies at 0
   int dx_splits, splits, rows;     // rows: of partial bias gradients
-  long long low;                   // from dz to what its rounding took (maps: image by image), or 0
+  long long dz_rows, low;          // low: from dz to what its rounding took (maps: image by image), or 0
   View xv, wv, dzv;                // as the products take them
 };
 BackwardSpace backward_space(const Problem& p, const void* x, const void* w, const void* dy,
@@ -255,25 +255,29 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   s.pad_x = pay && (z || dw) && !lies_well(p, s.xv, x_cols(p));
   s.pad_w = pay && (z || dx) && !lies_well(p, s.wv, p.K);
   s.pad_dz = pay && (z || dx || dw) && !lies_well(p, s.dzv, dz_cols(p));
+  // (where the copies lie comes below; that they are copies decides the kernels)
+  if (s.pad_x) s.xv = padded_x(p, nullptr);
+  if (s.pad_w) s.wv = padded_w(p, nullptr);
   const ProductPlan dz_plan =
       z ? product_plan(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype) : ProductPlan();
   // dz in 16 bits is rounded once, which makes the gradients' error 1.4 times that of their own
   // rounding; in small calls, where chance adds to that, what the rounding took follows as more k,
   // at a cost that the launches hide.  (Only the kernels of such calls can write it.)
-  if (z && !s.pad_dz && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
+  if (z && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
       (dz_plan.kernel <= kTile64Any || dz_plan.splits > 1))
-    s.low = tokens(p) ? p.M * p.rows : p.rows * p.P;
+    s.low = (tokens(p) ? p.M : p.rows) * (s.pad_dz ? whole(p, dz_cols(p)) : dz_cols(p));
+  s.dz_rows = dz_rows(p) * (s.low ? 2 : 1);
   size_t at = 0;
   if (s.pad_dz)
-    at += bytes_of(p, dz_rows(p), dz_cols(p));
+    at += bytes_of(p, s.dz_rows, dz_cols(p));
   else if (z)
-    at += align256((size_t)p.M * p.rows * elem(p.dtype) * (s.low ? 2 : 1));
+    at += align256((size_t)s.dz_rows * dz_cols(p) * elem(p.dtype));
   s.x = at;
   if (s.pad_x) at += bytes_of(p, x_rows(p), x_cols(p));
   s.w = at;
   if (s.pad_w) at += bytes_of(p, p.rows, p.K);
-  if (s.pad_x) s.xv = padded_x(p, ws + s.x);
-  if (s.pad_w) s.wv = padded_w(p, ws + s.w);
+  if (s.pad_x) s.xv.at = ws + s.x;
+  if (s.pad_w) s.wv.at = ws + s.w;
   if (s.pad_dz)
     s.dzv = padded_dz(p, ws);
   else if (z)
@@ -290,7 +294,8 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   parts(dz_plan.splits, p.M * p.rows);
   parts(s.dx_splits, p.M * p.K);
   parts(s.splits, (long long)p.rows * p.K);
-  at += align256(most * sizeof(float));
+  s.part_bytes = align256(most * sizeof(float));
+  at += s.part_bytes;
   s.sums = at;
   if (db) {
     s.rows = z ? product_sum_rows(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype)
@@ -328,9 +333,10 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
     g.sums = db ? (float*)(ws + s.sums) : nullptr;
     g.low = s.low;
     g.part = (float*)(ws + s.part);
+    g.part_bytes = s.part_bytes;
     e = product_launch(g, p.dtype, stream);
     if (s.pad_dz && e == hipSuccess)
-      e = product_zero_tails(ws, dz_rows(p), dz_cols(p), p.dtype, stream);
+      e = product_zero_tails(ws, s.dz_rows, dz_cols(p), p.dtype, stream);
   } else if (e == hipSuccess && s.pad_dz) {
     const View v = dz_view(p, dy);
     e = product_pad(dy, v.row, v.image, ws, tokens(p) ? p.M : p.rows, dz_rows(p), dz_cols(p),
@@ -339,6 +345,7 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
   if (dx && e == hipSuccess) {
     ProductArgs g = dx_args(p, s.dzv, s.low, s.wv, s.dx_splits > 1 ? (void*)(ws + s.part) : dx);
     g.splits = s.dx_splits;
+    g.part_bytes = s.part_bytes;
     e = product_launch(g, p.dtype, stream);
     if (e == hipSuccess && s.dx_splits > 1)
       e = product_add_splits((const float*)(ws + s.part), dx, p.M * p.K, s.dx_splits, p.dtype,
@@ -347,6 +354,7 @@ int product_backward(const char* fn, const Problem& p, const void* x, const void
   if (dw && e == hipSuccess) {
     ProductArgs g = dw_args(p, s.xv, s.dzv, s.low, s.splits > 1 ? (void*)(ws + s.part) : dw);
     g.splits = s.splits;
+    g.part_bytes = s.part_bytes;
     e = product_launch(g, p.dtype, stream);
     if (e == hipSuccess && s.splits > 1)
       e = product_add_splits((const float*)(ws + s.part), dw, (long long)p.rows * p.K, s.splits,
@@ -382,6 +390,7 @@ int product_forward(const char* fn, const Problem& p, const void* x, const void*
   if (e == hipSuccess) {
     ProductArgs g = y_args(p, s.xv, s.wv, bias, res, y);
     g.part = (float*)(ws + s.part);
+    g.part_bytes = s.total - s.part;
     e = product_launch(g, p.dtype, stream);
   }
   return api_launch(fn, e);

@@ -22,7 +22,8 @@ struct ProductArgs {
   void* out;
   const void* bias;   // along the channels, or NULL
   const void* other;  // residual or output gradient, or NULL; at ldother
-  float* part;        // workspace of product_part_bytes: 32-bit sums of the splits of k
+  float* part;        // workspace for 32-bit sums of the splits of k (kPartial's are its output)
+  size_t part_bytes;  // its size, or kPartial's output's
   float* sums;        // k*Dz: partial sums of dz over the tokens, product_sum_rows rows, or NULL
   long long lda, ldb, ldo, ldother;
   long long a_batch, b_batch, out_batch, other_batch;
@@ -45,6 +46,7 @@ enum ProductKernel : int {
   kFew32,
   kFew64,
   kTile64,
+  kTile64Deep,  // three steps in LDS
   kTile64Any,
   kTile128,
   kTile256,

@@ -62,21 +62,29 @@ template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int
 }
 
 // Which kernel: the one with the least modelled time.  A step of 128 bytes of k costs a block at
-// least `lag` (loads, barrier, latency), and the blocks of a CU share its matrix units, `work` a
-// block; a tile's epilogue and start cost `fixed` for every round of tiles over the card.  The
-// figures are measured (us; bf16: 8192 x K -> 4096 and 64 x 4096 -> 4096 tokens; fp32: 4096 x 1024
-// -> 1024 and 1000 x 1000 -> 1000): 256-tiles do 1520 TFLOP/s where there are enough of them, 128
-// are the best for some hundred, 64 for less.
+// least `far` (loads, barrier, latency; `near` where both operands stay in the L2 caches), and the
+// blocks of a CU share its matrix units, `work` a block; a tile's epilogue and start cost `fixed`
+// for every round of tiles over the card.  The figures are fitted to measured calls (us, bf16, by
+// 64-, deep 64-, 128- and 256-tiles: 512 tokens 4096 -> 4096 36, 28, 33, 43; 1024 tokens 51, 53, 47,
+// 53; 8192 tokens 4096 -> 1024 95, 98, 66, 76; 1024 -> 4096 111, 115, 83, 73; 128 -> 1024 12, 13,
+// 10, 18; fp32 4096 tokens 1024 -> 1024 by 64- and 128-tiles 73, 75; 8192 1024 -> 4096 520, 513).
 struct TileCost {
   int kernel, bi, bj, passes, blocks;  // blocks that a CU holds
-  double lag, work, fixed;
+  double far, near, work, fixed;
 };
-static constexpr TileCost kCost16[] = {{kTile64, 64, 64, 1, 4, 0.56, 0.20, 3.3},
-                                       {kTile128, 128, 128, 1, 2, 0.85, 0.57, 6.5},
-                                       {kTile256, 256, 256, 2, 1, 1.60, 1.65, 16.0}};
-static constexpr TileCost kCost32[] = {{kTile64, 64, 64, 1, 4, 0.65, 0.53, 4.0},
-                                       {kTile128, 128, 128, 1, 2, 2.00, 2.00, 8.0}};
+static constexpr TileCost kCost16[] = {{kTile64, 64, 64, 1, 4, 0.50, 0.20, 0.175, 3.5},
+                                       {kTile64Deep, 64, 64, 1, 3, 0.35, 0.20, 0.19, 3.5},
+                                       {kTile128, 128, 128, 1, 2, 0.66, 0.46, 0.47, 4.4},
+                                       {kTile256, 256, 256, 2, 1, 1.39, 1.39, 1.39, 14.0}};
+// Through registers, both operands along k or not (rows at odd places that are read across k cost
+// most; bf16, 1024 x 1021 -> 1021: forward 15, in four parts 23; dx 27, in four parts 20).
+static constexpr TileCost kCostAnyK16 = {kTile64Any, 64, 64, 1, 4, 0.60, 0.60, 0.21, 3.5};
+static constexpr TileCost kCostAnyK32 = {kTile64Any, 64, 64, 1, 4, 1.00, 1.00, 0.55, 3.5};
+static constexpr TileCost kCostAny = {kTile64Any, 64, 64, 1, 4, 1.35, 1.35, 0.60, 3.5};
+static constexpr TileCost kCost32[] = {{kTile64, 64, 64, 1, 4, 0.65, 0.60, 0.53, 3.0},
+                                       {kTile128, 128, 128, 1, 2, 2.00, 2.00, 1.96, 6.0}};
 constexpr int kCUs = 256;
+constexpr double kNear = 8e6;  // bytes of both operands
 
 static bool direct_any(const ProductArgs& g, const TileCost& c, int dtype) {
   return dtype == 0   ? direct_loads<float>(g, c.bi, c.bj)
@@ -88,6 +96,7 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
   const bool pair = g.mode == kGated || g.mode == kGatedDz;
   const long long pairs = ((long long)g.pair + 15) / 16 * 32;
   const long long ri = pair && g.channel_i ? pairs : g.I, rj = pair && !g.channel_i ? pairs : g.J;
+  const double bytes = dtype == 0 ? 4.0 : 2.0;  // bytes of a value
   ProductPlan best = {};
   double least = 1e300;
   if (g.channel_i && g.J <= 64) {
@@ -97,13 +106,17 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
     if (g.J <= 32) return best;
     const int blocks = ((pair ? g.pair : g.I) + 15) / 16;
     least = 2.0 + (double)((blocks + kCUs - 1) / kCUs) * (g.J + (pair ? 32 : 16)) * g.K *
-                      (dtype == 0 ? 4 : 2) / 50e3;
+                      bytes / 50e3;
   }
   const TileCost* costs = dtype == 0 ? kCost32 : kCost16;
-  for (int n = 0; n < (dtype == 0 ? 2 : 3); ++n) {
-    const TileCost& c = costs[n];
-    const bool direct = direct_any(g, c, dtype);
-    if (!direct && n > 0) break;  // through registers: the small tile alone
+  const bool near = ((double)g.I + g.J) * g.K * g.segments * g.batches * bytes <= kNear;
+  for (int n = 0; n < (dtype == 0 ? 2 : 4); ++n) {
+    const bool direct = direct_any(g, costs[n], dtype);
+    if (!direct && n > 0) break;
+    const TileCost& c = direct               ? costs[n]
+                        : !(g.a_k && g.b_k) ? kCostAny
+                        : dtype == 0        ? kCostAnyK32
+                                            : kCostAnyK16;
     const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
     const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
     const double tiles =
@@ -112,16 +125,15 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
       if (splits > 1 && splits * 4 > steps) break;  // some steps each
       const double blocks = tiles * splits, each = steps / splits;
       const double rounds = blocks / (kCUs * c.blocks);
-      double t = each * c.lag;
+      double t = each * (near ? c.near : c.far);
       if (t < blocks / kCUs * each * c.work) t = blocks / kCUs * each * c.work;
-      t += c.fixed * (rounds < 1 ? 1 : rounds);
+      t += 2.0 + c.fixed * (rounds < 1 ? 1 : rounds);
       // the partial sums go out and come back, and one more launch, with the epilogue if there is
       // one (128 tokens, 4096 -> 4096: 40 us in one part, 20 in eight)
-      if (splits > 1)
-        t += (g.mode == kPartial ? 5.5 : 6.5) + (double)g.I * g.J * splits * 8 / 6.5e6;
+      if (splits > 1) t += 5.5 + (double)g.I * g.J * splits * 8 / (direct ? 6.5e6 : 3.2e6);
       if (t < least) {
         least = t;
-        best = {direct ? c.kernel : kTile64Any, c.bi, c.bj, c.passes, splits};
+        best = {c.kernel, c.bi, c.bj, c.passes, splits};
       }
     }
   }
@@ -262,7 +274,10 @@ static hipError_t finish_t(const ProductArgs& g, int splits, hipStream_t stream)
 }
 template <typename T>
 static hipError_t launch_t(const ProductArgs& g, const ProductPlan& p, hipStream_t stream) {
-  if (g.mode == kPartial || p.splits == 1) return product_t<T>(g, p, stream);
+  const int splits = g.mode == kPartial ? g.splits : p.splits;
+  if (splits > 1 && (size_t)splits * g.I * g.J * sizeof(float) > g.part_bytes)
+    return hipErrorInvalidValue;  // not the workspace of this plan
+  if (g.mode == kPartial || splits == 1) return product_t<T>(g, p, stream);
   ProductArgs parts = g;
   parts.mode = kPartial;
   parts.out = g.part;

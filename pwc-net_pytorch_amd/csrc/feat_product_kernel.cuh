@@ -464,8 +464,8 @@ __device__ __forceinline__ void finish_tile(const ProductArgs& g, const float* t
   }
 }
 
-template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
-          bool DIRECT>
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, int STAGES, bool AKC, bool BKC,
+          int MODE, bool DIRECT>
 __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
     void product(const ProductArgs g) {
   constexpr int NW = NWI * NWJ;
@@ -476,10 +476,12 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   typedef Tile<T, BI, AKC, NW> TA;
   typedef Tile<T, BJ, BKC, NW> TB;
   typedef typename Frag<T>::type frag_t;
-  // Two buffers as four variables: the compiler then sees that a read of one does not have to wait
-  // for the direct loads that are under way into another.
+  // Each buffer is a variable: the compiler then sees that a read of one does not have to wait for
+  // the direct loads that are under way into another.
+  static_assert(STAGES >= 2 && STAGES <= 3 && (DIRECT || STAGES == 2), "stages");
+  constexpr int A2 = STAGES > 2 ? TA::BYTES : 16, B2 = STAGES > 2 ? TB::BYTES : 16;
   __shared__ __attribute__((aligned(16))) char a0[TA::BYTES], b0[TB::BYTES], a1[TA::BYTES],
-      b1[TB::BYTES];
+      b1[TB::BYTES], a2[A2], b2[B2];
   __shared__ float row_sums[NW][WJ];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -524,6 +526,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
       ++seg;
     }
   };
+  constexpr int LOADS = TA::LOADS + TB::LOADS;  // of a step
   auto start = [&](char* pa, char* pb) __attribute__((always_inline)) {
     aim();
 #pragma unroll
@@ -531,11 +534,13 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 #pragma unroll
     for (int n = 0; n < TB::LOADS; ++n) lb.load(pb, n);
   };
-  // the started loads are in LDS, and this wave's reads so far are done
-  auto settle = [&](char* pa, char* pb) __attribute__((always_inline)) {
+  // the loads into these are in LDS, `behind` steps' loads may be under way, and this wave's reads
+  // so far are done
+  auto settle = [&](char* pa, char* pb, auto behind) __attribute__((always_inline)) {
     la.finish(pa);
     lb.finish(pb);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(DIRECT ? decltype(behind)::value * LOADS : 0)
+                 : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
@@ -548,9 +553,9 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 
   // Two fragment sets: while one is multiplied the other is read.  A step has two halves of k:
   //   multiply half 0, reading half 1 | wait for the next step's loads, barrier |
-  //   multiply half 1, reading half 0 of the next step and starting the loads of the step after it
+  //   multiply half 1, reading half 0 of the next step and starting the loads of the step STAGES on
   //   into the buffer that all waves have read
-  // so the loads have a whole step, the reads half a step, and one barrier a step is enough.  Where
+  // so the loads have STAGES - 1 steps, the reads half a step, and one barrier a step is enough.  Where
   // one wave a SIMD has to feed the matrix unit alone, reads and loads stand between its
   // instructions, a row of fragments at a time: issued in one go they fill the queues and it waits
   // behind them (8192 x K -> 4096 tokens: 1430 -> 1520 TFLOP/s).  With two waves a SIMD one
@@ -562,7 +567,7 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 #pragma unroll
     for (int i = 0; i < FI; ++i) fa[kk][i] = TA::frag(pa, wi + i * 16, kk);
   };
-  // half kk is multiplied, half 1 - kk is read from (pa, pb); LOAD: the next loads into (qa, qb)
+  // half kk is multiplied, half 1 - kk is read from (pa, pb); LOAD: loads start into (qa, qb)
   auto half = [&](int kk, const char* pa, const char* pb, auto load, char* qa, char* qb)
       __attribute__((always_inline)) {
     constexpr bool LOAD = decltype(load)::value;
@@ -597,11 +602,11 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
       }
     }
   };
-  auto step = [&](char* ca, char* cb, char* na, char* nb) __attribute__((always_inline)) {
-    half(0, ca, cb, std::false_type(), nullptr, nullptr);
-    settle(na, nb);
+  auto step = [&](char* pa, char* pb, char* qa, char* qb) __attribute__((always_inline)) {
+    half(0, pa, pb, std::false_type(), nullptr, nullptr);
+    settle(qa, qb, std::integral_constant<int, STAGES - 2>());
     __builtin_amdgcn_sched_barrier(0);
-    half(1, na, nb, std::true_type(), ca, cb);
+    half(1, qa, qb, std::true_type(), pa, pb);
   };
   // (the sums stand in their registers before the wait, and are taken from them behind the next)
   auto pin = [&]() __attribute__((always_inline)) {
@@ -617,31 +622,44 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   }
   start(a0, b0);
   if constexpr (DIRECT) {
-    // the second step's loads follow at once; the first is there when only they are under way
+    // the next steps' loads follow at once; the first is there when only they are under way
     start(a1, b1);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TA::LOADS + TB::LOADS) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    if constexpr (STAGES > 2) start(a2, b2);
+    settle(a0, b0, std::integral_constant<int, STAGES - 1>());
     read(a0, b0, 0);
   } else {
-    settle(a0, b0);
+    settle(a0, b0, std::integral_constant<int, 0>());
     read(a0, b0, 0);
     start(a1, b1);
   }
+  // the steps of all buffers, or of the first `left`
+  auto round = [&](int left) __attribute__((always_inline)) {
+    step(a0, b0, a1, b1);
+    if constexpr (STAGES == 2) {
+      if (left > 1) step(a1, b1, a0, b0);
+    } else {
+      if (left > 1) step(a1, b1, a2, b2);
+      if (left > 2) step(a2, b2, a0, b0);
+    }
+  };
   if constexpr (kPinned) {
     // (a step past the end multiplies zeros)
-    for (; s < end; s += 2) {
-      step(a0, b0, a1, b1);
-      step(a1, b1, a0, b0);
-    }
+    for (; s < end; s += STAGES) round(STAGES);
+  } else if constexpr (DIRECT) {
+    // (written out: with exchanged pointers a read waits for the loads into the other buffers too)
+    for (; s + STAGES <= end; s += STAGES) round(STAGES);
+    if (s < end) round(end - s);
   } else {
-    // (written out: with exchanged pointers a read waits for all loads, those into the other buffer
-    // too; 1024 x 4096 -> 4096 took 55 us)
-    for (; s + 2 <= end; s += 2) {
-      step(a0, b0, a1, b1);
-      step(a1, b1, a0, b0);
+    char *pa = a0, *pb = b0, *qa = a1, *qb = b1;
+    for (; s < end; ++s) {
+      step(pa, pb, qa, qb);
+      char* t = pa;
+      pa = qa;
+      qa = t;
+      t = pb;
+      pb = qb;
+      qb = t;
     }
-    if (s < end) step(a0, b0, a1, b1);
   }
   // the last matrix instructions, 8 passes of 4 cycles, before their sums are read
   if constexpr (kPinned) {
@@ -908,8 +926,8 @@ static hipError_t launch_few(const ProductArgs& g, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool AKC, bool BKC, int MODE,
-          bool DIRECT>
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, int STAGES, bool AKC, bool BKC,
+          int MODE, bool DIRECT>
 static hipError_t launch(ProductArgs g, hipStream_t stream) {
   constexpr bool kPair = MODE == kGated || MODE == kGatedDz, CI = AKC && BKC;
   const long long pairs = (g.pair + 15) / 16 * 32;
@@ -918,16 +936,16 @@ static hipError_t launch(ProductArgs g, hipStream_t stream) {
   const long long blocks =
       (long long)g.tiles_i * g.tiles_j * (g.mode == kPartial ? g.splits : g.batches);
   if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-  product<T, BI, BJ, NWI, NWJ, PASSES, AKC, BKC, MODE, DIRECT>
+  product<T, BI, BJ, NWI, NWJ, PASSES, STAGES, AKC, BKC, MODE, DIRECT>
       <<<grid_of(blocks), NWI * NWJ * 64, 0, stream>>>(g);
   return hipGetLastError();
 }
 
 // the combinations of operands and epilogues that the calls use
-template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, bool DIRECT>
+template <typename T, int BI, int BJ, int NWI, int NWJ, int PASSES, int STAGES, bool DIRECT>
 static hipError_t by_operands(const ProductArgs& g, hipStream_t stream) {
 #define PRODUCT(AKC, BKC, MODE) \
-  return launch<T, BI, BJ, NWI, NWJ, PASSES, AKC, BKC, MODE, DIRECT>(g, stream)
+  return launch<T, BI, BJ, NWI, NWJ, PASSES, STAGES, AKC, BKC, MODE, DIRECT>(g, stream)
   if (g.a_k && g.b_k) switch (g.mode) {
       case kLinear: PRODUCT(true, true, kLinear);
       case kLinearDz: PRODUCT(true, true, kLinearDz);
@@ -956,11 +974,14 @@ hipError_t product_t(const ProductArgs& g, const ProductPlan& p, hipStream_t str
     case kFew16: return launch_few<T, 1, 1>(g, stream);
     case kFew32: return launch_few<T, 1, 2>(g, stream);
     case kFew64: return launch_few<T, 1, 4>(g, stream);
-    case kTile64: return by_operands<T, 64, 64, 2, 2, 1, true>(g, stream);
-    case kTile64Any: return by_operands<T, 64, 64, 2, 2, 1, false>(g, stream);
-    case kTile128: return by_operands<T, 128, 128, 2, 2, 1, true>(g, stream);
+    case kTile64: return by_operands<T, 64, 64, 2, 2, 1, 2, true>(g, stream);
+    case kTile64Deep:
+      if constexpr (sizeof(T) == 2) return by_operands<T, 64, 64, 2, 2, 1, 3, true>(g, stream);
+      break;
+    case kTile64Any: return by_operands<T, 64, 64, 2, 2, 1, 2, false>(g, stream);
+    case kTile128: return by_operands<T, 128, 128, 2, 2, 1, 2, true>(g, stream);
     case kTile256:
-      if constexpr (sizeof(T) == 2) return by_operands<T, 256, 256, 2, 2, 2, true>(g, stream);
+      if constexpr (sizeof(T) == 2) return by_operands<T, 256, 256, 2, 2, 2, 2, true>(g, stream);
   }
   return hipErrorInvalidValue;
 }

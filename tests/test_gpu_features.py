@@ -239,7 +239,8 @@ def test_few_tokens(tokens, dtype):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("is_map,dims,K,O,gated", [
     (False, (1,), 512, 96, False), (False, (7,), 264, 130, True), (False, (40,), 1000, 65, True),
-    (False, (3440,), 176, 8, True), (False, (777,), 65, 33, False), (True, (7, 3, 2), 1, 40, False),
+    (False, (3440,), 176, 8, True), (False, (777,), 65, 33, False), (False, (301,), 511, 509, False),
+    (False, (150,), 773, 257, True), (True, (7, 3, 2), 1, 40, False),
     (True, (3, 24, 28), 32, 48, True), (True, (2, 37, 53), 33, 17, True)])
 def test_small_gradients_keep_their_bits(is_map, dims, K, O, gated, dtype):
     """In small 16-bit calls dz is kept in two parts, u^2 off instead of u (the second part of a
@@ -274,7 +275,8 @@ def test_small_gradients_beyond_the_type():
 def test_some_tokens(tokens, dtype):
     """Too few tokens to fill the card: long rows are summed in parts, whatever follows."""
     for K, O, gated, act in ((2048, 520, False, "gelu"), (1536, 200, True, "silu"),
-                             (2055, 67, False, "none"), (1032, 51, True, "gelu_tanh")):
+                             (2055, 67, False, "none"), (1032, 51, True, "gelu_tanh"),
+                             (2053, 1021, False, "silu"), (1029, 2047, True, "silu")):
         case = _product_case(False, (tokens,), K, O, dtype, act, True, not gated, gated)
         _check_product(*case, act, gated, -1)
 
