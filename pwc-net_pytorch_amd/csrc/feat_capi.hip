@@ -242,7 +242,7 @@ ForwardSpace forward_space(const Problem& p, const void* x, const void* w, const
 
 struct BackwardSpace {
   bool pad_x, pad_w, pad_dz;
-  size_t x, w, part, part_bytes, sums, total;  // dz, or the padded dy, lies at 0
+  size_t x, w, part, part_bytes, dw_part, dw_part_bytes, sums, total;  // dz, or the padded dy, lies at 0
   int dx_splits, splits, rows;     // rows: of partial bias gradients
   long long dz_rows, low;          // low: from dz to what its rounding took (maps: image by image), or 0
   View xv, wv, dzv;                // as the products take them
@@ -285,17 +285,17 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   if (s.low && !tokens(p)) s.dzv.image *= 2;
   s.dx_splits = dx ? product_plan(dx_args(p, s.dzv, s.low, s.wv, nullptr), p.dtype).splits : 1;
   s.splits = dw ? product_plan(dw_args(p, s.xv, s.dzv, s.low, nullptr), p.dtype).splits : 1;
-  // (the parts of each product are added before the next one's are written)
-  s.part = at;
-  size_t most = 0;
-  auto parts = [&](int splits, long long values) {
-    if (splits > 1 && most < (size_t)splits * values) most = (size_t)splits * values;
+  // (dz's parts are done with before dx's are written)
+  auto parts = [](int splits, long long values) {
+    return splits > 1 ? align256((size_t)splits * values * sizeof(float)) : 0;
   };
-  parts(dz_plan.splits, p.M * p.rows);
-  parts(s.dx_splits, p.M * p.K);
-  parts(s.splits, (long long)p.rows * p.K);
-  s.part_bytes = align256(most * sizeof(float));
-  at += s.part_bytes;
+  const size_t dz_part = parts(dz_plan.splits, p.M * p.rows);
+  s.part = at;
+  s.part_bytes = parts(s.dx_splits, p.M * p.K);
+  if (s.part_bytes < dz_part) s.part_bytes = dz_part;
+  s.dw_part = at += s.part_bytes;
+  s.dw_part_bytes = parts(s.splits, (long long)p.rows * p.K);
+  at += s.dw_part_bytes;
   s.sums = at;
   if (db) {
     s.rows = z ? product_sum_rows(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype)
@@ -306,66 +306,77 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   return s;
 }
 
+LayJob lay_x(const Problem& p, const void* x, bool pad, void* to) {
+  if (!pad) return {};
+  const View v = x_view(p, x);
+  return {v.at, to, v.row, v.image, tokens(p) ? p.M : p.K, x_rows(p), x_cols(p)};
+}
+LayJob lay_w(const Problem& p, const void* w, bool pad, void* to) {
+  if (!pad) return {};
+  return {w, to, p.K, 0, p.rows, p.rows, p.K};
+}
+// dy as dz, or nothing but the zeros behind a computed one
+LayJob lay_dz(const Problem& p, bool computed, const void* dy, const BackwardSpace& s, void* to) {
+  if (!s.pad_dz) return {};
+  const View v = dz_view(p, dy);
+  return {computed ? nullptr : v.at, to,       v.row, v.image, tokens(p) ? p.M : p.rows,
+          s.dz_rows,                 dz_cols(p)};
+}
+
 int product_backward(const char* fn, const Problem& p, const void* x, const void* w,
                      const void* bias, const void* dy, void* dx, void* dw, void* db,
                      void* workspace, size_t bytes, hipStream_t stream) {
   if (const char* e = bad_problem(p)) return api_fail(fn, e);
-  if (p.M == 0) {  // sums over no tokens
-    hipError_t e = hipSuccess;
-    if (dw) e = product_add_splits(nullptr, dw, (long long)p.rows * p.K, 0, p.dtype, stream);
-    if (db && e == hipSuccess) e = product_add_splits(nullptr, db, p.rows, 0, p.dtype, stream);
-    return api_launch(fn, e);
-  }
+  const long long values = (long long)p.rows * p.K;
+  if (p.M == 0)  // sums over no tokens
+    return api_launch(fn, product_sum({{nullptr, dw, dw ? values : 0, 0},
+                                       {nullptr, db, db ? p.rows : 0, 0}}, p.dtype, stream));
   if (!x || !w || !dy) return api_fail(fn, "null buffer");
   if (!dx && !dw && !db) return api_launch(fn, hipSuccess);
   char* ws = (char*)workspace;
   const BackwardSpace s = backward_space(p, x, w, dy, ws, dx, dw, db);
   if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
   if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
-  hipError_t e = hipSuccess;
-  if (s.pad_x)
-    e = product_pad(x_view(p, x).at, x_view(p, x).row, x_view(p, x).image, ws + s.x,
-                    tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype, stream);
-  if (s.pad_w && e == hipSuccess)
-    e = product_pad(w, p.K, 0, ws + s.w, p.rows, p.rows, p.K, p.dtype, stream);
-  if (e == hipSuccess && needs_z(p)) {
+  // the copies, and zeros behind the rows of a dz that is to come
+  const bool z = needs_z(p);
+  hipError_t e = product_lay_out(
+      {lay_x(p, x, s.pad_x, ws + s.x), lay_w(p, w, s.pad_w, ws + s.w), lay_dz(p, z, dy, s, ws)},
+      p.dtype, stream);
+  if (e == hipSuccess && z) {
     ProductArgs g = dz_args(p, s.xv, s.wv, bias, dy, s.dzv);
     g.sums = db ? (float*)(ws + s.sums) : nullptr;
     g.low = s.low;
     g.part = (float*)(ws + s.part);
     g.part_bytes = s.part_bytes;
     e = product_launch(g, p.dtype, stream);
-    if (s.pad_dz && e == hipSuccess)
-      e = product_zero_tails(ws, s.dz_rows, dz_cols(p), p.dtype, stream);
-  } else if (e == hipSuccess && s.pad_dz) {
-    const View v = dz_view(p, dy);
-    e = product_pad(dy, v.row, v.image, ws, tokens(p) ? p.M : p.rows, dz_rows(p), dz_cols(p),
-                    p.dtype, stream);
   }
+  // sums of parts in one launch at the end, unless they would have left the cache by then
+  SumJob sum_dx = {}, sum_dw = {}, sum_db = {};
+  const bool later = s.part_bytes + s.dw_part_bytes <= (32u << 20);
   if (dx && e == hipSuccess) {
     ProductArgs g = dx_args(p, s.dzv, s.low, s.wv, s.dx_splits > 1 ? (void*)(ws + s.part) : dx);
     g.splits = s.dx_splits;
     g.part_bytes = s.part_bytes;
     e = product_launch(g, p.dtype, stream);
-    if (e == hipSuccess && s.dx_splits > 1)
-      e = product_add_splits((const float*)(ws + s.part), dx, p.M * p.K, s.dx_splits, p.dtype,
-                             stream);
+    if (s.dx_splits > 1) sum_dx = {(const float*)(ws + s.part), dx, p.M * p.K, s.dx_splits};
+    if (e == hipSuccess && !later) {
+      e = product_sum({sum_dx}, p.dtype, stream);
+      sum_dx = {};
+    }
   }
   if (dw && e == hipSuccess) {
-    ProductArgs g = dw_args(p, s.xv, s.dzv, s.low, s.splits > 1 ? (void*)(ws + s.part) : dw);
+    ProductArgs g = dw_args(p, s.xv, s.dzv, s.low, s.splits > 1 ? (void*)(ws + s.dw_part) : dw);
     g.splits = s.splits;
-    g.part_bytes = s.part_bytes;
+    g.part_bytes = s.dw_part_bytes;
     e = product_launch(g, p.dtype, stream);
-    if (e == hipSuccess && s.splits > 1)
-      e = product_add_splits((const float*)(ws + s.part), dw, (long long)p.rows * p.K, s.splits,
-                             p.dtype, stream);
+    if (s.splits > 1) sum_dw = {(const float*)(ws + s.dw_part), dw, values, s.splits};
   }
   if (db && e == hipSuccess) {
     float* sums = (float*)(ws + s.sums);
-    if (!needs_z(p))
-      e = product_column_sums(dy, sums, p.layout, p.B, p.P, p.rows, s.rows, p.dtype, stream);
-    if (e == hipSuccess) e = sum_rows(sums, db, p.rows, s.rows, p.dtype, stream);
+    if (!z) e = product_column_sums(dy, sums, p.layout, p.B, p.P, p.rows, s.rows, p.dtype, stream);
+    sum_db = {sums, db, p.rows, s.rows};
   }
+  if (e == hipSuccess) e = product_sum({sum_dx, sum_dw, sum_db}, p.dtype, stream);
   return api_launch(fn, e);
 }
 
@@ -379,14 +390,8 @@ int product_forward(const char* fn, const Problem& p, const void* x, const void*
   const ForwardSpace s = forward_space(p, x, w, ws);
   if (s.total > 0 && (!workspace || bytes < s.total)) return api_fail(fn, "workspace too small");
   if (!aligned_to(workspace, 256)) return api_fail(fn, "workspace not aligned");
-  hipError_t e = hipSuccess;
-  if (s.pad_x) {
-    const View v = x_view(p, x);
-    e = product_pad(x, v.row, v.image, ws, tokens(p) ? p.M : p.K, x_rows(p), x_cols(p), p.dtype,
-                    stream);
-  }
-  if (s.pad_w && e == hipSuccess)
-    e = product_pad(w, p.K, 0, ws + s.w, p.rows, p.rows, p.K, p.dtype, stream);
+  hipError_t e = product_lay_out({lay_x(p, x, s.pad_x, ws), lay_w(p, w, s.pad_w, ws + s.w)},
+                                 p.dtype, stream);
   if (e == hipSuccess) {
     ProductArgs g = y_args(p, s.xv, s.wv, bias, res, y);
     g.part = (float*)(ws + s.part);

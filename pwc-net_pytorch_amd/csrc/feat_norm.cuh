@@ -17,8 +17,6 @@ struct NormArgs {
   float eps;
 };
 
-// out[c] = sum over `rows` of part[row][c], in their order
-hipError_t sum_rows(const float* part, void* out, int C, int rows, int dtype, hipStream_t s);
 int norm_parts(int layout, long long B, long long P, int C, int dtype);
 hipError_t norm_forward(const NormArgs& a, int dtype, hipStream_t s);
 hipError_t norm_no_rows(const NormArgs& a, int dtype, hipStream_t s);  // dw = db = 0

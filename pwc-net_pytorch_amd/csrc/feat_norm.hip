@@ -645,17 +645,6 @@ template <typename T> static hipError_t no_rows_t(const NormArgs& a, hipStream_t
   return hipGetLastError();
 }
 
-hipError_t sum_rows(const float* part, void* out, int C, int rows, int dtype, hipStream_t s) {
-  const dim3 grid((C + 31) / 32, 1);
-  if (dtype == 0)
-    norm_add_parts<float><<<grid, 1024, 0, s>>>(part, (float*)out, nullptr, C, rows);
-  else if (dtype == 1)
-    norm_add_parts<__half><<<grid, 1024, 0, s>>>(part, (__half*)out, nullptr, C, rows);
-  else
-    norm_add_parts<__hip_bfloat16><<<grid, 1024, 0, s>>>(part, (__hip_bfloat16*)out, nullptr, C,
-                                                        rows);
-  return hipGetLastError();
-}
 hipError_t norm_no_rows(const NormArgs& a, int dtype, hipStream_t s) {
   return dtype == 0   ? no_rows_t<float>(a, s)
          : dtype == 1 ? no_rows_t<__half>(a, s)

@@ -66,15 +66,25 @@ int product_sum_rows(const ProductArgs& g, int dtype);
 int product_column_parts(int layout, long long B, long long P, int C);
 hipError_t product_column_sums(const void* dy, float* part, int layout, long long B, long long P,
                                int C, int parts, int dtype, hipStream_t stream);
+
+// Several small passes over memory in one launch, each with a share of the grid.
+constexpr int kJobs = 3;
 // dst: `rows` rows of `cols` values, zeros up to the next 16 bytes; src: rows `row` apart, groups of
-// `per_image` rows `image` apart
-hipError_t product_pad(const void* src, long long row, long long image, void* dst,
-                       long long per_image, long long rows, long long cols, int dtype,
-                       hipStream_t stream);
-hipError_t product_zero_tails(void* dst, long long rows, long long cols, int dtype,
-                              hipStream_t stream);
-hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
-                              hipStream_t stream);
+// `per_image` rows `image` apart.  Without src the zeros alone.  rows 0: no job
+struct LayJob {
+  const void* src;
+  void* dst;
+  long long row, image, per_image, rows, cols;
+};
+hipError_t product_lay_out(const LayJob (&jobs)[kJobs], int dtype, hipStream_t stream);
+// out[n] = sum over `parts` rows of n values, in a fixed order (zeros for none).  n 0: no job
+struct SumJob {
+  const float* part;
+  void* out;
+  long long n;
+  int parts;
+};
+hipError_t product_sum(const SumJob (&jobs)[kJobs], int dtype, hipStream_t stream);
 
 }  // namespace feat
 }  // namespace pwc

@@ -27,24 +27,12 @@
 // 16x16x4 instructions).  The order of k within a fragment does not matter as long as both
 // operands share it; N tiles of 16 bits are turned by the transposing LDS read.
 
-#include "feat_norm.cuh"
 #include "feat_product.cuh"
 
 namespace pwc {
 namespace feat {
 
 constexpr int kStepBytes = 128;  // of either operand's k, as in the kernel
-
-// out[n] = sum over the splits, in their order (the same sums whatever ran first)
-template <typename T>
-__global__ __launch_bounds__(256) void add_splits(const float* __restrict__ part,
-                                                  T* __restrict__ out, long long n, int splits) {
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += part[s * n + i];
-    out[i] = narrow<T>(v);
-  }
-}
 
 // Direct loads want whole 16-byte chunks at 16-byte places and offsets within 31 bits.
 template <typename T> static bool direct_loads(const ProductArgs& g, int bi, int bj) {
@@ -296,15 +284,6 @@ size_t product_part_bytes(const ProductArgs& g, int dtype) {
   return splits > 1 ? align256((size_t)splits * g.I * g.J * sizeof(float)) : 0;
 }
 
-template <typename T>
-static hipError_t add_splits_t(const float* part, void* out, long long n, int splits,
-                               hipStream_t stream) {
-  const long long blocks = (n + 255) / 256;
-  add_splits<T><<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, stream>>>(part, (T*)out, n,
-                                                                               splits);
-  return hipGetLastError();
-}
-
 // Rows of partial sums that a kLinearDz / kGatedDz launch writes.
 int product_sum_rows(const ProductArgs& g, int dtype) {
   const ProductPlan p = product_plan(g, dtype);
@@ -315,50 +294,95 @@ int product_sum_rows(const ProductArgs& g, int dtype) {
 }
 
 // ---- rows at 16-byte places ----
-template <typename T>
-__global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, long long row,
-                                                long long image, T* __restrict__ dst,
-                                                long long per_image, long long rows,
-                                                long long cols) {
+struct LayJobs {
+  LayJob job[kJobs];
+};
+template <typename T> __global__ __launch_bounds__(256) void lay_out(const LayJobs jobs) {
   constexpr int E = 16 / (int)sizeof(T);
-  const long long chunks = (cols + E - 1) / E;
-  for (long long id = blockIdx.x * 256LL + threadIdx.x; id < rows * chunks;
-       id += gridDim.x * 256LL) {
+  const LayJob& j = jobs.job[blockIdx.y];
+  T* dst = (T*)j.dst;
+  const long long chunks = (j.cols + E - 1) / E, pitch = chunks * E;
+  const long long first = blockIdx.x * 256LL + threadIdx.x, next = gridDim.x * 256LL;
+  if (!j.src) {
+    for (long long r = first; r < j.rows; r += next)
+      for (long long c = j.cols; c < pitch; ++c) dst[r * pitch + c] = narrow<T>(0.f);
+    return;
+  }
+  for (long long id = first; id < j.rows * chunks; id += next) {
     const long long r = id / chunks, c = (id - r * chunks) * E;
-    const long long m = r / per_image;
-    const T* p = src + m * image + (r - m * per_image) * row + c;
-    *(u32x4*)(dst + id * E) = cols - c >= E ? load16(p) : load_some(p, (int)(cols - c));
+    const long long m = r / j.per_image;
+    const T* p = (const T*)j.src + m * j.image + (r - m * j.per_image) * j.row + c;
+    *(u32x4*)(dst + id * E) = j.cols - c >= E ? load16(p) : load_some(p, (int)(j.cols - c));
   }
 }
-template <typename T>
-__global__ __launch_bounds__(256) void zero_tails(T* __restrict__ dst, long long rows,
-                                                  long long cols, long long pitch) {
-  for (long long r = blockIdx.x * 256LL + threadIdx.x; r < rows; r += gridDim.x * 256LL)
-    for (long long c = cols; c < pitch; ++c) dst[r * pitch + c] = narrow<T>(0.f);
-}
-static unsigned some_blocks(long long n) {
-  const long long b = (n + 255) / 256;
-  return (unsigned)(b < 16384 ? b : 16384);
-}
-hipError_t product_pad(const void* src, long long row, long long image, void* dst,
-                       long long per_image, long long rows, long long cols, int dtype,
-                       hipStream_t stream) {
+hipError_t product_lay_out(const LayJob (&jobs)[kJobs], int dtype, hipStream_t stream) {
+  LayJobs all = {};
+  long long blocks = 0;
+  int n = 0;
+  const long long e = dtype == 0 ? 4 : 8;
+  for (const LayJob& j : jobs) {
+    const long long chunks = (j.cols + e - 1) / e;
+    if (j.rows == 0 || (!j.src && chunks * e == j.cols)) continue;
+    all.job[n++] = j;
+    const long long b = ((j.src ? j.rows * chunks : j.rows) + 255) / 256;
+    if (blocks < b) blocks = b;
+  }
+  if (n == 0) return hipSuccess;
+  const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384), n);
   if (dtype == 0)
-    pad_rows<float><<<some_blocks(rows * ((cols + 3) / 4)), 256, 0, stream>>>(
-        (const float*)src, row, image, (float*)dst, per_image, rows, cols);
+    lay_out<float><<<grid, 256, 0, stream>>>(all);
   else  // 16 bits are moved as they are
-    pad_rows<__half><<<some_blocks(rows * ((cols + 7) / 8)), 256, 0, stream>>>(
-        (const __half*)src, row, image, (__half*)dst, per_image, rows, cols);
+    lay_out<__half><<<grid, 256, 0, stream>>>(all);
   return hipGetLastError();
 }
-hipError_t product_zero_tails(void* dst, long long rows, long long cols, int dtype,
-                              hipStream_t stream) {
-  const long long e = dtype == 0 ? 4 : 8, pitch = (cols + e - 1) / e * e;
-  if (pitch == cols) return hipSuccess;
+
+// ---- sums of parts ----
+struct SumJobs {
+  SumJob job[kJobs];
+  int groups[kJobs];  // threads that share a value's parts: many parts of few values
+};
+template <typename T> __global__ __launch_bounds__(1024) void sum_parts(const SumJobs jobs) {
+  __shared__ float red[1024];
+  const SumJob& j = jobs.job[blockIdx.y];
+  const int groups = jobs.groups[blockIdx.y], cols = 1024 / groups;
+  const int col = threadIdx.x % cols, group = threadIdx.x / cols;
+  for (long long c0 = (long long)blockIdx.x * cols; c0 < j.n; c0 += (long long)gridDim.x * cols) {
+    const long long c = c0 + col;
+    float s = 0.f;
+    if (c < j.n) {
+#pragma unroll 8
+      for (int k = group; k < j.parts; k += groups) s += j.part[k * j.n + c];
+    }
+    if (groups > 1) {
+      __syncthreads();
+      red[threadIdx.x] = s;
+      __syncthreads();
+      if (group == 0)
+        for (int k = 1; k < groups; ++k) s += red[k * cols + col];
+    }
+    if (group == 0 && c < j.n) ((T*)j.out)[c] = narrow<T>(s);
+  }
+}
+hipError_t product_sum(const SumJob (&jobs)[kJobs], int dtype, hipStream_t stream) {
+  SumJobs all = {};
+  long long blocks = 0;
+  int n = 0;
+  for (const SumJob& j : jobs) {
+    if (j.n == 0) continue;
+    all.job[n] = j;
+    all.groups[n] = j.parts > 8 && j.n <= (1 << 20) ? 32 : 1;
+    const long long cols = 1024 / all.groups[n], b = (j.n + cols - 1) / cols;
+    if (blocks < b) blocks = b;
+    ++n;
+  }
+  if (n == 0) return hipSuccess;
+  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), n);
   if (dtype == 0)
-    zero_tails<float><<<some_blocks(rows), 256, 0, stream>>>((float*)dst, rows, cols, pitch);
+    sum_parts<float><<<grid, 1024, 0, stream>>>(all);
+  else if (dtype == 1)
+    sum_parts<__half><<<grid, 1024, 0, stream>>>(all);
   else
-    zero_tails<__half><<<some_blocks(rows), 256, 0, stream>>>((__half*)dst, rows, cols, pitch);
+    sum_parts<__hip_bfloat16><<<grid, 1024, 0, stream>>>(all);
   return hipGetLastError();
 }
 
@@ -434,15 +458,6 @@ hipError_t product_column_sums(const void* dy, float* part, int layout, long lon
   return dtype == 0   ? column_sums_t<float>(dy, part, layout, B, P, C, parts, stream)
          : dtype == 1 ? column_sums_t<__half>(dy, part, layout, B, P, C, parts, stream)
                       : column_sums_t<__hip_bfloat16>(dy, part, layout, B, P, C, parts, stream);
-}
-
-hipError_t product_add_splits(const float* part, void* out, long long n, int splits, int dtype,
-                              hipStream_t stream) {
-  // many splits of few values: 32 threads share a value's splits
-  if (splits > 8 && n <= (1 << 20)) return sum_rows(part, out, (int)n, splits, dtype, stream);
-  return dtype == 0   ? add_splits_t<float>(part, out, n, splits, stream)
-         : dtype == 1 ? add_splits_t<__half>(part, out, n, splits, stream)
-                      : add_splits_t<__hip_bfloat16>(part, out, n, splits, stream);
 }
 
 }  // namespace feat
