@@ -75,6 +75,42 @@ __device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
   }
 }
 
+// Four neighbouring values at any alignment, zeros (nothing) from `left` on
+typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T>
+__device__ __forceinline__ void load_four(const T* p, int left, float (&v)[4]) {
+  u32x4 q = {0u, 0u, 0u, 0u};
+  if (left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      q = load16(p);
+    } else {
+      const u32x2_at2 h = *(const u32x2_at2*)p;
+      q = u32x4{h[0], h[1], 0u, 0u};
+    }
+  } else if (left > 0) {
+    q = load_some(p, left);
+  }
+  const Pack<T, 16 / sizeof(T)> o = __builtin_bit_cast(Pack<T, 16 / sizeof(T)>, q);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = to_f32(o.v[e]);
+}
+template <typename T>
+__device__ __forceinline__ void store_four(T* p, const float (&v)[4], int left) {
+  Pack<T, 16 / sizeof(T)> o = {};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o.v[e] = narrow<T>(v[e]);
+  const u32x4 q = __builtin_bit_cast(u32x4, o);
+  if (left >= 4) {
+    if constexpr (sizeof(T) == 4)
+      *(u32x4_at4*)p = q;
+    else
+      *(u32x2_at2*)p = u32x2_at2{q[0], q[1]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) p[e] = o.v[e];
+  }
+}
 // what rounding takes from the values; nothing where it gives an infinity or a NaN
 template <typename T, int V> __device__ __forceinline__ void rounded_off(float (&v)[V]) {
 #pragma unroll

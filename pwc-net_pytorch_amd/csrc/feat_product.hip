@@ -137,29 +137,17 @@ __global__ __launch_bounds__(256) void finish_parts(const ProductArgs g, int spl
   __shared__ float red[kDz ? 3 : 1][kPair ? 2 : 1][256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int outs = kPair ? g.pair : g.I, i = (blockIdx.x * 64 + lane) * 4, left = outs - i;
-  auto four = [&](const auto* p, int n, float(&v)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = 0.f;
-    if (n >= 4) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = to_f32(p[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (e < n) v[e] = to_f32(p[e]);
-    }
-  };
   const T* bias = (const T*)g.bias;
   float b[4], c[4], sv[4], sw[4];
-  four(bias + i, bias ? left : 0, b);
-  four(bias + g.pair + i, bias && kPair ? left : 0, c);
+  load_four(bias + i, bias ? left : 0, b);
+  load_four(bias + g.pair + i, bias && kPair ? left : 0, c);
 #pragma unroll
   for (int e = 0; e < 4; ++e) sv[e] = sw[e] = 0.f;
   for (int r = 0; r < each; ++r) {
     const int j = (blockIdx.y * each + r) * 4 + wave;
     if (j >= g.J || left <= 0) break;
     float v[4], w[4], d[4], t[4], o[4];
-    four((const T*)g.other + (long long)j * g.ldother + i, g.other ? left : 0, o);
+    load_four((const T*)g.other + (long long)j * g.ldother + i, g.other ? left : 0, o);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = b[e];
@@ -168,11 +156,11 @@ __global__ __launch_bounds__(256) void finish_parts(const ProductArgs g, int spl
     const float* p = g.part + (long long)j * g.I + i;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s, p += (long long)g.I * g.J) {
-      four(p, left, t);
+      load_four(p, left, t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += t[e];
       if constexpr (kPair) {
-        four(p + g.pair, left, t);
+        load_four(p + g.pair, left, t);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] += t[e];
       }
@@ -205,12 +193,8 @@ __global__ __launch_bounds__(256) void finish_parts(const ProductArgs g, int spl
         rounded_off<T, 4>(w);
         out += g.low;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) {
-          out[e] = narrow<T>(v[e]);
-          if (MODE == kGatedDz) out[g.pair + e] = narrow<T>(w[e]);
-        }
+      store_four(out, v, left);
+      if (MODE == kGatedDz) store_four(out + g.pair, w, left);
     }
   }
   if constexpr (kDz) {
@@ -337,52 +321,77 @@ hipError_t product_lay_out(const LayJob (&jobs)[kJobs], int dtype, hipStream_t s
 }
 
 // ---- sums of parts ----
+// Bound by memory.  Few parts of many values: a thread takes four values.  Many parts of few values:
+// `groups` threads share a value, eight parts each, and join through LDS; the order is the same
+// whatever runs first.
 struct SumJobs {
   SumJob job[kJobs];
-  int groups[kJobs];  // threads that share a value's parts: many parts of few values
+  int groups[kJobs], first[kJobs + 1];  // first: blocks before the job's
 };
-template <typename T> __global__ __launch_bounds__(1024) void sum_parts(const SumJobs jobs) {
-  __shared__ float red[1024];
-  const SumJob& j = jobs.job[blockIdx.y];
-  const int groups = jobs.groups[blockIdx.y], cols = 1024 / groups;
-  const int col = threadIdx.x % cols, group = threadIdx.x / cols;
-  for (long long c0 = (long long)blockIdx.x * cols; c0 < j.n; c0 += (long long)gridDim.x * cols) {
+template <typename T> __global__ __launch_bounds__(512) void sum_parts(const SumJobs jobs) {
+  __shared__ float red[512];
+  int which = 0;
+#pragma unroll
+  for (int k = 1; k < kJobs; ++k) which += (int)blockIdx.x >= jobs.first[k];
+  const SumJob& j = jobs.job[which];
+  const int groups = jobs.groups[which], blocks = jobs.first[which + 1] - jobs.first[which];
+  const long long block = (int)blockIdx.x - jobs.first[which];
+  T* out = (T*)j.out;
+  if (groups == 1) {
+    for (long long c = (block * 512 + threadIdx.x) * 4; c < j.n; c += blocks * 2048LL) {
+      const int have = j.n - c < 4 ? (int)(j.n - c) : 4;
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int k = 0; k < j.parts; ++k) {
+        const float* p = j.part + k * j.n + c;
+        const Pack<float, 4> v =
+            __builtin_bit_cast(Pack<float, 4>, have == 4 ? load16(p) : load_some(p, have));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v.v[e];
+      }
+      store_four(out + c, s, have);
+    }
+    return;
+  }
+  const int cols = 512 / groups, col = threadIdx.x % cols, group = threadIdx.x / cols;
+  for (long long c0 = block * cols; c0 < j.n; c0 += (long long)blocks * cols) {
     const long long c = c0 + col;
     float s = 0.f;
     if (c < j.n) {
 #pragma unroll 8
       for (int k = group; k < j.parts; k += groups) s += j.part[k * j.n + c];
     }
-    if (groups > 1) {
-      __syncthreads();
-      red[threadIdx.x] = s;
-      __syncthreads();
-      if (group == 0)
-        for (int k = 1; k < groups; ++k) s += red[k * cols + col];
-    }
-    if (group == 0 && c < j.n) ((T*)j.out)[c] = narrow<T>(s);
+    __syncthreads();
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (group > 0 || c >= j.n) continue;
+    for (int k = 1; k < groups; ++k) s += red[k * cols + col];
+    out[c] = narrow<T>(s);
   }
 }
 hipError_t product_sum(const SumJob (&jobs)[kJobs], int dtype, hipStream_t stream) {
   SumJobs all = {};
-  long long blocks = 0;
   int n = 0;
+  long long blocks = 0;
   for (const SumJob& j : jobs) {
     if (j.n == 0) continue;
+    int groups = 1;
+    while (groups < 32 && groups * 16 <= j.parts) groups *= 2;
+    const long long each = groups == 1 ? 2048 : 512 / groups, b = (j.n + each - 1) / each;
     all.job[n] = j;
-    all.groups[n] = j.parts > 8 && j.n <= (1 << 20) ? 32 : 1;
-    const long long cols = 1024 / all.groups[n], b = (j.n + cols - 1) / cols;
-    if (blocks < b) blocks = b;
+    all.groups[n] = groups;
+    all.first[n] = (int)blocks;
+    blocks += b < 65536 ? b : 65536;
     ++n;
   }
   if (n == 0) return hipSuccess;
-  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), n);
+  for (int k = n; k <= kJobs; ++k) all.first[k] = (int)blocks;
   if (dtype == 0)
-    sum_parts<float><<<grid, 1024, 0, stream>>>(all);
+    sum_parts<float><<<(unsigned)blocks, 512, 0, stream>>>(all);
   else if (dtype == 1)
-    sum_parts<__half><<<grid, 1024, 0, stream>>>(all);
+    sum_parts<__half><<<(unsigned)blocks, 512, 0, stream>>>(all);
   else
-    sum_parts<__hip_bfloat16><<<grid, 1024, 0, stream>>>(all);
+    sum_parts<__hip_bfloat16><<<(unsigned)blocks, 512, 0, stream>>>(all);
   return hipGetLastError();
 }
 
