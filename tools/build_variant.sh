@@ -9,7 +9,7 @@ UNIT=${UNIT:?unit}
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 OBJ=$ROOT/pwc-net_pytorch_amd/build/obj
 mkdir -p $OUTDIR
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -ffp-contract=fast-honor-pragmas \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=fast-honor-pragmas \
   -munsafe-fp-atomics -fvisibility=hidden -fno-slp-vectorize $DEFS -c -o $OUTDIR/$UNIT.o \
   $ROOT/pwc-net_pytorch_amd/csrc/$UNIT.hip
 objs=$(ls $OBJ/*.o | grep -v "/$UNIT.o$")
