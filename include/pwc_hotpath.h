@@ -359,7 +359,8 @@ PWC_API int pwc_rotary(const void* x, void* y, const void* positions, const void
 
 /* y = act(x weight^T + bias) + residual; weight [O][K], bias [O] or NULL, residual like y or
  * NULL.  The workspace holds copies of x and weight with rows at 16-byte places, where they are not
- * and the call is large enough to gain by it (of the pointers given to the size functions only the
+ * and the call is large enough to gain by it, and 32-bit sums over parts of K, where there are too
+ * few tokens to fill the card otherwise (of the pointers given to the size functions only the
  * alignment is looked at; a size of 0 means that none is used). */
 PWC_API size_t pwc_linear_forward_workspace_size(const void* x, const void* weight, int layout,
                                                  long long B, long long P, int K, int O,
