@@ -9,6 +9,10 @@
 // mean costs no digits), every sum is in 32 bits.  The weight's gradient is summed by each thread
 // for its own channels over the rows of a block that stays on its CU, then over the blocks in
 // their order: no atomics, the same sums each time.
+//
+// Measured: 16383 x 2048 bf16 tokens 29 us forward (4.6 TB/s) and 46 backward (4.4; a 1 GiB copy does
+// 5.1), a block a row; the 8 x 32 x 96 x 112 fp32 map 7.6 and 11.5 us, 64 pixels a block, and 4 us
+// for the sums over blocks.
 #include "feat_common.cuh"
 #include "feat_norm.cuh"
 
@@ -362,7 +366,8 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
 }
 
 // ------------------------------------------------------------------------------ any C
-// Rows longer than the registers are read again for each pass.  S threads share a row: a whole
+// Rows longer than the registers are read again for each pass (from the cache: 2000 x 9000 bf16
+// tokens are 36 MB), bound by those reads.  S threads share a row: a whole
 // block (tokens, S = 256), or one of 64 pixels' four threads (maps, S = 4).
 struct RowAt {
   long long base, y, stride;  // first value in x, in y / dy / dx; between channels
