@@ -97,13 +97,13 @@ View dz_view(const Problem& p, const void* dz) {
 constexpr double kKeepLow = 5e8;  // operations of a product whose dz is kept in two parts
 
 // The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
-// not, large ones are laid out so first.  Forward alone that is worth its launches from some GFLOP
-// on (us, as they lie / laid out first; 16 bits: 2047 x 1023 -> 1023, 4.3 GFLOP: 19 / 25;
-// 8191 x 1023 -> 4095: 164 / 103).  Backward the three products share the copies, and rows of odd
-// 16-bit lengths that are read across k cost most (act'; 1001 x 511 -> 511: 56 / 38, 2047 x 1023 ->
-// 1023: 137 / 65, 301 x 511 -> 511 without one 43 / 29; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 60; fp32 2001 x 701 -> 1001: 160 / 131),
-// unless so few channels meet that the products are all traffic anyway (map 16 x 64 x 113 x 129 ->
-// 64: 81 / 88, fp32 136 / 155).
+// not, large ones are laid out so first.  Forward alone that is worth its launch from some GFLOP on
+// (us, as they lie / laid out first; 16 bits: 2047 x 1023 -> 1023, 4.3 GFLOP: 19 / 25; 8191 x 1023 ->
+// 4095: 164 / 103).  Backward the three products share the copies, and rows of odd 16-bit lengths
+// that are read across k cost most (with an activation: 1001 x 511 -> 511: 56 / 38, 2047 x 1023 ->
+// 1023: 137 / 65; without: 301 x 511 -> 511: 43 / 29; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 55;
+// fp32 2001 x 701 -> 1001: 160 / 130), unless so few channels meet that the products are all traffic
+// anyway (map 16 x 64 x 113 x 129 -> 64: 81 / 88, fp32 136 / 155).
 bool pads_pay(const Problem& p, bool backward) {
   const double operations = 2.0 * (double)p.M * p.rows * p.K;
   if (!backward) return operations >= 8e9;
@@ -242,9 +242,11 @@ ForwardSpace forward_space(const Problem& p, const void* x, const void* w, const
 
 struct BackwardSpace {
   bool pad_x, pad_w, pad_dz;
-  size_t x, w, part, part_bytes, dw_part, dw_part_bytes, sums, total;  // dz, or the padded dy, lies at 0
+  // dz, or the padded dy, lies at 0
+  size_t x, w, part, part_bytes, dw_part, dw_part_bytes, sums, total;
   int dx_splits, splits, rows;     // rows: of partial bias gradients
-  long long dz_rows, low;          // low: from dz to what its rounding took (maps: image by image), or 0
+  long long dz_rows;
+  long long low;  // from dz to what its rounding took (maps: image by image), or 0
   View xv, wv, dzv;                // as the products take them
 };
 BackwardSpace backward_space(const Problem& p, const void* x, const void* w, const void* dy,

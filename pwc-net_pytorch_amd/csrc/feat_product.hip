@@ -330,8 +330,8 @@ hipError_t product_lay_out(const LayJob (&jobs)[kJobs], int dtype, hipStream_t s
 }
 
 // ---- sums of parts ----
-// Bound by memory (two parts of 4096 x 1024 values and a bias gradient, 34 MB read: 10.5 us).  Few parts of
-// many values: a thread takes four values.  Many parts of few values:
+// Bound by memory (two parts of 4096 x 1024 values and a bias gradient, 34 MB read: 10.5 us).  Few
+// parts of many values: a thread takes four values.  Many parts of few values:
 // `groups` threads share a value, eight parts each, and join through LDS; the order is the same
 // whatever runs first.
 struct SumJobs {
@@ -406,8 +406,8 @@ hipError_t product_sum(const SumJob (&jobs)[kJobs], int dtype, hipStream_t strea
 }
 
 // Partial column sums of dy, for a linear without an activation: tokens [M][C], a wave V channels
-// of a lane by 4 waves' rows; maps [B][C][P], a block a channel.  Bound by reading dy (8192 x 4096 bf16,
-// 67 MB: 11 us and the sums over the parts).
+// of a lane by 4 waves' rows; maps [B][C][P], a block a channel.  Bound by reading dy (8192 x 4096
+// bf16, 67 MB: 15 us with the sums over the parts).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void sum_tokens(const T* __restrict__ dy,
                                                   float* __restrict__ part, long long M, int C) {

@@ -141,7 +141,7 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
   uint32_t off[Tl::LOADS];  // DIRECT: bytes from base, or kOOB
   int at[Tl::LOADS];        // first k (K) or row k (N) of the chunk within the step
   long long row[DIRECT ? 1 : Tl::LOADS];
-  int left[DIRECT ? 1 : Tl::LOADS];  // N: valid values from the chunk's start; K: 0 or 1 (row valid)
+  int left[DIRECT ? 1 : Tl::LOADS];  // N: valid values from the chunk's start; K: row valid, 0 or 1
   u32x4 reg[DIRECT ? 1 : Tl::LOADS];
 
   // `pair` > 0: rows alternate in groups of 16 between the halves of a matrix of 2 * pair rows
@@ -539,8 +539,8 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   auto settle = [&](char* pa, char* pb, auto behind) __attribute__((always_inline)) {
     la.finish(pa);
     lb.finish(pb);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(DIRECT ? decltype(behind)::value * LOADS : 0)
-                 : "memory");
+    constexpr int flying = DIRECT ? decltype(behind)::value * LOADS : 0;
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(flying) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
@@ -555,8 +555,8 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
   //   multiply half 0, reading half 1 | wait for the next step's loads, barrier |
   //   multiply half 1, reading half 0 of the next step and starting the loads of the step STAGES on
   //   into the buffer that all waves have read
-  // so the loads have STAGES - 1 steps, the reads half a step, and one barrier a step is enough.  Where
-  // one wave a SIMD has to feed the matrix unit alone, reads and loads stand between its
+  // so the loads have STAGES - 1 steps, the reads half a step, and one barrier a step is enough.
+  // Where one wave a SIMD has to feed the matrix unit alone, reads and loads stand between its
   // instructions, a row of fragments at a time: issued in one go they fill the queues and it waits
   // behind them (8192 x K -> 4096 tokens: 1430 -> 1520 TFLOP/s).  With two waves a SIMD one
   // multiplies while the other issues, and the same order costs a third of the rate.
@@ -733,8 +733,8 @@ __global__ __launch_bounds__(kFewWaves * 64, JB < 4 ? 4 : 2) void few_tokens(con
     for (int f = 0; f < FA; ++f) {
       const int i = i0 + f / HALVES * 16 + r;
       oa[f][n] = i < outs;
-      pa[f][n] =
-          (const T*)g.a + ((long long)(kPair && f % 2 ? g.pair : 0) + (oa[f][n] ? i : 0)) * g.lda + at;
+      const long long row = (long long)(kPair && f % 2 ? g.pair : 0) + (oa[f][n] ? i : 0);
+      pa[f][n] = (const T*)g.a + row * g.lda + at;
     }
 #pragma unroll
     for (int f = 0; f < JB; ++f) {
