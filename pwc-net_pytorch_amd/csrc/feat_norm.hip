@@ -366,9 +366,10 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
 }
 
 // ------------------------------------------------------------------------------ any C
-// Rows longer than the registers are read again for each pass (from the cache: 2000 x 9000 bf16
-// tokens are 36 MB), bound by those reads.  S threads share a row: a whole
-// block (tokens, S = 256), or one of 64 pixels' four threads (maps, S = 4).
+// Rows longer than the registers are read again for each pass, mostly from the caches, and bound by
+// those reads: S threads share a row -- a whole block, V channels each (tokens), or 16 that have one
+// of 64 pixels (maps) -- with several loads under way.  16384 x 9000 bf16 tokens: 161 us forward (3.7
+// TB/s of what one read and one write are), 362 backward; the 8 x 300 x 2688 bf16 map 17 and 35.
 struct RowAt {
   long long base, y, stride;  // first value in x, in y / dy / dx; between channels
   long long m;
@@ -393,28 +394,39 @@ template <bool MAP> __device__ __forceinline__ RowAt row_at(const NormArgs& a) {
   }
   return r;
 }
+constexpr int any_threads(bool map) { return map ? 1024 : 256; }
 template <bool MAP> __device__ __forceinline__ float any_sum(float v, float (*red)[64]) {
   if constexpr (MAP) {
     float s[1] = {v};
-    pixel_sum<4, 1>(s, red);
+    pixel_sum<16, 1>(s, red);
     return s[0];
   } else {
     return row_sum<256>(v, red[0]);
   }
 }
 
-template <typename T, bool MAP> __global__ __launch_bounds__(256) void norm_any(const NormArgs a) {
-  __shared__ float red[4][64];
+template <typename T, bool MAP, int V>
+__global__ __launch_bounds__(any_threads(MAP)) void norm_any(const NormArgs a) {
+  __shared__ float red[MAP ? 16 : 1][64];
   const RowAt r = row_at<MAP>(a);
-  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x, S = MAP ? 4 : 256;
+  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x * V, S = MAP ? 16 : 256 * V;
   const T* x = (const T*)a.x + r.base;
   float s = 0.f;
-  for (int c = first; c < a.C; c += S) s += to_f32(x[c * r.stride]);
+#pragma unroll 4
+  for (int c = first; c < a.C; c += S) {
+    float v[V];
+    load_values<T, V>(x + c * r.stride, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += v[e];
+  }
   const float mu = any_sum<MAP>(s, red) / a.C;
   s = 0.f;
+#pragma unroll 4
   for (int c = first; c < a.C; c += S) {
-    const float d = to_f32(x[c * r.stride]) - mu;
-    s += d * d;
+    float v[V];
+    load_values<T, V>(x + c * r.stride, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += (v[e] - mu) * (v[e] - mu);
   }
   const float rs = 1.f / sqrtf(any_sum<MAP>(s, red) / a.C + a.eps);
   if (!r.ok) return;
@@ -423,68 +435,103 @@ template <typename T, bool MAP> __global__ __launch_bounds__(256) void norm_any(
     a.rstd[r.m] = rs;
   }
   T* y = (T*)a.y + r.y;
+#pragma unroll 2
   for (int c = first; c < a.C; c += S) {
-    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
-    const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
-    y[c * r.stride] = narrow<T>((to_f32(x[c * r.stride]) - mu) * rs * w + b);
+    float v[V], w[V], b[V];
+    load_values<T, V>(x + c * r.stride, v);
+    if (a.w) load_values<T, V>((const T*)a.w + c, w);
+    if (a.b) load_values<T, V>((const T*)a.b + c, b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (v[e] - mu) * rs * (a.w ? w[e] : 1.f) + (a.b ? b[e] : 0.f);
+    store_values<T, V>(y + c * r.stride, v);
   }
 }
 
-template <typename T, bool MAP>
-__global__ __launch_bounds__(256) void norm_any_dx(const NormArgs a) {
-  __shared__ float red[4][64];
+template <typename T, bool MAP, int V>
+__global__ __launch_bounds__(any_threads(MAP)) void norm_any_dx(const NormArgs a) {
+  __shared__ float red[MAP ? 16 : 1][64];
   const RowAt r = row_at<MAP>(a);
-  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x, S = MAP ? 4 : 256;
+  const int first = MAP ? threadIdx.x >> 6 : threadIdx.x * V, S = MAP ? 16 : 256 * V;
   const T* x = (const T*)a.x + r.base;
   const T* dy = (const T*)a.dy + r.y;
   const float mu = r.ok ? a.mean[r.m] : 0.f, rs = r.ok ? a.rstd[r.m] : 0.f;
   float s1 = 0.f, s2 = 0.f;
+  auto take = [&](int c, float(&h)[V], float(&xh)[V]) __attribute__((always_inline)) {
+    float w[V];
+    load_values<T, V>(dy + c * r.stride, h);
+    load_values<T, V>(x + c * r.stride, xh);
+    if (a.w) load_values<T, V>((const T*)a.w + c, w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (a.w) h[e] *= w[e];
+      xh[e] = (xh[e] - mu) * rs;
+    }
+  };
+#pragma unroll 2
   for (int c = first; c < a.C; c += S) {
-    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
-    const float h = to_f32(dy[c * r.stride]) * w;
-    s1 += h;
-    s2 += h * (to_f32(x[c * r.stride]) - mu) * rs;
+    float h[V], xh[V];
+    take(c, h, xh);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      s1 += h[e];
+      s2 += h[e] * xh[e];
+    }
   }
   s1 = any_sum<MAP>(s1, red) / a.C;
   s2 = any_sum<MAP>(s2, red) / a.C;
   if (!r.ok) return;
   T* dx = (T*)a.dx + r.y;
+#pragma unroll 2
   for (int c = first; c < a.C; c += S) {
-    const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
-    const float xh = (to_f32(x[c * r.stride]) - mu) * rs;
-    dx[c * r.stride] = narrow<T>(rs * (to_f32(dy[c * r.stride]) * w - s1 - xh * s2));
+    float h[V], xh[V];
+    take(c, h, xh);
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] = rs * (h[e] - s1 - xh[e] * s2);
+    store_values<T, V>(dx + c * r.stride, h);
   }
 }
 
-// dw, db of one channel over a share of the rows: tokens, a thread a channel; maps, a block
-template <typename T, bool MAP>
+// dw, db of one channel over a share of the rows: tokens, a thread V channels; maps, a block one
+template <typename T, bool MAP, int V>
 __global__ __launch_bounds__(256) void norm_any_dw(const NormArgs a, int parts) {
   __shared__ float red[4];
   const long long part = blockIdx.y;
-  float sw = 0.f, sb = 0.f;
-  const long long c = MAP ? blockIdx.x : blockIdx.x * 256LL + threadIdx.x;
+  const long long lo = a.M * part / parts, hi = a.M * (part + 1) / parts;
+  float sw[V], sb[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sw[e] = sb[e] = 0.f;
+  const long long c = MAP ? blockIdx.x : (blockIdx.x * 256LL + threadIdx.x) * V;
   if (MAP) {
-    const long long lo = a.M * part / parts, hi = a.M * (part + 1) / parts;
+#pragma unroll 2
     for (long long m = lo + threadIdx.x; m < hi; m += 256) {
       const long long img = m / a.P, p = m - img * a.P;
       const float d = to_f32(((const T*)a.dy)[(img * a.C + c) * a.P + p]);
-      sw += d * (to_f32(((const T*)a.x)[img * a.x_stride + c * a.P + p]) - a.mean[m]) * a.rstd[m];
-      sb += d;
+      sw[0] += d * (to_f32(((const T*)a.x)[img * a.x_stride + c * a.P + p]) - a.mean[m]) * a.rstd[m];
+      sb[0] += d;
     }
-    sw = row_sum<256>(sw, red);
-    sb = row_sum<256>(sb, red);
+    sw[0] = row_sum<256>(sw[0], red);
+    sb[0] = row_sum<256>(sb[0], red);
     if (threadIdx.x != 0) return;
   } else {
     if (c >= a.C) return;
-    const long long lo = a.M * part / parts, hi = a.M * (part + 1) / parts;
+#pragma unroll 4
     for (long long m = lo; m < hi; ++m) {
-      const float d = to_f32(((const T*)a.dy)[m * a.C + c]);
-      sw += d * (to_f32(((const T*)a.x)[m * a.x_stride + c]) - a.mean[m]) * a.rstd[m];
-      sb += d;
+      float d[V], x[V];
+      load_values<T, V>((const T*)a.dy + m * a.C + c, d);
+      load_values<T, V>((const T*)a.x + m * a.x_stride + c, x);
+      const float mu = a.mean[m], rs = a.rstd[m];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        sw[e] += d[e] * (x[e] - mu) * rs;
+        sb[e] += d[e];
+      }
     }
   }
-  a.part[part * a.C + c] = sw;
-  a.part[(parts + part) * a.C + c] = sb;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    a.part[part * a.C + c + e] = sw[e];
+    a.part[(parts + part) * a.C + c + e] = sb[e];
+  }
 }
 
 // dw, db: the blocks' sums [2][blocks][C] in their order; 32 channels by 32 shares of the blocks
@@ -612,31 +659,40 @@ template <typename T> static bool map(const NormArgs& a, bool back, int parts, h
   return true;
 }
 
-template <typename T> static hipError_t forward_t(const NormArgs& a, hipStream_t s) {
-  const bool is_map = a.layout == kMap;
-  if (is_map ? map<T>(a, false, 0, s) : tokens<T>(a, false, 0, s)) return hipGetLastError();
-  if (is_map)
-    norm_any<T, true><<<grid_of(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
+template <typename T, bool MAP, int V>
+static void any_c(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  const dim3 grid = grid_of(MAP ? a.B * ((a.P + 63) / 64) : a.M);
+  if (!back) {
+    norm_any<T, MAP, V><<<grid, any_threads(MAP), 0, s>>>(a);
+    return;
+  }
+  if (a.dx) norm_any_dx<T, MAP, V><<<grid, any_threads(MAP), 0, s>>>(a);
+  if (a.part)
+    norm_any_dw<T, MAP, V>
+        <<<dim3(MAP ? a.C : (a.C + 256 * V - 1) / (256 * V), parts), 256, 0, s>>>(a, parts);
+}
+template <typename T> static void any_c(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (a.layout == kMap)
+    any_c<T, true, 1>(a, back, parts, s);
+  else if (vector_rows<T>(a))
+    any_c<T, false, V>(a, back, parts, s);
   else
-    norm_any<T, false><<<grid_of(a.M), 256, 0, s>>>(a);
+    any_c<T, false, 1>(a, back, parts, s);
+}
+
+template <typename T> static hipError_t forward_t(const NormArgs& a, hipStream_t s) {
+  if (!(a.layout == kMap ? map<T>(a, false, 0, s) : tokens<T>(a, false, 0, s)))
+    any_c<T>(a, false, 0, s);
   return hipGetLastError();
 }
 
 template <typename T> static hipError_t backward_t(const NormArgs& a, int parts, hipStream_t s) {
-  const bool is_map = a.layout == kMap;
-  if (!(is_map ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s))) {
-    if (a.dx) {
-      if (is_map)
-        norm_any_dx<T, true><<<grid_of(a.B * ((a.P + 63) / 64)), 256, 0, s>>>(a);
-      else
-        norm_any_dx<T, false><<<grid_of(a.M), 256, 0, s>>>(a);
-    }
-    if (a.part) {
-      if (is_map)
-        norm_any_dw<T, true><<<dim3(a.C, parts), 256, 0, s>>>(a, parts);
-      else
-        norm_any_dw<T, false><<<dim3((a.C + 255) / 256, parts), 256, 0, s>>>(a, parts);
-    }
+  if (!(a.layout == kMap ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s))) {
+    // these blocks have a channel or some, and share the rows: thousands (maps) or dozens each
+    const long long most = a.M / (a.layout == kMap ? 4096 : 32) + 1;
+    if (parts > most) parts = (int)most;
+    any_c<T>(a, true, parts, s);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.part) return e;

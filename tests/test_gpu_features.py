@@ -508,7 +508,8 @@ def test_layer_norm_tokens(C, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("C", [1, 2, 3, 16, 17, 32, 64, 65, 96, 128, 129, 192, 256, 257, 300])
+@pytest.mark.parametrize("C", [1, 2, 3, 16, 17, 32, 64, 65, 96, 128, 129, 192, 256, 257, 300, 513,
+                               1000])
 def test_layer_norm_map(C, dtype):
     gen = _gen("norm map", C, str(dtype))
     for dims in ((1, 1, 1), (2, 3, 5), (3, 16, 16), (2, 7, 19), (1, 8, 8)):
@@ -522,11 +523,11 @@ def test_layer_norm_map(C, dtype):
 def test_layer_norm_many_rows(dtype):
     """More rows than the blocks that stay: each takes several turns."""
     gen = _gen("norm rows", str(dtype))
-    for M, C in ((70000, 8), (9001, 72), (5003, 1032)):
+    for M, C in ((70000, 8), (9001, 72), (5003, 1032), (301, 9216)):
         x = _rand(gen, M, C, dtype=dtype, shift=0.5)
         _check_norm(x, _rand(gen, C, dtype=dtype), _rand(gen, C, dtype=dtype),
                     _rand(gen, M, C, dtype=dtype), -1)
-    for B, C, H, W in ((8, 20, 96, 101), (9, 70, 88, 88)):
+    for B, C, H, W in ((8, 20, 96, 101), (9, 70, 88, 88), (3, 270, 48, 57)):
         x = _rand(gen, B, C, H, W, dtype=dtype, shift=0.5)
         _check_norm(x, _rand(gen, C, dtype=dtype), _rand(gen, C, dtype=dtype),
                     _rand(gen, B, C, H, W, dtype=dtype), 1)
