@@ -34,7 +34,28 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red)
   return v;
 }
 
-template <typename T, int TPR, int NV, int V>
+// V values of a row, of which `have` exist (WHOLE: all or none do, and the caller has looked): rows of
+// odd lengths are read in 16-byte pieces too, from any address.
+template <typename T, int V, bool WHOLE>
+__device__ __forceinline__ void load_row(const T* p, int have, float (&v)[V]) {
+  if constexpr (WHOLE) {
+    load_values<T, V>(p, v);
+  } else {
+    as_floats<T, V>(have >= V ? load16(p) : load_some(p, have), v);
+  }
+}
+template <typename T, int V, bool WHOLE>
+__device__ __forceinline__ void store_row(T* p, int have, const float (&v)[V]) {
+  if (WHOLE || have >= V) {
+    store_values<T, V>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < have) p[e] = narrow<T>(v[e]);
+  }
+}
+
+template <typename T, int TPR, int NV, int V, bool WHOLE>
 __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
   __shared__ float red[4];
   constexpr int RPB = 256 / TPR;
@@ -48,7 +69,7 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
   for (int k = 0; k < NV; ++k) {
     const int c = (k * TPR + t) * V;
     if (c < a.C) {
-      load_values<T, V>(x + c, v[k]);
+      load_row<T, V, WHOLE>(x + c, a.C - c, v[k]);
 #pragma unroll
       for (int e = 0; e < V; ++e) s += v[k][e];
     }
@@ -61,7 +82,7 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         v[k][e] -= mu;
-        s += v[k][e] * v[k][e];
+        if (WHOLE || (k * TPR + t) * V + e < a.C) s += v[k][e] * v[k][e];
       }
   const float r = 1.f / sqrtf(row_sum<TPR>(s, red) / a.C + a.eps);
   if (!row) return;
@@ -75,16 +96,16 @@ __global__ __launch_bounds__(256) void norm_tokens(const NormArgs a) {
     const int c = (k * TPR + t) * V;
     if (c < a.C) {
       float w[V], b[V];
-      if (a.w) load_values<T, V>((const T*)a.w + c, w);
-      if (a.b) load_values<T, V>((const T*)a.b + c, b);
+      if (a.w) load_row<T, V, WHOLE>((const T*)a.w + c, a.C - c, w);
+      if (a.b) load_row<T, V, WHOLE>((const T*)a.b + c, a.C - c, b);
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * r * (a.w ? w[e] : 1.f) + (a.b ? b[e] : 0.f);
-      store_values<T, V>(y + c, v[k]);
+      store_row<T, V, WHOLE>(y + c, a.C - c, v[k]);
     }
   }
 }
 
-template <typename T, int TPR, int NV, int V>
+template <typename T, int TPR, int NV, int V, bool WHOLE>
 __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
   extern __shared__ float lds[];
   constexpr int RPB = 256 / TPR;
@@ -99,7 +120,7 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
       w[k][e] = 1.f;
       dw[k][e] = db[k][e] = 0.f;
     }
-    if (a.w && c < a.C) load_values<T, V>((const T*)a.w + c, w[k]);
+    if (a.w && c < a.C) load_row<T, V, WHOLE>((const T*)a.w + c, a.C - c, w[k]);
   }
   for (long long m0 = (long long)blockIdx.x * RPB; m0 < a.M; m0 += (long long)gridDim.x * RPB) {
     const long long m = m0 + threadIdx.x / TPR;
@@ -113,11 +134,11 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + t) * V;
       if (row && c < a.C) {
-        load_values<T, V>(x + c, xh[k]);
-        load_values<T, V>(dy + c, h[k]);
+        load_row<T, V, WHOLE>(x + c, a.C - c, xh[k]);
+        load_row<T, V, WHOLE>(dy + c, a.C - c, h[k]);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          xh[k][e] = (xh[k][e] - mu) * r;
+          xh[k][e] = WHOLE || c + e < a.C ? (xh[k][e] - mu) * r : 0.f;
           dw[k][e] += h[k][e] * xh[k][e];
           db[k][e] += h[k][e];
           h[k][e] *= w[k][e];
@@ -135,7 +156,7 @@ __global__ __launch_bounds__(256) void norm_tokens_backward(const NormArgs a) {
         if (c < a.C) {
 #pragma unroll
           for (int e = 0; e < V; ++e) h[k][e] = r * (h[k][e] - s1 - xh[k][e] * s2);
-          store_values<T, V>((T*)a.dx + m * a.C + c, h[k]);
+          store_row<T, V, WHOLE>((T*)a.dx + m * a.C + c, a.C - c, h[k]);
         }
       }
     }
@@ -197,24 +218,23 @@ __device__ __forceinline__ void pixel_sum(float (&v)[PV], float (*red)[64 * PV])
   }
 }
 // Sums over a wave of N values a lane (N a power of two): halves are exchanged, so N + 6 shuffles do
-// what 6 N would.  Lane l returns the sum of value l / (64 / N).
-template <int N> __device__ __forceinline__ float fold_lanes(float (&v)[N]) {
-  const int l = threadIdx.x & 63;
-  int bit = 32;
+// what 6 N would.  Lane l returns the sum of value l / (64 / N).  (Steps by recursion: with a step
+// count that the compiler does not see through, the values move to LDS.)
+template <int N, int BIT, int M> __device__ __forceinline__ float fold_from(float (&v)[M]) {
+  if constexpr (N > 1) {
+    const bool up = threadIdx.x & BIT;
 #pragma unroll
-  for (int n = N; n > 1; n /= 2, bit /= 2) {
-    const bool up = l & bit;
-#pragma unroll
-    for (int k = 0; k < N / 2; ++k)
-      if (k < n / 2) {
-        const float give = up ? v[k] : v[k + n / 2], keep = up ? v[k + n / 2] : v[k];
-        v[k] = keep + __shfl_xor(give, bit, 64);
-      }
+    for (int k = 0; k < N / 2; ++k) {
+      const float give = up ? v[k] : v[k + N / 2], keep = up ? v[k + N / 2] : v[k];
+      v[k] = keep + __shfl_xor(give, BIT, 64);
+    }
+    return fold_from<N / 2, BIT / 2>(v);
+  } else {
+    return lanes_sum<2 * BIT>(v[0]);
   }
-  float s = v[0];
-#pragma unroll
-  for (; bit > 0; bit /= 2) s += __shfl_xor(s, bit, 64);
-  return s;
+}
+template <int N> __device__ __forceinline__ float fold_lanes(float (&v)[N]) {
+  return fold_from<N, 32>(v);
 }
 template <typename T, int PV>
 __device__ __forceinline__ void load_pixels(const T* p, uint32_t at, bool ok, float (&v)[PV]) {
@@ -224,6 +244,17 @@ __device__ __forceinline__ void load_pixels(const T* p, uint32_t at, bool ok, fl
   if (ok) o = *(const Pack<T, PV>*)(p + at);
 #pragma unroll
   for (int e = 0; e < PV; ++e) v[e] = to_f32(o.v[e]);
+}
+// A wave's channels g, g + G, ...: lane k holds channel k's value (`otherwise` where there is none),
+// so that one load fetches all; a load a channel would be waited for one after the other.
+template <typename T>
+__device__ __forceinline__ float wave_channels(const void* p, int g, int G, int C,
+                                               float otherwise) {
+  const int c = (int)(threadIdx.x & 63) * G + g;
+  return p && c < C ? to_f32(((const T*)p)[c]) : otherwise;
+}
+__device__ __forceinline__ float channel_of(float held, int k) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), k));
 }
 template <typename T, int PV>
 __device__ __forceinline__ void store_pixels(T* p, uint32_t at, const float (&v)[PV]) {
@@ -244,6 +275,8 @@ __global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
   const uint32_t p = (uint32_t)((id % tiles * 64 + l) * PV);
   const bool ok = p < P && img < a.B;
   const T* x = (const T*)a.x + img * a.x_stride;
+  const float weights = wave_channels<T>(a.w, g, G, a.C, 1.f);
+  const float biases = wave_channels<T>(a.b, g, G, a.C, 0.f);
   float v[NC][PV], s[PV], r[PV], mu[PV];
 #pragma unroll
   for (int e = 0; e < PV; ++e) s[e] = 0.f;
@@ -283,8 +316,7 @@ __global__ __launch_bounds__(64 * G) void norm_map(const NormArgs a) {
   for (int k = 0; k < NC; ++k) {
     const int c = k * G + g;
     if (c < a.C) {
-      const float w = a.w ? to_f32(((const T*)a.w)[c]) : 1.f;
-      const float b = a.b ? to_f32(((const T*)a.b)[c]) : 0.f;
+      const float w = channel_of(weights, k), b = channel_of(biases, k);
 #pragma unroll
       for (int e = 0; e < PV; ++e) v[k][e] = v[k][e] * r[e] * w + b;
       store_pixels<T, PV>(y, c * P + p, v[k]);
@@ -299,6 +331,7 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
   const int g = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);  // channels: uniform
   const uint32_t P = (uint32_t)a.P;  // (an image's offsets fit 32 bits)
   const long long tiles = (a.P + 64 * PV - 1) / (64 * PV);
+  const float weights = wave_channels<T>(a.w, g, G, a.C, 1.f);
   float dw[NC], db[NC];
 #pragma unroll
   for (int k = 0; k < NC; ++k) dw[k] = db[k] = 0.f;
@@ -324,7 +357,7 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
 #pragma unroll
     for (int k = 0; k < NC; ++k)
       if (k * G + g < a.C) {
-        const float w = a.w ? to_f32(((const T*)a.w)[k * G + g]) : 1.f;
+        const float w = channel_of(weights, k);
 #pragma unroll
         for (int e = 0; e < PV; ++e) {
           xh[k][e] = (xh[k][e] - mu[e]) * r[e];
@@ -579,8 +612,10 @@ template <typename T> static bool vector_rows(const NormArgs& a) {
 }
 
 // Blocks of the backward pass, each with a row of partial sums: tokens, four of 256 threads that stay
-// on each of 256 CUs; maps, twice that (a tile of 64 pixels each up to 131072 pixels: with 1024
-// blocks the l4 map's 1344 tiles took two turns, 24 us instead of 11).
+// on each of 256 CUs, fewer where a row takes a whole block and they would have less than eight (4096 x
+// 8192 bf16: 85 us with 1024 blocks, whose sums are as much traffic as the rows, 59 with 512; 16383 x
+// 2048: 46 and 55); maps, twice that (a tile of 64 pixels each up to 131072 pixels: with 1024 blocks
+// the l4 map's 1344 tiles took two turns, 24 us instead of 11).
 constexpr int kBlocksTokens = 1024, kBlocksMaps = 2048;
 
 int norm_parts(int layout, long long B, long long P, int C, int dtype) {
@@ -590,42 +625,40 @@ int norm_parts(int layout, long long B, long long P, int C, int dtype) {
     rows = 64;
   } else {
     const int V = dtype == 0 ? 4 : 8;
-    const RowPlan p = row_plan(C, C % V == 0 ? V : 1);
+    const RowPlan p = row_plan(C, V);
     if (p.tpr) rows = 256 / p.tpr;
   }
   const long long n = (M + rows - 1) / rows;
-  const long long most = layout == kMap ? kBlocksMaps : kBlocksTokens;
+  long long most = layout == kMap ? kBlocksMaps : kBlocksTokens;
+  if (layout == kTokens && rows == 1 && n / 8 < most) most = n / 8 > 256 ? n / 8 : 256;
   return (int)(n < most ? n : most);
 }
 
-template <typename T, int TPR, int V, int NV = 1>
+template <typename T, int TPR, bool WHOLE, int NV = 1>
 static void tokens_nv(const NormArgs& a, int nv, bool back, int parts, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
   if constexpr (NV * V <= most_values(TPR)) {
-    if (nv != NV) return tokens_nv<T, TPR, V, 2 * NV>(a, nv, back, parts, s);
+    if (nv != NV) return tokens_nv<T, TPR, WHOLE, 2 * NV>(a, nv, back, parts, s);
     const dim3 grid = grid_of((a.M + 256 / TPR - 1) / (256 / TPR));
     const size_t lds = 16 + (TPR < 256 ? 8 * sizeof(float) * a.C : 0);
     if (back)
-      norm_tokens_backward<T, TPR, NV, V><<<parts, 256, lds, s>>>(a);
+      norm_tokens_backward<T, TPR, NV, V, WHOLE><<<parts, 256, lds, s>>>(a);
     else
-      norm_tokens<T, TPR, NV, V><<<grid, 256, 0, s>>>(a);
+      norm_tokens<T, TPR, NV, V, WHOLE><<<grid, 256, 0, s>>>(a);
   }
 }
-
-template <typename T> static bool tokens(const NormArgs& a, bool back, int parts, hipStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = vector_rows<T>(a);
-  const RowPlan p = row_plan(a.C, vec ? V : 1);
+template <typename T, bool WHOLE>
+static bool tokens_whole(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  const RowPlan p = row_plan(a.C, 16 / (int)sizeof(T));
   if (p.tpr == 0) return false;
-  if (vec) {
-    p.tpr == 8    ? tokens_nv<T, 8, V>(a, p.nv, back, parts, s)
-    : p.tpr == 64 ? tokens_nv<T, 64, V>(a, p.nv, back, parts, s)
-                  : tokens_nv<T, 256, V>(a, p.nv, back, parts, s);
-  } else {
-    p.tpr == 8    ? tokens_nv<T, 8, 1>(a, p.nv, back, parts, s)
-    : p.tpr == 64 ? tokens_nv<T, 64, 1>(a, p.nv, back, parts, s)
-                  : tokens_nv<T, 256, 1>(a, p.nv, back, parts, s);
-  }
+  p.tpr == 8    ? tokens_nv<T, 8, WHOLE>(a, p.nv, back, parts, s)
+  : p.tpr == 64 ? tokens_nv<T, 64, WHOLE>(a, p.nv, back, parts, s)
+                : tokens_nv<T, 256, WHOLE>(a, p.nv, back, parts, s);
   return true;
+}
+template <typename T> static bool tokens(const NormArgs& a, bool back, int parts, hipStream_t s) {
+  return vector_rows<T>(a) ? tokens_whole<T, true>(a, back, parts, s)
+                           : tokens_whole<T, false>(a, back, parts, s);
 }
 
 template <typename T, int PV>
@@ -634,19 +667,27 @@ static void map_pv(const NormArgs& a, bool back, int parts, hipStream_t s) {
 #define NORM_MAP(G, NC)                                                    \
   (back ? norm_map_backward<T, G, NC, PV><<<parts, 64 * G, 0, s>>>(a)      \
         : norm_map<T, G, NC, PV><<<grid, 64 * G, 0, s>>>(a))
-  // eight channels a thread where eight waves hold them: the backward pass keeps five values a
-  // channel, and more of them leave fewer waves on a CU
-  a.C <= 8     ? NORM_MAP(1, 8)
-  : a.C <= 32  ? NORM_MAP(4, 8)
-  : a.C <= 64  ? NORM_MAP(8, 8)
-  : a.C <= 128 ? NORM_MAP(8, 16)
-               : NORM_MAP(8, 32);
+  // eight channels a thread where sixteen waves hold them: the backward pass keeps five values a
+  // channel, and more of them leave fewer waves on a CU (16 x 128 x 7168 bf16 by 8 waves 92 us, by 16
+  // 47; 16 x 256 x 7168 373 and 121)
+  if (a.C <= 8) {
+    NORM_MAP(1, 8);
+  } else if (a.C <= 32) {
+    NORM_MAP(4, 8);
+  } else if (a.C <= 64) {
+    NORM_MAP(8, 8);
+  } else if (a.C <= 128) {
+    NORM_MAP(16, 8);
+  } else if constexpr (PV == 1) {
+    NORM_MAP(16, 16);
+  } else {  // (forward alone: the backward pass of more channels would not fit the registers)
+    norm_map<T, 16, 16, PV><<<grid, 1024, 0, s>>>(a);
+  }
 #undef NORM_MAP
 }
 template <typename T> static bool map(const NormArgs& a, bool back, int parts, hipStream_t s) {
   if (a.C > 256 || a.C * a.P >= 1LL << 30) return false;
   if constexpr (sizeof(T) == 2) {
-    // (the backward pass of more channels would not fit the registers with pairs)
     bool pairs = (a.C <= 128 || !back) && a.P % 2 == 0 && (a.B == 1 || a.x_stride % 2 == 0);
     for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx})
       pairs = pairs && aligned_to(p, 4);
