@@ -208,9 +208,12 @@ template <typename T> static hipError_t rotary_t(RotaryArgs a, hipStream_t strea
                      every({a.xs_b, a.xs_n, a.xs_h, a.ys_b, a.ys_n, a.ys_h}, V);
     const int v = vec ? V : 1;
     const long long units = (a.R + v - 1) / v + (a.D - 2 * a.R + 2 * v - 1) / (2 * v);
-    // Heads in one thread share its angles, as long as the threads fill the card: 2 x 9603 x 24 x
-    // 128 bf16 took 57 us with 150 or 300 thousand threads, 54.5 with 600.
-    long long groups = (512LL << 10) / (a.B * a.N * units) + 1;
+    // Heads in one thread share its angles, which bound calls whose rows come from the cache, as long
+    // as the threads fill the card (2 x 4096 x 8 x 128 bf16: 10 us with 128 thousand threads, 15 with
+    // 512); rows from memory want more loads under way (2 x 9603 x 24 x 128: 57 and 54 us).
+    const long long bytes = 2 * a.B * a.N * a.H * a.D * (long long)sizeof(T);
+    const long long threads = bytes > (128LL << 20) ? 512LL << 10 : 128LL << 10;
+    long long groups = threads / (a.B * a.N * units) + 1;
     if (groups > a.H) groups = a.H;
     a.heads_each = (int)((a.H + groups - 1) / groups);
     a.head_groups = (a.H + a.heads_each - 1) / a.heads_each;
