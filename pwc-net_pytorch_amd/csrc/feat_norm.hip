@@ -11,8 +11,8 @@
 // their order: no atomics, the same sums each time.
 //
 // Measured: 16383 x 2048 bf16 tokens 29 us forward (4.6 TB/s) and 46 backward (4.4; a 1 GiB copy does
-// 5.1), a block a row; the 8 x 32 x 96 x 112 fp32 map 7.6 and 11.5 us, 64 pixels a block, and 4 us
-// for the sums over blocks.
+// 5.1), a block a row; the 8 x 32 x 96 x 112 fp32 map 6.5 and 9.6 us, 64 pixels a block, and 4 us for
+// the sums over blocks.
 #include "feat_common.cuh"
 #include "feat_norm.cuh"
 
@@ -615,7 +615,7 @@ template <typename T> static bool vector_rows(const NormArgs& a) {
 // on each of 256 CUs, fewer where a row takes a whole block and they would have less than eight (4096 x
 // 8192 bf16: 85 us with 1024 blocks, whose sums are as much traffic as the rows, 59 with 512; 16383 x
 // 2048: 46 and 55); maps, twice that (a tile of 64 pixels each up to 131072 pixels: with 1024 blocks
-// the l4 map's 1344 tiles took two turns, 24 us instead of 11).
+// the l4 map's 1344 tiles took two turns and twice the time).
 constexpr int kBlocksTokens = 1024, kBlocksMaps = 2048;
 
 int norm_parts(int layout, long long B, long long P, int C, int dtype) {
