@@ -806,6 +806,59 @@ def test_other_stream_and_captured():
         step(data[0][0][0].clone().requires_grad_(True), data[0][0][1])
 
 
+def test_every_path_captured():
+    """Products in parts, of few tokens, with rows laid out first and with two-part gradients, and
+    norms of long rows: captured, and replayed on new inputs between eager calls."""
+    import pwcnet_amd as P
+    bf, hf = torch.bfloat16, torch.float16
+    cases = [("gelu", False, (100, 2048), 520, bf), ("silu", True, (7, 1024), 200, bf),
+             ("tanh", False, (301, 511), 509, bf), ("gelu", False, (3001, 517), 1021, bf),
+             ("none", False, (64, 4096), 1200, hf), ("silu", True, (2, 96, 37, 53), 385, hf),
+             ("norm", None, (301, 9216), 0, bf), ("norm", None, (2, 270, 21, 19), 0, hf)]
+
+    def step(kind, gated, leaves, g):
+        dim = -1 if leaves[0].dim() == 2 else 1
+        if kind == "norm":
+            y = P.layer_norm(*leaves, channel_dim=dim)
+        elif gated:
+            y = P.gated_linear(*leaves, activation=kind, channel_dim=dim)
+        else:
+            y = P.linear(*leaves, activation=kind, channel_dim=dim)
+        return [y.detach(), *torch.autograd.grad(y, leaves, g)]
+
+    for kind, gated, dims, O, dtype in cases:
+        if kind == "norm":
+            gen = _gen("captured", dims)
+            C = dims[-1] if len(dims) == 2 else dims[1]
+            made = [(_rand(gen, *dims, dtype=dtype), _rand(gen, C, dtype=dtype),
+                     _rand(gen, C, dtype=dtype), _rand(gen, *dims, dtype=dtype)) for _ in range(2)]
+        else:
+            made = []
+            for n in range(2):
+                is_map = len(dims) == 4
+                lead = (dims[0], *dims[2:]) if is_map else dims[:1]
+                x, w, b, _, g = _product_case(is_map, lead, dims[1], O, dtype, kind, True, False,
+                                              gated, seed=n)
+                made.append((x, w, b, g))
+        want = [step(kind, gated, [t.clone().requires_grad_(True) for t in m[:3]], m[3])
+                for m in made]
+        held = [t.clone().requires_grad_(True) for t in made[0][:3]]
+        grad = made[0][3].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(kind, gated, held, grad)
+        for turn in (1, 0, 1, 1):
+            with torch.no_grad():
+                for to, t in zip((*held, grad), made[turn]):
+                    to.copy_(t)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[turn])), (kind, dims, turn)
+            again = step(kind, gated, [t.clone().requires_grad_(True) for t in made[0][:3]],
+                         made[0][3])
+            assert all(torch.equal(a, b) for a, b in zip(again, want[0])), (kind, dims, turn)
+
+
 def test_block_against_formula():
     """norm, gated, project with the skip, rotary: a run of them against 64 bits, with gradients.
 
