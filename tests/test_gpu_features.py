@@ -1141,3 +1141,91 @@ def test_dispatch_modes_see_single_nodes():
     with Names():
         got = P.linear(x, w, activation="gelu", channel_dim=-1)
     assert torch.equal(got, want) and any("pwcnet.linear" in n for n in seen)
+
+
+def test_rotary_entry_turns_in_place():
+    """y == x with equal strides; a second call with `inverse` turns back."""
+    import ctypes
+    import pwcnet_amd as P
+    from pwcnet_amd import _lib
+    lib = _lib.load()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        for shape, perm, pairs in (((2, 9, 6, 64), (0, 1, 2, 3), 24),
+                                   ((2, 6, 20, 35), (0, 3, 1, 2), 10)):
+            base = _rand(_gen("in place", str(dtype), shape), *shape, dtype=dtype)
+            x = base.permute(*perm)
+            inv, axis = P.rotary_frequencies((pairs,), device=DEV)
+            want = P.rotary(x, inv, axis, grid=(x.shape[1],))
+            s = _lib.RotaryShape(B=x.shape[0], N=x.shape[1], heads=x.shape[2], D=x.shape[3],
+                                 pairs=pairs, axes=1)
+            s.x_stride[:] = s.y_stride[:] = x.stride()
+            s.grid[:] = [x.shape[1], 0, 0, 0]
+            _lib.check(lib.pwc_rotary(x.data_ptr(), x.data_ptr(), None, inv.data_ptr(),
+                                      axis.data_ptr(), ctypes.byref(s), 0, code, stream), "rotary")
+            assert torch.equal(x, want)
+            back = P.features.rotary_forward(want, inv, axis, grid=(x.shape[1],), inverse=True)
+            _lib.check(lib.pwc_rotary(x.data_ptr(), x.data_ptr(), None, inv.data_ptr(),
+                                      axis.data_ptr(), ctypes.byref(s), 1, code, stream), "rotary")
+            assert torch.equal(x, back)
+
+
+@pytest.mark.parametrize("layout,B,P_,K,O,gated,act", [
+    (1, 1, 100, 2048, 520, 0, 6), (1, 1, 7, 1024, 131, 1, 5), (1, 1, 301, 511, 509, 0, 4),
+    (1, 1, 3001, 517, 1021, 1, 5), (0, 2, 1961, 96, 385, 1, 6), (0, 3, 35, 33, 17, 0, 0),
+    (1, 1, 64, 4096, 1200, 0, 0), (0, 5, 1, 40, 24, 1, 5)])
+def test_entries_stay_in_their_buffers(layout, B, P_, K, O, gated, act):
+    """Outputs and a workspace of exactly the asked size stand between values that stay as they were;
+    each subset of the gradients gives the full call's."""
+    import ctypes
+    from pwcnet_amd import _lib
+    lib = _lib.load()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    gen = _gen("buffers", layout, B, P_, K, O, gated)
+    rows, M = O * (2 if gated else 1), B * P_
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        x, w = (_rand(gen, M, K, dtype=dtype), _rand(gen, rows, K, dtype=dtype, scale=K ** -0.5))
+        b, dy = _rand(gen, rows, dtype=dtype), _rand(gen, M, O, dtype=dtype)
+        stride = K if layout == 1 else K * P_
+        guard = 4096
+
+        def buffer(values, size):
+            buf = torch.full((values * size + 2 * guard,), 0x5A, dtype=torch.uint8, device=DEV)
+            return buf, buf.data_ptr() + guard
+
+        def kept(buf, used):
+            return bool((buf[:guard] == 0x5A).all()) and bool((buf[guard + used:] == 0x5A).all())
+
+        size = dtype.itemsize
+        name = "gated_linear" if gated else "linear"
+        asked = getattr(lib, f"pwc_{name}_forward_workspace_size")(
+            x.data_ptr(), w.data_ptr(), layout, B, P_, K, O, stride, code)
+        y, at = buffer(M * O, size)
+        ws, ws_at = buffer(asked, 1)
+        middle = () if gated else (None,)
+        _lib.check(getattr(lib, f"pwc_{name}_forward")(
+            x.data_ptr(), w.data_ptr(), b.data_ptr(), *middle, at, layout, B, P_, K, O, stride, act,
+            0.1, code, ws_at, asked, stream), name)
+        torch.cuda.synchronize()
+        assert kept(y, M * O * size) and kept(ws, asked)
+        back_size = getattr(lib, f"pwc_{name}_backward_workspace_size")
+        asked = back_size(x.data_ptr(), w.data_ptr(), dy.data_ptr(), layout, B, P_, K, O, stride,
+                          *(() if gated else (act,)), code)
+        full = None
+        for which in (7, 1, 2, 4, 3, 5, 6):
+            outs = [buffer(n, size) for n in (M * K, rows * K, rows)]
+            ws, ws_at = buffer(asked, 1)
+            _lib.check(getattr(lib, f"pwc_{name}_backward")(
+                x.data_ptr(), w.data_ptr(), b.data_ptr(), dy.data_ptr(),
+                *(o[1] if which >> k & 1 else None for k, o in enumerate(outs)), layout, B, P_, K, O,
+                stride, act, 0.1, code, ws_at, asked, stream), name)
+            torch.cuda.synchronize()
+            assert kept(ws, asked)
+            for o, n in zip(outs, (M * K, rows * K, rows)):
+                assert kept(o[0], n * size)
+            full = full or [o[0].clone() for o in outs]
+            for k, o in enumerate(outs):
+                if which >> k & 1:
+                    assert torch.equal(o[0], full[k]), (which, k)
+                else:
+                    assert bool((o[0] == 0x5A).all())
