@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/pwc_hotpath.h"
@@ -77,6 +78,9 @@ int dtype_code(at::ScalarType t) {
 }
 
 void check(const char* what, const Tensor& x, std::initializer_list<const Tensor*> others) {
+  // torch.jit.trace would record the outputs' allocation and not the launch that fills them
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what,
+              ": not seen by torch.jit.trace: call torch.ops.pwcnet or pwcnet_amd's functions");
   auto one = [&](const Tensor& t) {
     TORCH_CHECK(t.is_cuda(), what, ": pwcnet_amd runs on HIP devices only (got a ", t.device(),
                 " tensor); there is no CPU implementation");

@@ -156,6 +156,7 @@ class CostVolumeLayer(nn.Module):
 def _traced(x):
     """Tracers see one opaque torch.ops.pwcnet node; eager calls go straight to the kernels."""
     return (type(x) not in (torch.Tensor, nn.Parameter) or torch.compiler.is_compiling()
+            or torch._C._get_tracing_state() is not None  # torch.jit.trace
             or torch._C._len_torch_dispatch_stack() > 0)
 
 
@@ -171,6 +172,8 @@ def rotary(x, inv_freq, axis, positions=None, grid=None, origin=None, interleave
     """x [B, N, heads, D] with its channel pairs turned by position[axis[j]] * inv_freq[j]; see
     ``features.rotary_forward``.  ``inv_freq`` and ``axis`` come from ``rotary_frequencies``."""
     if _traced(x):
+        if torch._C._get_tracing_state() is not None:  # its sizes are no ints: they stay as traced
+            grid, origin = (v and [int(n) for n in v] for v in (grid, origin))
         grid = None if grid is None else list(grid)
         origin = None if origin is None else list(origin)
         return _library.rotary(x, inv_freq, axis, positions, grid, origin, interleaved, False)

@@ -1,0 +1,49 @@
+"""GPU: the feature operators called in other ways than eagerly on plain tensors, and at values and
+sizes where a kernel's arithmetic could leave its formula."""
+import math
+import zlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _gen(*parts):
+    return torch.Generator().manual_seed(zlib.crc32(repr(parts).encode()))
+
+
+def _rand(gen, *shape, dtype=torch.float32, scale=1.0, shift=0.0):
+    return (torch.randn(*shape, generator=gen) * scale + shift).to(dtype).to(DEV)
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ------------------------------------------------------------------------------- torch.jit.trace
+@pytest.mark.filterwarnings("ignore")
+def test_jit_trace_replays():
+    """Traced operators, a block and rotary positions give the eager values and gradients on new
+    inputs, with memory in between that an unfilled output would show."""
+    import pwcnet_amd as P
+    gen = _gen("trace")
+    w, b = _rand(gen, 24, 16), _rand(gen, 24)
+    n = _rand(gen, 16)
+    calls = [lambda x: P.layer_norm(x, n, n), lambda x: P.linear(x, w, b, activation="gelu"),
+             lambda x: P.gated_linear(x, w, b), P.RotaryPosition((4, 4)).to(DEV),
+             P.FeatureBlock(16).to(DEV)]
+    for call in calls:
+        traced = torch.jit.trace(call, _rand(gen, 2, 16, 9, 11))
+        for batch in (2, 3):
+            x = _rand(gen, batch, 16, 9, 11).requires_grad_(True)
+            want = call(x)
+            g = _rand(gen, *want.shape)
+            keep = torch.full((4, *want.shape), float("nan"), device=DEV)
+            del keep
+            got = traced(x)
+            assert torch.equal(got, want)
+            assert torch.equal(torch.autograd.grad(got, x, g)[0],
+                               torch.autograd.grad(want, x, g)[0])
