@@ -77,11 +77,22 @@ int dtype_code(at::ScalarType t) {
        : t == at::kBFloat16 ? PWC_DTYPE_BF16 : -1;
 }
 
+// No tensor that stands for others (torch.func's, a subclass with a dispatch of its own): it has no
+// memory, or not the values that its caller means.
+void plain(const char* what, const Tensor& t) {
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched,
+                                         c10::DispatchKey::FuncTorchGradWrapper,
+                                         c10::DispatchKey::Functionalize, c10::DispatchKey::Python});
+  TORCH_CHECK_TYPE(!t.key_set().has_any(wrapped), what,
+                   ": plain tensors only: call torch.ops.pwcnet or pwcnet_amd's functions");
+}
+
 void check(const char* what, const Tensor& x, std::initializer_list<const Tensor*> others) {
   // torch.jit.trace would record the outputs' allocation and not the launch that fills them
   TORCH_CHECK(!torch::jit::tracer::isTracing(), what,
               ": not seen by torch.jit.trace: call torch.ops.pwcnet or pwcnet_amd's functions");
   auto one = [&](const Tensor& t) {
+    plain(what, t);
     TORCH_CHECK(t.is_cuda(), what, ": pwcnet_amd runs on HIP devices only (got a ", t.device(),
                 " tensor); there is no CPU implementation");
     TORCH_CHECK(t.device() == x.device(), what, ": tensors on different devices (", t.device(),
@@ -258,6 +269,8 @@ Tensor rotary_forward(const Tensor& x, const Tensor& inv_freq, const Tensor& axi
                       bool interleaved, bool inverse) {
   const char* what = "rotary";
   check(what, x, {});
+  for (const Tensor* t : {&inv_freq, &axis, &positions})
+    if (t->defined()) plain(what, *t);
   TORCH_CHECK_VALUE(x.dim() == 4, what, ": expected [B, N, heads, D], got shape ", x.sizes());
   TORCH_CHECK_TYPE(inv_freq.scalar_type() == at::kDouble && axis.scalar_type() == at::kInt, what,
                    ": inv_freq is fp64 and axis int32, got ", inv_freq.scalar_type(), " and ",

@@ -153,17 +153,27 @@ class CostVolumeLayer(nn.Module):
 # ---------------------------------------------------------------------------------------
 # feature operators (features.py): functions and modules
 # ---------------------------------------------------------------------------------------
-def _traced(x):
-    """Tracers see one opaque torch.ops.pwcnet node; eager calls go straight to the kernels."""
-    return (type(x) not in (torch.Tensor, nn.Parameter) or torch.compiler.is_compiling()
-            or torch._C._get_tracing_state() is not None  # torch.jit.trace
-            or torch._C._len_torch_dispatch_stack() > 0)
+def _traced(*tensors):
+    """Tracers, subclasses and torch.func see one opaque torch.ops.pwcnet node; eager calls go
+    straight to the kernels."""
+    if torch.compiler.is_compiling():
+        return True
+    functorch = torch._C._functorch
+    if functorch.peek_interpreter_stack() is not None:
+        # (a node without a forward-mode formula would give zeros)
+        if any(i.key() == functorch.TransformType.Jvp for i in functorch.get_interpreter_stack()):
+            raise RuntimeError("pwcnet_amd: the feature operators have no forward-mode derivatives")
+        return True
+    return (torch._C._get_tracing_state() is not None  # torch.jit.trace
+            or torch._C._len_torch_dispatch_stack() > 0
+            or any(t is not None and type(t) not in (torch.Tensor, nn.Parameter)
+                   for t in tensors))
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=1):
     """(x - mean) / sqrt(var + eps) * weight + bias over the channels of each pixel of a map
     [B, C, *spatial] (``channel_dim=1``) or of each token [..., C] (``channel_dim=-1``)."""
-    if _traced(x):
+    if _traced(x, weight, bias):
         return _library.layer_norm(x, weight, bias, eps, channel_dim)[0]
     return _features._ext.layer_norm(x, weight, bias, eps, channel_dim)
 
@@ -171,7 +181,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, channel_dim=1):
 def rotary(x, inv_freq, axis, positions=None, grid=None, origin=None, interleaved=False):
     """x [B, N, heads, D] with its channel pairs turned by position[axis[j]] * inv_freq[j]; see
     ``features.rotary_forward``.  ``inv_freq`` and ``axis`` come from ``rotary_frequencies``."""
-    if _traced(x):
+    if _traced(x, inv_freq, axis, positions):
         if torch._C._get_tracing_state() is not None:  # its sizes are no ints: they stay as traced
             grid, origin = (v and [int(n) for n in v] for v in (grid, origin))
         grid = None if grid is None else list(grid)
@@ -185,7 +195,7 @@ def linear(x, weight, bias=None, residual=None, activation="none", negative_slop
     """act(x W^T + bias) + residual over x's channels: on maps a 1x1 convolution with its
     activation and skip in one kernel.  ``activation``: one of ``features.ACTIVATIONS``."""
     activation = activation or "none"
-    if _traced(x):
+    if _traced(x, weight, bias, residual):
         return _library.linear(x, weight, bias, residual, activation, negative_slope, channel_dim)
     return _features._ext.linear(x, weight, bias, residual, activation, negative_slope,
                                  channel_dim)
@@ -195,7 +205,7 @@ def gated_linear(x, weight, bias=None, activation="silu", negative_slope=0.1, ch
     """act(x Wg^T + bg) * (x Wu^T + bu) over x's channels, weight = [Wg; Wu]: both projections,
     the activation and the product in one kernel."""
     activation = activation or "none"
-    if _traced(x):
+    if _traced(x, weight, bias):
         return _library.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
     return _features._ext.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
 

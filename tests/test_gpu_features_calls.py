@@ -47,3 +47,30 @@ def test_jit_trace_replays():
             assert torch.equal(got, want)
             assert torch.equal(torch.autograd.grad(got, x, g)[0],
                                torch.autograd.grad(want, x, g)[0])
+
+
+# ------------------------------------------------------------------------------- torch.func
+@pytest.mark.filterwarnings("ignore")
+def test_vmap_gives_each_samples_values():
+    """vmap over samples, over weights and with gradients from outside: the eager results, sample by
+    sample; torch.func.grad is refused, as for every node of the package."""
+    import pwcnet_amd as P
+    gen = _gen("vmap")
+    x, w = _rand(gen, 3, 40, 16), _rand(gen, 3, 24, 16)
+    inv, axis = P.rotary_frequencies((4, 4), device=DEV)
+    at = torch.randint(0, 99, (40, 2), generator=gen).to(DEV)
+    calls = [lambda x, w: P.layer_norm(x, channel_dim=-1),
+             lambda x, w: P.linear(x, w, activation="gelu", channel_dim=-1),
+             lambda x, w: P.gated_linear(x, w, channel_dim=-1),
+             lambda x, w: P.rotary(x.view(1, 40, 1, 16), inv, axis, at)]
+    for call in calls:
+        want = torch.stack([call(x[k], w[k]) for k in range(3)])
+        assert torch.equal(torch.vmap(call)(x, w), want)
+        leaf = x.clone().requires_grad_(True)
+        g = _rand(gen, *want.shape)
+        got, = torch.autograd.grad(torch.vmap(call)(leaf, w), leaf, g)
+        for k in range(3):
+            one = x[k].clone().requires_grad_(True)
+            assert torch.equal(got[k], torch.autograd.grad(call(one, w[k]), one, g[k])[0])
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v, w[0]).sum())(x[0])
