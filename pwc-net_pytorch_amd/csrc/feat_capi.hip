@@ -57,7 +57,8 @@ struct Problem {
 const char* bad_problem(const Problem& p) {
   if (const char* e = bad_shape(p.layout, p.B, p.P, p.K, p.dtype)) return e;
   if (p.O <= 0 || p.O > (1 << 23)) return "bad number of output channels";
-  if (p.M > kIntMax) return "dimension too large";
+  // tokens are counted in 32 bits, up to the end of a tile, and of the tiles of a block's turn
+  if (p.M > kIntMax - 0xffff) return "dimension too large";
   if (p.act < 0 || p.act > kActGeluTanh) return "unknown activation";
   if (p.M > (1LL << 40) / p.rows || (long long)p.rows * p.K > (1LL << 40))
     return "dimension too large";

@@ -35,6 +35,7 @@
 // were no faster.  Few tokens are bound by the bytes of W (few_tokens), some hundred by latency.
 
 #include "feat_product.cuh"
+#include "feat_steps.cuh"
 
 namespace pwc {
 namespace feat {
@@ -113,7 +114,7 @@ ProductPlan product_plan(const ProductArgs& g, int dtype) {
                         : dtype == 0        ? kCostAnyK32
                                             : kCostAnyK16;
     const int ks = kStepBytes / (dtype == 0 ? 4 : 2);
-    const double steps = (double)g.segments * ((g.K + ks - 1) / ks);
+    const double steps = (double)g.segments * Steps::of(g.K, ks);
     const double tiles =
         (double)((ri + c.bi - 1) / c.bi) * ((rj + c.bj - 1) / c.bj) * g.batches;
     for (int splits = 1; splits <= (g.mode == kPartial || g.channel_i ? 512 : 1); splits *= 2) {

@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "feat_product.cuh"
+#include "feat_steps.cuh"
 
 namespace pwc {
 namespace feat {
@@ -137,7 +138,7 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
   typedef Tile<T, R, KC, NW> Tl;
   const T* base;      // of the tile's first row and this batch
   long long ld;
-  int K, limit;       // k in a segment; N: rows left of the tile's own dimension
+  int limit;          // N: rows left of the tile's own dimension
   uint32_t off[Tl::LOADS];  // DIRECT: bytes from base, or kOOB
   int at[Tl::LOADS];        // first k (K) or row k (N) of the chunk within the step
   long long row[DIRECT ? 1 : Tl::LOADS];
@@ -145,10 +146,8 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
   u32x4 reg[DIRECT ? 1 : Tl::LOADS];
 
   // `pair` > 0: rows alternate in groups of 16 between the halves of a matrix of 2 * pair rows
-  __device__ __forceinline__ void init(const T* b, long long ld_, int K_, int r0, int rows,
-                                       int pair) {
+  __device__ __forceinline__ void init(const T* b, long long ld_, int r0, int rows, int pair) {
     ld = ld_;
-    K = K_;
     base = KC ? b + (pair ? (long long)(r0 / 2) : (long long)r0) * ld : b + r0;
     limit = rows - r0;
 #pragma unroll
@@ -182,12 +181,13 @@ template <typename T, int R, bool KC, int NW, bool DIRECT> struct Loader {
     }
   }
 
-  // the step at k0 of the segment at `seg` values from base: where it lies, then its loads
+  // the step at k0 of the segment at `seg` values from base, which has `have` values of k: where it
+  // lies, then its loads
   const T* from;
   int left_k;
-  __device__ __forceinline__ void aim(long long seg, int k0) {
+  __device__ __forceinline__ void aim(long long seg, int k0, int have) {
     from = base + seg + (KC ? (long long)k0 : (long long)k0 * ld);
-    left_k = K - k0;
+    left_k = have;
   }
   __device__ __forceinline__ void load(char* lds, int n) {
     if constexpr (DIRECT) {
@@ -501,30 +501,20 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
 
   Loader<T, BI, AKC, NW, DIRECT> la;
   Loader<T, BJ, BKC, NW, DIRECT> lb;
-  la.init((const T*)g.a + batch * g.a_batch, g.lda, g.K, i0, g.I, kPair && CI ? g.pair : 0);
-  lb.init((const T*)g.b + batch * g.b_batch, g.ldb, g.K, j0, g.J, kPair && !CI ? g.pair : 0);
+  la.init((const T*)g.a + batch * g.a_batch, g.lda, i0, g.I, kPair && CI ? g.pair : 0);
+  lb.init((const T*)g.b + batch * g.b_batch, g.ldb, j0, g.J, kPair && !CI ? g.pair : 0);
 
   // steps of this block: all of K, or its share of the segments' steps
-  const int per_seg = (g.K + TA::KS - 1) / TA::KS;
-  const int total = g.segments * per_seg;
-  int s = 0, end = total;
-  if (PART) {
-    s = (int)((long long)total * z / g.splits);
-    end = (int)((long long)total * (z + 1) / g.splits);
-  }
-  // the step whose loads start next
-  int seg = s / per_seg, k0 = (s - seg * per_seg) * TA::KS, next = s;
+  Steps at_step;  // the one whose loads start next
+  at_step.init(g.segments, g.K, TA::KS, PART ? z : 0, PART ? g.splits : 1);
+  int s = 0;
+  const int end = at_step.left;
   auto aim = [&]() __attribute__((always_inline)) {
     // past the end every chunk is outside: zeros, without an access to memory
-    const int k = next < end ? k0 : 0x3fffffff;
-    la.aim((seg >> g.a_halves) * g.a_segment, k);
-    lb.aim(seg * g.b_segment, k);
-    ++next;
-    k0 += TA::KS;
-    if (k0 >= g.K) {
-      k0 = 0;
-      ++seg;
-    }
+    const int have = at_step.have(g.K);
+    la.aim((at_step.seg >> g.a_halves) * g.a_segment, at_step.k0, have);
+    lb.aim(at_step.seg * g.b_segment, at_step.k0, have);
+    at_step.next(g.K, TA::KS);
   };
   constexpr int LOADS = TA::LOADS + TB::LOADS;  // of a step
   auto start = [&](char* pa, char* pb) __attribute__((always_inline)) {

@@ -1,7 +1,13 @@
 """CPU: ways of calling the feature operators other than eagerly on plain tensors (no call here
 reaches a device), and what the entries ask for."""
+import ctypes
+import os
+import subprocess
+
 import pytest
 import torch
+
+from conftest import PKG
 
 
 # ------------------------------------------------------------------------------- torch.jit.trace
@@ -96,3 +102,62 @@ def test_forward_mode_is_refused_under_torch_func():
                                            (x,), (x,))):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 run()
+
+
+# ------------------------------------------------------------------------------- steps of k
+_WALK = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "feat_steps.cuh"
+// all blocks of one product: together they take every step once, and none past their ends
+static long long walk(int segments, int K, int KS, int splits) {
+  long long seen = 0;
+  int seg = 0, k0 = 0;
+  for (int z = 0; z < splits; ++z) {
+    pwc::feat::Steps s;
+    s.init(segments, K, KS, z, splits);
+    const int mine = s.left;
+    for (int n = 0; n < mine; ++n, s.next(K, KS)) {
+      if (s.seg != seg || s.k0 != k0 || s.have(K) != K - k0 || s.have(K) <= 0) return -1;
+      seen += s.have(K) < KS ? s.have(K) : KS;
+      if (K - k0 > KS) k0 += KS; else k0 = 0, ++seg;
+    }
+    for (int n = 0; n < 5; ++n, s.next(K, KS))
+      if (s.have(K) != 0) return -2;
+  }
+  return seg == segments && k0 == 0 ? seen : -3;
+}
+int main(int, char** v) { printf("%lld\n", walk(atoi(v[1]), atoi(v[2]), atoi(v[3]), atoi(v[4]))); }
+"""
+
+
+def test_steps_of_long_sums(tmp_path):
+    """The product's walk over k, compiled for the host: every value once, nothing past the end, and
+    no signed overflow (-ftrapv), up to the largest k that the entries take."""
+    (tmp_path / "walk.cpp").write_text(_WALK)
+    exe = str(tmp_path / "walk")
+    subprocess.run(["g++", "-O1", "-ftrapv", "-I", os.path.join(PKG, "csrc"), "-o", exe,
+                    str(tmp_path / "walk.cpp")], check=True)
+    most = 2 ** 31 - 2 ** 16
+    for segments, K, KS, splits in ((1, 1, 64, 1), (1, 64, 64, 1), (3, 65, 64, 1), (5, 1961, 64, 4),
+                                    (1, 100000, 32, 128), (7, 31, 32, 2), (1, 2 ** 30 - 1, 64, 512),
+                                    (1, 2 ** 30, 64, 512), (1, 2 ** 30 + 32, 64, 512),
+                                    (1, 2 ** 30 + 32, 32, 1), (1, most, 64, 3), (1, most, 32, 512),
+                                    (2 ** 24, 3, 64, 512)):
+        out = subprocess.run([exe, *map(str, (segments, K, KS, splits))], check=True,
+                             capture_output=True, text=True)
+        assert int(out.stdout) == segments * K, (segments, K, KS, splits, out.stdout)
+
+
+def test_token_counts_that_tiles_would_overflow_are_refused():
+    from pwcnet_amd import _lib
+    lib, p = _lib.load(), ctypes.c_void_p(64)
+    for M, text in ((2 ** 31 - 1, b"too large"), (2 ** 31 - 2 ** 16 + 1, b"too large"),
+                    (2 ** 31 - 2 ** 16, b"null")):
+        for layout in (0, 1):
+            assert lib.pwc_linear_forward(None, p, None, None, p, layout, 1, M, 1, 1, 2 ** 31, 0, 0.1,
+                                          2, None, 0, None) == 0
+            assert text in lib.pwc_last_error(), lib.pwc_last_error()
+            assert lib.pwc_gated_linear_backward(None, p, None, p, p, p, p, layout, 1, M, 1, 1,
+                                                 2 ** 31, 0, 0.1, 2, None, 0, None) == 0
+            assert text in lib.pwc_last_error(), lib.pwc_last_error()

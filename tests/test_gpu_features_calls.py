@@ -74,3 +74,25 @@ def test_vmap_gives_each_samples_values():
             assert torch.equal(got[k], torch.autograd.grad(call(one, w[k]), one, g[k])[0])
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda v: call(v, w[0]).sum())(x[0])
+
+
+# ------------------------------------------------------------------------------- long sums
+def test_weight_gradient_of_an_image_past_2_30():
+    """The weight gradient sums over an image's pixels: more than 2^30 of them, with the loads of the
+    steps past the last outside."""
+    from pwcnet_amd import features
+    P_ = 2 ** 30 + 32
+    x = torch.zeros(1, 2, P_, dtype=torch.bfloat16, device=DEV)
+    dy = torch.zeros(1, 3, P_, dtype=torch.bfloat16, device=DEV)
+    gen = _gen("long")
+    at = torch.cat((torch.randint(0, P_, (4000,), generator=gen), torch.arange(P_ - 300, P_),
+                    torch.arange(2 ** 30 - 70, 2 ** 30 + 3))).unique().to(DEV)
+    x[0, :, at] = _rand(gen, 2, at.numel(), dtype=torch.bfloat16)
+    dy[0, :, at] = _rand(gen, 3, at.numel(), dtype=torch.bfloat16)
+    w = _rand(gen, 3, 2, dtype=torch.bfloat16)
+    dw = features.linear_backward(x, w, None, dy, needs=(False, True, False))[1]
+    a, b = dy[0, :, at].double(), x[0, :, at].double()
+    ref = a @ b.t()
+    # fp32 sums of the values that are there (zeros add nothing), then one rounding
+    tol = at.numel() * 2.0 ** -24 * (a.abs() @ b.abs().t())
+    assert ((dw.double() - ref).abs() <= tol + u(torch.bfloat16) * (ref.abs() + tol)).all()
