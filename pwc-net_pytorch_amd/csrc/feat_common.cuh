@@ -182,13 +182,9 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
       if (FAST) {
         const float g = __builtin_amdgcn_exp2f(-0.7213475204444817f * z2);
         const float t = tail_f(z[e], g);
-        if constexpr (SLOPE) {
-          const float p = z[e] > 0.f ? 1.f - t : t;
-          f[e] = z[e] * p;
-          d[e] = p + z[e] * (0.3989422804014327f * g);
-        } else {
-          f[e] = fmaxf(z[e], 0.f) - fabsf(z[e]) * t;  // z Phi(z)
-        }
+        const float p = z[e] > 0.f ? 1.f - t : t;
+        f[e] = z[e] * p;
+        if constexpr (SLOPE) d[e] = p + z[e] * (0.3989422804014327f * g);
       } else {
         const float p = 0.5f * erfcf(-0.7071067811865476f * z[e]);
         f[e] = z[e] * p;

@@ -96,3 +96,56 @@ def test_weight_gradient_of_an_image_past_2_30():
     # fp32 sums of the values that are there (zeros add nothing), then one rounding
     tol = at.numel() * 2.0 ** -24 * (a.abs() @ b.abs().t())
     assert ((dw.double() - ref).abs() <= tol + u(torch.bfloat16) * (ref.abs() + tol)).all()
+
+
+# ------------------------------------------------------------------------------- activations
+ACTS = ["none", "relu", "leaky_relu", "sigmoid", "tanh", "silu", "gelu", "gelu_tanh"]
+
+
+def act64(z, name, slope=0.1):
+    """act(z) in 64 bits"""
+    if name == "relu":
+        return z.clamp_min(0)
+    if name == "leaky_relu":
+        return torch.where(z > 0, z, slope * z)
+    if name == "sigmoid":
+        return torch.sigmoid(z)
+    if name == "tanh":
+        return torch.tanh(z)
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "gelu":
+        return z * torch.special.ndtr(z)
+    if name == "gelu_tanh":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z
+
+
+# few tokens, tiles, parts of k, a map
+PATHS = [((3, 64), 24, -1), ((200, 64), 72, -1), ((100, 2048), 520, -1), ((2, 64, 9, 8), 40, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_of_what_is_no_number(act, dtype):
+    """Infinities and NaN, from the bias, through each activation on each path of the products: what
+    the formula gives (-inf * 0 is no number there either)."""
+    import pwcnet_amd as P
+    for shape, O, dim in PATHS:
+        x = _rand(_gen("no number", act), *shape, dtype=dtype)
+        at = torch.tensor([math.inf, -math.inf, math.nan, 0.5, -2.0])
+        b = at.repeat(O // 5 + 1)[:O].to(dtype).to(DEV)
+        w = torch.zeros(O, x.shape[dim], dtype=dtype, device=DEV)
+        want = act64(b.double(), act)
+        for y in (P.linear(x, w, b, None, act, 0.1, dim),
+                  P.gated_linear(x, torch.cat((w, w)), torch.cat((b, torch.ones_like(b))), act, 0.1,
+                                 dim)):
+            got = y.movedim(dim, -1).double()
+            full = want.expand_as(got)
+            whole = torch.isfinite(full)
+            # (2^-20 for the activation in 32 bits, then the output's rounding)
+            tol = u(dtype) * full.abs() + 2.0 ** -20
+            assert ((got - full).abs() <= tol)[whole].all(), (shape, act)
+            assert torch.equal(torch.isnan(got), torch.isnan(full)), (shape, act)
+            inf = torch.isinf(full)
+            assert torch.equal(got[inf], full[inf]), (shape, act)
