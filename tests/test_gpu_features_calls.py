@@ -149,3 +149,37 @@ def test_activations_of_what_is_no_number(act, dtype):
             assert torch.equal(torch.isnan(got), torch.isnan(full)), (shape, act)
             inf = torch.isinf(full)
             assert torch.equal(got[inf], full[inf]), (shape, act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_gelu_of_far_negative_values(dtype):
+    """gelu and its derivative where they fall below the type's step of 1: bounds relative to the
+    value itself.
+
+    The exponent of exp(-z^2 / 2) is rounded twice (2 z^2 / 2 2^-24 of the value: 2^-16 at -13), the
+    tail's polynomial is off by 1.1e-5, a few roundings of 2^-24 follow: 2^-14.5 covers them.  Below
+    the type's normal numbers half a step of the subnormal ones; and 32 bits' own (2^-149)."""
+    import pwcnet_amd as P
+    from pwcnet_amd import features
+    z = torch.linspace(-13, -3, 520).to(dtype).to(DEV)
+    zd = z.double()
+    y = zd * torch.exp(torch.special.log_ndtr(zd))
+    d = (torch.exp(torch.special.log_ndtr(zd))
+         + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi))
+    floor = torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2 + 2.0 ** -149
+    rel = 2.0 ** -14.5
+    for shape, O, dim in PATHS:
+        if O < 520:
+            b = z[::520 // O + 1]
+            at = slice(None, None, 520 // O + 1)
+        else:
+            b, at = z, slice(None)
+        x = _rand(_gen("far gelu"), *shape, dtype=dtype)
+        w = torch.zeros(b.numel(), x.shape[dim], dtype=dtype, device=DEV)
+        got = P.linear(x, w, b, activation="gelu", channel_dim=dim).movedim(dim, -1).double()
+        assert ((got - y[at]).abs() <= (u(dtype) + rel) * y[at].abs() + floor).all(), shape
+    # the bias gradient of one token is dz
+    one = torch.ones(1, 520, dtype=dtype, device=DEV)
+    w = torch.zeros(520, 8, dtype=dtype, device=DEV)
+    db = features.linear_backward(one[:, :8].contiguous(), w, z, one, "gelu", channel_dim=-1)[2]
+    assert ((db.double() - d).abs() <= (u(dtype) + rel) * d.abs() + floor).all()
