@@ -192,7 +192,7 @@ def _tokens(x, channel_dim):
 @torch.library.custom_op(f"{_NS}::layer_norm", mutates_args=())
 def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                channel_dim: int) -> Tuple[Tensor, Tensor, Tensor]:
-    """(y, mean, rstd)"""
+    """(y, mean, rstd); mean and rstd have no gradient."""
     return _features.layer_norm_forward(x, weight, bias, eps, channel_dim, True)
 
 
@@ -218,6 +218,7 @@ def _(x, weight, grad, mean, rstd, channel_dim):
 def _norm_setup(ctx, inputs, output):
     x, weight, bias, eps, ctx.channel_dim = inputs
     ctx.has = (weight is not None, bias is not None)
+    ctx.mark_non_differentiable(output[1], output[2])  # for the backward pass, and as they are
     ctx.save_for_backward(x, weight, output[1], output[2])
 
 

@@ -161,3 +161,22 @@ def test_token_counts_that_tiles_would_overflow_are_refused():
             assert lib.pwc_gated_linear_backward(None, p, None, p, p, p, p, layout, 1, M, 1, 1,
                                                  2 ** 31, 0, 0.1, 2, None, 0, None) == 0
             assert text in lib.pwc_last_error(), lib.pwc_last_error()
+
+
+# ------------------------------------------------------------------------------- the nodes
+def test_statistics_of_the_norm_node_have_no_gradient():
+    """A loss on them would get zeros: they do not ask for a gradient, compiled or not."""
+    x = torch.empty(4, 8, device="meta", requires_grad=True)
+    w = torch.empty(8, device="meta", requires_grad=True)
+
+    def call(x, w):
+        return torch.ops.pwcnet.layer_norm(x, w, None, 1e-5, -1)
+
+    for f in (call, torch.compile(call, backend="aot_eager", fullgraph=True)):
+        y, mean, rstd = f(x, w)
+        assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+        for loss in (mean.sum(), rstd.sum()):
+            with pytest.raises(RuntimeError, match="does not require grad"):
+                loss.backward()
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        assert dx.shape == x.shape and dw.shape == w.shape
