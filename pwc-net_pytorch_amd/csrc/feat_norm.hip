@@ -567,7 +567,9 @@ __global__ __launch_bounds__(256) void norm_any_dw(const NormArgs a, int parts) 
   }
 }
 
-// dw, db: the blocks' sums [2][blocks][C] in their order; 32 channels by 32 shares of the blocks
+// dw, db: the blocks' sums [2][blocks][C] in a fixed order; 32 channels by 32 shares of the blocks.
+// A share is eight sums, and they and the shares are joined in pairs, so a value goes through blocks /
+// 256 + 8 additions: one after the other, the rounding of 32-bit gradients would be the sum's.
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_add_parts(const float* __restrict__ part,
                                                        T* __restrict__ dw, T* __restrict__ db,
@@ -576,18 +578,25 @@ __global__ __launch_bounds__(1024) void norm_add_parts(const float* __restrict__
   const int l = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + l;
   const float* p = part + (long long)blockIdx.y * blocks * C;
-  float s = 0.f;
+  float s[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[k] = 0.f;
   if (c < C) {
-#pragma unroll 8
-    for (int b = g; b < blocks; b += 32) s += p[(long long)b * C + c];
+    int b = g;
+    for (; b + 32 * 7 < blocks; b += 256)  // (whole rounds: eight loads under way)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] += p[(long long)(b + 32 * k) * C + c];
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+      if (b + 32 * k < blocks) s[k] += p[(long long)(b + 32 * k) * C + c];
   }
-  red[g][l] = s;
+  red[g][l] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
-  if (g == 0 && c < C) {
-    for (int k = 1; k < 32; ++k) s += red[k][l];
-    T* out = blockIdx.y == 0 ? dw : db;
-    if (out) out[c] = narrow<T>(s);
-  }
+  // half a wave a channel: lane l has share l of channel g
+  const float v = lanes_sum<32>(red[l][g]);
+  const int at = blockIdx.x * 32 + g;
+  T* out = blockIdx.y == 0 ? dw : db;
+  if (l == 0 && at < C && out) out[at] = narrow<T>(v);
 }
 
 // ------------------------------------------------------------------------------ launches

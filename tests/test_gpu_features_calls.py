@@ -183,3 +183,27 @@ def test_gelu_of_far_negative_values(dtype):
     w = torch.zeros(520, 8, dtype=dtype, device=DEV)
     db = features.linear_backward(one[:, :8].contiguous(), w, z, one, "gelu", channel_dim=-1)[2]
     assert ((db.double() - d).abs() <= (u(dtype) + rel) * d.abs() + floor).all()
+
+
+# ------------------------------------------------------------------------------- layer norm
+@pytest.mark.parametrize("shape,dim", [((8, 32, 96, 112), 1), ((8, 20, 96, 101), 1), ((86016, 64), -1),
+                                       ((3000, 2048), -1)])
+def test_sums_over_blocks_in_pairs(shape, dim):
+    """The bias gradient of 2^24 in the first row and 1 in every 64th, which additions one after the
+    other to the large one would lose.
+
+    At most 8 values of a block's own, 6 levels of its lanes, 2048 / 256 rounds and 8 levels of the
+    blocks' sums follow one another, each off by at most 2^-24 of the total."""
+    import pwcnet_amd as P
+    dy = torch.zeros(shape, device=DEV)
+    flat = dy.movedim(dim, -1)
+    C, M = flat.shape[-1], flat.numel() // flat.shape[-1]
+    n = torch.arange(M, device=DEV)
+    one = torch.where(n % 64 == 0, 1.0, 0.0)
+    one[0] = 2.0 ** 24
+    flat.copy_(one.view(*flat.shape[:-1], 1).expand_as(flat))
+    x = _rand(_gen("pairs", shape), *shape)
+    b = torch.zeros(C, device=DEV, requires_grad=True)
+    got, = torch.autograd.grad(P.layer_norm(x, None, b, channel_dim=dim), b, dy)
+    want = one.double().sum()
+    assert ((got.double() - want).abs() <= 30 * 2.0 ** -24 * want).all()
