@@ -627,16 +627,19 @@ template <typename T> static bool vector_rows(const NormArgs& a) {
 // the l4 map's 1344 tiles took two turns and twice the time).
 constexpr int kBlocksTokens = 1024, kBlocksMaps = 2048;
 
+// maps whose pixels' channels are held in registers
+static bool map_held(long long P, int C) { return C <= 256 && C * P < 1LL << 30; }
+
 int norm_parts(int layout, long long B, long long P, int C, int dtype) {
   const long long M = layout == kMap ? B * P : P;
-  long long rows = 1;  // rows of a block's turn
-  if (layout == kMap) {
-    rows = 64;
-  } else {
-    const int V = dtype == 0 ? 4 : 8;
-    const RowPlan p = row_plan(C, V);
-    if (p.tpr) rows = 256 / p.tpr;
+  const RowPlan p = layout == kMap ? RowPlan{} : row_plan(C, dtype == 0 ? 4 : 8);
+  if (layout == kMap ? !map_held(P, C) : !p.tpr) {
+    // norm_any_dw's blocks have a channel or some, and share the rows: thousands (maps) or dozens each
+    const long long n = M / (layout == kMap ? 4096 : 32) + 1;
+    const long long most = layout == kMap ? kBlocksMaps : kBlocksTokens;
+    return (int)(M == 0 ? 0 : n < most ? n : most);
   }
+  const long long rows = layout == kMap ? 64 : 256 / p.tpr;  // of a block's turn
   const long long n = (M + rows - 1) / rows;
   long long most = layout == kMap ? kBlocksMaps : kBlocksTokens;
   if (layout == kTokens && rows == 1 && n / 8 < most) most = n / 8 > 256 ? n / 8 : 256;
@@ -695,7 +698,7 @@ static void map_pv(const NormArgs& a, bool back, int parts, hipStream_t s) {
 #undef NORM_MAP
 }
 template <typename T> static bool map(const NormArgs& a, bool back, int parts, hipStream_t s) {
-  if (a.C > 256 || a.C * a.P >= 1LL << 30) return false;
+  if (!map_held(a.P, a.C)) return false;
   if constexpr (sizeof(T) == 2) {
     bool pairs = (a.C <= 128 || !back) && a.P % 2 == 0 && (a.B == 1 || a.x_stride % 2 == 0);
     for (const void* p : {a.x, a.dy, (const void*)a.y, (const void*)a.dx})
@@ -738,12 +741,8 @@ template <typename T> static hipError_t forward_t(const NormArgs& a, hipStream_t
 }
 
 template <typename T> static hipError_t backward_t(const NormArgs& a, int parts, hipStream_t s) {
-  if (!(a.layout == kMap ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s))) {
-    // these blocks have a channel or some, and share the rows: thousands (maps) or dozens each
-    const long long most = a.M / (a.layout == kMap ? 4096 : 32) + 1;
-    if (parts > most) parts = (int)most;
+  if (!(a.layout == kMap ? map<T>(a, true, parts, s) : tokens<T>(a, true, parts, s)))
     any_c<T>(a, true, parts, s);
-  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.part) return e;
   norm_add_parts<T><<<dim3((a.C + 31) / 32, 2), 1024, 0, s>>>(a.part, (T*)a.dw, (T*)a.db, a.C,

@@ -180,3 +180,16 @@ def test_statistics_of_the_norm_node_have_no_gradient():
                 loss.backward()
         dx, dw = torch.autograd.grad(y.sum(), (x, w))
         assert dx.shape == x.shape and dw.shape == w.shape
+
+
+# ------------------------------------------------------------------------------- workspaces
+def test_norm_workspace_of_long_rows():
+    """Partial sums of rows that no registers hold: as many as the kernel writes, a share of x."""
+    from pwcnet_amd import _lib
+    size = _lib.load().pwc_layer_norm_backward_workspace_size
+    for M, C in ((1, 9000), (300, 9216), (20, 2 ** 20), (16384, 9216), (16384, 2 ** 20)):
+        # [2][parts][C] in 32 bits, 32 rows at least to a part (and one part)
+        assert 0 < size(1, 1, M, C, 2) <= 2 * (M // 32 + 1) * C * 4 + 255
+    for B, P, C in ((1, 50, 300), (2, 5000, 2 ** 16), (16, 7168, 257)):
+        assert 0 < size(0, B, P, C, 0) <= 2 * (B * P // 4096 + 1) * C * 4 + 255
+    assert size(1, 1, 0, 9216, 2) == 0 and size(0, 3, 0, 300, 0) == 0
