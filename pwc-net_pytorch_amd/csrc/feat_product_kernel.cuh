@@ -35,7 +35,9 @@ __device__ __forceinline__ f32x4 mma(const s16x8& a, const s16x8& b, f32x4 c, __
 }
 // The same with the sums pinned to the accumulation registers: left to itself the compiler moves
 // a 256 x 256 tile's sums between the two register files, 350 moves a step.  Nothing but these
-// instructions touches the sums until the waits behind the loop have let the last of them finish.
+// instructions touches the sums until the waits behind the loop have let the last of them finish, and
+// no operand is written right before one: the compiler keeps no wait states for inline asm, so the
+// build looks at what it made (check_pinned.py).
 __device__ __forceinline__ void mma_pinned(const s16x8& a, const s16x8& b, f32x4& c, __half) {
   asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
