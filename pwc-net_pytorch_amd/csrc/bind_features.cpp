@@ -558,6 +558,8 @@ Tensor rotary(const Tensor& x, const Tensor& inv_freq, const Tensor& axis,
               bool interleaved) {
   TORCH_CHECK_VALUE(!positions.has_value() || !positions->requires_grad(),
                     "rotary: positions have no gradient");
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !inv_freq.requires_grad(),
+                    "rotary: inv_freq has no gradient");
   if (wants_grad({&x}))
     return RotaryFunction::apply(x, inv_freq, axis, positions, grid, origin, interleaved);
   return rotary_forward(x, inv_freq, axis, some(positions), grid, origin, interleaved, false);

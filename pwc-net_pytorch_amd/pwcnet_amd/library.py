@@ -246,6 +246,8 @@ def _(x, inv_freq, axis, positions, grid, origin, interleaved, inverse):
 
 def _rotary_setup(ctx, inputs, output):
     x, inv_freq, axis, positions, *ctx.args = inputs
+    if any(ctx.needs_input_grad[1:4]):
+        raise ValueError("rotary: positions and inv_freq have no gradient")
     ctx.save_for_backward(inv_freq, axis, positions)
 
 

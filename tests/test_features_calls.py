@@ -193,3 +193,23 @@ def test_norm_workspace_of_long_rows():
     for B, P, C in ((1, 50, 300), (2, 5000, 2 ** 16), (16, 7168, 257)):
         assert 0 < size(0, B, P, C, 0) <= 2 * (B * P // 4096 + 1) * C * 4 + 255
     assert size(1, 1, 0, 9216, 2) == 0 and size(0, 3, 0, 300, 0) == 0
+
+
+# ------------------------------------------------------------------------------- rotary
+def test_rotary_refuses_what_it_has_no_gradient_for():
+    """Frequencies and positions that ask for a gradient are refused, not left without one: by the
+    function, by the node and compiled."""
+    import pwcnet_amd as P
+    f, a = P.rotary_frequencies((4,))
+    x, at = torch.zeros(1, 5, 2, 8), torch.zeros(5, 1)
+    ops = torch.ops.pwcnet
+    for freq, places in ((f.clone().requires_grad_(True), at), (f, at.clone().requires_grad_(True))):
+        with pytest.raises(ValueError, match="no gradient"):
+            P.rotary(x, freq, a, places)
+        meta = [t.detach().to("meta").requires_grad_(t.requires_grad) for t in (x, freq, a, places)]
+        with pytest.raises(ValueError, match="no gradient"):
+            ops.rotary(*meta, None, None, False, False)
+        with pytest.raises(Exception, match="no gradient"):
+            torch.compile(lambda *v: P.rotary(*v), backend="aot_eager")(*meta)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="HIP"):  # asks for none: as ever
+        P.rotary(x, f.clone().requires_grad_(True), a, at)
