@@ -270,7 +270,10 @@ Tensor rotary_forward(const Tensor& x, const Tensor& inv_freq, const Tensor& axi
   const char* what = "rotary";
   check(what, x, {});
   for (const Tensor* t : {&inv_freq, &axis, &positions})
-    if (t->defined()) plain(what, *t);
+    if (t->defined()) {
+      plain(what, *t);
+      TORCH_CHECK_TYPE(!t->is_neg(), what, ": negated views are not read: resolve_neg() first");
+    }
   TORCH_CHECK_VALUE(x.dim() == 4, what, ": expected [B, N, heads, D], got shape ", x.sizes());
   TORCH_CHECK_TYPE(inv_freq.scalar_type() == at::kDouble && axis.scalar_type() == at::kInt, what,
                    ": inv_freq is fp64 and axis int32, got ", inv_freq.scalar_type(), " and ",

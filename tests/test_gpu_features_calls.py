@@ -207,3 +207,19 @@ def test_sums_over_blocks_in_pairs(shape, dim):
     got, = torch.autograd.grad(P.layer_norm(x, None, b, channel_dim=dim), b, dy)
     want = one.double().sum()
     assert ((got.double() - want).abs() <= 30 * 2.0 ** -24 * want).all()
+
+
+# ------------------------------------------------------------------------------- rotary
+def test_rotary_refuses_negated_places():
+    """Lazily negated positions and frequencies are refused, not read with the wrong sign."""
+    import pwcnet_amd as P
+    f, a = P.rotary_frequencies((4,), device=DEV)
+    x = torch.zeros(1, 5, 2, 8, device=DEV)
+    at = torch.ones(5, 1, device=DEV)
+    neg_at = torch.conj(torch.complex(at, at)).imag
+    neg_f = torch.conj(torch.complex(f, f)).imag
+    assert neg_at.is_neg() and neg_f.is_neg()
+    for freq, places in ((f, neg_at), (neg_f, at)):
+        with pytest.raises(TypeError, match="negated"):
+            P.rotary(x, freq, a, places)
+    assert P.rotary(x, neg_f.resolve_neg(), a, neg_at.resolve_neg()).shape == x.shape
