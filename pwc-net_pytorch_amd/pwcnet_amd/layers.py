@@ -254,6 +254,9 @@ class RotaryPosition(nn.Module):
 
     def forward(self, x, positions=None, origin=None):
         if self.channel_dim == -1:
+            if origin is not None:
+                raise ValueError("RotaryPosition: tokens stand at their positions; origin belongs "
+                                 "to maps")
             return rotary(x, self.inv_freq, self.axis, positions, interleaved=self.interleaved)
         spatial, axes = tuple(x.shape[2:]), len(self.sections)
         if x.dim() < 3 or len(spatial) > axes or x.shape[1] % self.heads:

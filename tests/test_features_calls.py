@@ -213,3 +213,16 @@ def test_rotary_refuses_what_it_has_no_gradient_for():
             torch.compile(lambda *v: P.rotary(*v), backend="aot_eager")(*meta)
     with torch.no_grad(), pytest.raises(RuntimeError, match="HIP"):  # asks for none: as ever
         P.rotary(x, f.clone().requires_grad_(True), a, at)
+
+
+def test_rotary_position_of_tokens_refuses_an_origin():
+    """It was dropped; maps refuse it beside positions too."""
+    import pwcnet_amd as P
+    at = torch.zeros(5, 1, device="meta")
+    m = P.RotaryPosition((4,), channel_dim=-1).to("meta")
+    x = torch.empty(1, 5, 2, 8, device="meta")
+    for places in (at, None):
+        with pytest.raises(ValueError, match="origin"):
+            m(x, places, origin=(3,))
+    with pytest.raises(ValueError, match="origin"):
+        m(x, origin=(0,))
