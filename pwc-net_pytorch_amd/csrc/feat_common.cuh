@@ -203,7 +203,8 @@ __device__ __forceinline__ void activate(int act, const float (&z)[N], float (&f
   } else if (act == kActGeluTanh) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float q = z[e] * z[e];
+      // (from 100 on p is 0 or 1 whatever z^2 is; as infinity it would make 0 * inf of the slope)
+      const float q = fminf(z[e] * z[e], 1e4f);
       const float p = sigmoid_f<FAST>(2.f * kSqrt2OverPi * (z[e] + 0.044715f * z[e] * q));
       f[e] = z[e] * p;
       if (SLOPE) d[e] = p + f[e] * (1.f - p) * 2.f * kSqrt2OverPi * (1.f + 0.134145f * q);

@@ -223,3 +223,31 @@ def test_rotary_refuses_negated_places():
         with pytest.raises(TypeError, match="negated"):
             P.rotary(x, freq, a, places)
     assert P.rotary(x, neg_f.resolve_neg(), a, neg_at.resolve_neg()).shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_of_large_values(act, dtype):
+    """Values up to the type's largest, whose squares and cubes are beyond 32 bits: the activation and
+    its slope are finite wherever the formula's are.  (One rounding, 2^-20 for the functions.)"""
+    import pwcnet_amd as P
+    from pwcnet_amd import features
+    most = torch.finfo(dtype).max
+    at = [v for v in (30.0, 120.0, 6e4, 1e13, 1e19, 1e25, 3e38) if v <= most] + [most]
+    z = torch.tensor([s * v for v in at for s in (1, -1)]).to(dtype).to(DEV)
+    zd = z.double().requires_grad_(True)
+    # (the cube and tanh's argument fit 64 bits)
+    want = act64(zd, act)
+    slope, = torch.autograd.grad(want.sum(), zd)
+    if act in ("silu", "gelu", "gelu_tanh"):  # 0 * z of 64-bit autograd aside: 1 or 0 from 120 on
+        slope = torch.where(zd.abs() >= 100, (zd > 0).double(), slope)
+    want = want.detach()
+    O = z.numel()
+    w = torch.zeros(O, 8, dtype=dtype, device=DEV)
+    for M in (1, 128):
+        x = torch.ones(M, 8, dtype=dtype, device=DEV)
+        y = P.linear(x, w, z, None, act, 0.1, -1).double()
+        assert ((y - want).abs() <= u(dtype) * want.abs() + 2.0 ** -20).all(), (act, y)
+        dy = torch.full((M, O), 1 / M, dtype=dtype, device=DEV)
+        db = features.linear_backward(x, w, z, dy, act, 0.1, -1)[2].double()
+        assert ((db - slope).abs() <= 2 * u(dtype) * slope.abs() + 2.0 ** -20).all(), (act, db)
