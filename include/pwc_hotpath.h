@@ -372,8 +372,11 @@ PWC_API int pwc_linear_forward(const void* x, const void* weight, const void* bi
                                size_t workspace_bytes, void* stream);
 /* grad_x, grad_weight, grad_bias (each may be NULL: not computed).  The residual's gradient is
  * grad_out itself.  Deterministic.  The size is that of all three.  With an activation, the
- * gradient of the sums is kept in `dtype` between the products, in small 16-bit calls as a value and
- * what its rounding took; where x or weight is infinite a gradient is infinite or NaN. */
+ * gradient of the sums is kept in `dtype` between the products: in small 16-bit calls (at most 0.5
+ * GFLOP a product, by the kernels of small tiles) as a value and what its rounding took, in others as a
+ * value alone, which makes the error of the gradients 1.4 times that of their own rounding.  In fp16 it is infinite beyond 65504
+ * and nothing below 2^-25, as it is between the layers of an fp16 program: scale the loss.  Where x or
+ * weight is infinite a gradient is infinite or NaN. */
 PWC_API size_t pwc_linear_backward_workspace_size(const void* x, const void* weight,
                                                   const void* grad_out, int layout, long long B,
                                                   long long P, int K, int O, long long x_stride,

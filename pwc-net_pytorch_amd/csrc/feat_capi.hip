@@ -95,7 +95,15 @@ View dz_view(const Problem& p, const void* dz) {
   return {dz, p.P, p.rows * p.P, 0};
 }
 
-constexpr double kKeepLow = 5e8;  // operations of a product whose dz is kept in two parts
+// Operations of a product up to which a 16-bit dz is kept in two parts.  Rounded once it makes the
+// gradients' error 1.4 times that of their own rounding (bf16 2-norms 0.0024 against 0.0017; the two
+// parts 0.0017), as in a program that keeps it between its layers.  The second part is a second
+// product of each gradient: up to here 2 to 12 us of a backward pass of 14 to 35 (us, one part / two:
+// 64 x 96 -> 96 13.5 / 15.1, 256 x 512 -> 512 20 / 26, 8 x 96 x 24 x 28 -> 96 16 / 17), which hide
+// behind the 45 us that autograd takes for the call; from there on it shows and doubles what bounds
+// the call (1024 x 512 -> 512 gated, 1.1 GFLOP, 31 / 46; 1024 x 1024 -> 4096, 8.6, 62 / 81).  So a
+// token's gradients in a large batch have one rounding more than in a small one.
+constexpr double kKeepLow = 5e8;
 
 // The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
 // not, large ones are laid out so first.  Forward alone that is worth its launch from some GFLOP on
@@ -263,9 +271,7 @@ BackwardSpace backward_space(const Problem& p, const void* x, const void* w, con
   if (s.pad_w) s.wv = padded_w(p, nullptr);
   const ProductPlan dz_plan =
       z ? product_plan(dz_args(p, s.xv, s.wv, nullptr, nullptr, s.dzv), p.dtype) : ProductPlan();
-  // dz in 16 bits is rounded once, which makes the gradients' error 1.4 times that of their own
-  // rounding; in small calls, where chance adds to that, what the rounding took follows as more k,
-  // at a cost that the launches hide.  (Only the kernels of such calls can write it.)
+  // (only the kernels of small calls can write what dz's rounding took, which follows as more k)
   if (z && p.dtype != 0 && 2.0 * (double)p.M * p.rows * p.K <= kKeepLow &&
       (dz_plan.kernel <= kTile64Any || dz_plan.splits > 1))
     s.low = (tokens(p) ? p.M : p.rows) * (s.pad_dz ? whole(p, dz_cols(p)) : dz_cols(p));

@@ -193,7 +193,8 @@ def rotary(x, inv_freq, axis, positions=None, grid=None, origin=None, interleave
 def linear(x, weight, bias=None, residual=None, activation="none", negative_slope=0.1,
            channel_dim=1):
     """act(x W^T + bias) + residual over x's channels: on maps a 1x1 convolution with its
-    activation and skip in one kernel.  ``activation``: one of ``features.ACTIVATIONS``."""
+    activation and skip in one kernel.  ``activation``: one of ``features.ACTIVATIONS``.  How the
+    16-bit backward pass rounds: ``features.linear_backward``."""
     activation = activation or "none"
     if _traced(x, weight, bias, residual):
         return _library.linear(x, weight, bias, residual, activation, negative_slope, channel_dim)
@@ -203,7 +204,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", negative_slop
 
 def gated_linear(x, weight, bias=None, activation="silu", negative_slope=0.1, channel_dim=1):
     """act(x Wg^T + bg) * (x Wu^T + bu) over x's channels, weight = [Wg; Wu]: both projections,
-    the activation and the product in one kernel."""
+    the activation and the product in one kernel.  How the 16-bit backward pass rounds:
+    ``features.linear_backward``."""
     activation = activation or "none"
     if _traced(x, weight, bias):
         return _library.gated_linear(x, weight, bias, activation, negative_slope, channel_dim)
