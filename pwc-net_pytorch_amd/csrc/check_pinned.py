@@ -10,7 +10,7 @@ kernel that has such instructions, in the text that was built:
     across a loop's end (the hardware wants 2; loads are waited for by count, which the compiler
     does for inline asm too);
   * the sums' first values are written 4 wait states before the first, and the sums are read 19
-    after the last (16 passes want that many, these have 8).
+    after the last (the longest matrix instructions want that many, these fewer).
 
     check_pinned.py FILE.s KERNELS     exit status 1 unless FILE.s has KERNELS of them, all clean
 """

@@ -27,10 +27,10 @@
 // 16x16x4 instructions).  The order of k within a fragment does not matter as long as both
 // operands share it; N tiles of 16 bits are turned by the transposing LDS read.
 //
-// What bounds them (bf16, 8192 x K -> 4096): the matrix units in the steps, 1500 TFLOP/s by 256-tiles
-// against a library product's 1420, and the memory at a tile's end, where a CU writes 128 KiB and
-// nothing multiplies: 31 us of the 73 at K = 1024 with nothing else to do there, 84 with gelu, 101
-// and more where the operands come from memory.  Tiles of half that size would overlap the two, and
+// What bounds them (bf16, 8192 x K -> 4096): the matrix units in the steps, 1520 to 1565 TFLOP/s by
+// 256-tiles between K = 512 and 8192 (the largest library product, 8192^3, has 1583), and the memory at
+// a tile's end, where a CU writes 128 KiB and nothing multiplies: 34 us of the 79 at K = 1024 (a library
+// product 59) with nothing else to do there, 105 with gelu where the operands come from memory.  Tiles of half that size would overlap the two, and
 // lose more in the steps; a tile's sums stored from the registers, without the turn through LDS,
 // were no faster.  Few tokens are bound by the bytes of W (few_tokens), some hundred by latency.
 

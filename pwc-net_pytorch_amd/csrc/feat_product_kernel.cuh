@@ -653,7 +653,8 @@ __global__ __launch_bounds__(NWI* NWJ * 64, BI* BJ > 128 * 128 ? 1 : 2)
       qb = t;
     }
   }
-  // the last matrix instructions, 8 passes of 4 cycles, before their sums are read
+  // the last matrix instructions (16 cycles each by the counters) before their sums are read: any
+  // instruction of the matrix unit would be done
   if constexpr (kPinned) {
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
     pin();

@@ -8,7 +8,7 @@
 // whole turn before it is rounded to 32: at position 40000 the angle of the first pair keeps
 // 2^-24 of a turn, where a product in 32 bits has lost 2^-9.  Its sine and cosine serve all heads
 // (tokens) or all images with the same positions (maps).  Measured: 2 x 9603 x 24 x 128 bf16 tokens
-// 54 us (4.4 TB/s; a 1 GiB copy does 5.1), the 16 x 32 x 112 x 256 fp16 map 15.3 us (3.8).
+// 54 us (4.4 TB/s; a 1 GiB copy does 5.2), the 16 x 32 x 112 x 256 fp16 map 15.3 us (3.8).
 #include "feat_common.cuh"
 #include "feat_rotary.cuh"
 
