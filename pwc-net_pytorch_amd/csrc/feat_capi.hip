@@ -107,12 +107,12 @@ constexpr double kKeepLow = 5e8;
 
 // The products load directly (memory to LDS) from rows at 16-byte places.  Where a call's rows are
 // not, large ones are laid out so first.  Forward alone that is worth its launch from some GFLOP on
-// (us, as they lie / laid out first; 16 bits: 2047 x 1023 -> 1023, 4.3 GFLOP: 19 / 25; 8191 x 1023 ->
-// 4095: 164 / 103).  Backward the three products share the copies, and rows of odd 16-bit lengths
-// that are read across k cost most (with an activation: 1001 x 511 -> 511: 56 / 38, 2047 x 1023 ->
-// 1023: 137 / 65; without: 301 x 511 -> 511: 43 / 29; map 5 x 96 x 37 x 53 -> 385 gated: 62 / 55;
-// fp32 2001 x 701 -> 1001: 160 / 130), unless so few channels meet that the products are all traffic
-// anyway (map 16 x 64 x 113 x 129 -> 64: 81 / 88, fp32 136 / 155).
+// (us, as they lie / laid out first; bf16: 2047 x 1023 -> 1023, 4.3 GFLOP: 20 / 22; 4095 x 1023 ->
+// 1023, 8.6: 31 / 29; 8191 x 1023 -> 4095: 216 / 91).  Backward the three products share the copies,
+// and rows of odd 16-bit lengths that are read across k cost most (with an activation: 1001 x 511 ->
+// 511: 52 / 34, fp16 2047 x 1023 -> 1023: 136 / 54; without: 301 x 511 -> 511: 44 / 22; map 5 x 96 x 37
+// x 53 -> 385 gated: 57 / 48; fp32 2001 x 701 -> 1001: 128 / 121), unless so few channels meet that the
+// products are all traffic anyway (map 16 x 64 x 113 x 129 -> 64: 79 / 83, fp32 127 / 144).
 bool pads_pay(const Problem& p, bool backward) {
   const double operations = 2.0 * (double)p.M * p.rows * p.K;
   if (!backward) return operations >= 8e9;

@@ -401,8 +401,8 @@ __global__ __launch_bounds__(64 * G) void norm_map_backward(const NormArgs a) {
 // ------------------------------------------------------------------------------ any C
 // Rows longer than the registers are read again for each pass, mostly from the caches, and bound by
 // those reads: S threads share a row -- a whole block, V channels each (tokens), or 16 that have one
-// of 64 pixels (maps) -- with several loads under way.  16384 x 9000 bf16 tokens: 161 us forward (3.7
-// TB/s of what one read and one write are), 362 backward; the 8 x 300 x 2688 bf16 map 17 and 35.
+// of 64 pixels (maps) -- with several loads under way.  16384 x 9000 bf16 tokens: 156 us forward (3.8
+// TB/s of what one read and one write are), 242 backward; the 8 x 300 x 2688 bf16 map 16 and 34.
 struct RowAt {
   long long base, y, stride;  // first value in x, in y / dy / dx; between channels
   long long m;
